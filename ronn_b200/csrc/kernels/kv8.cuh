@@ -1,0 +1,130 @@
+// 8-bit paged KV cache: codes, scales and their conversions.
+//
+// Codes of K and of V: [num_blocks, kv_heads, 16, head_dim] bytes, int8 (-127 .. 127) or e4m3; one fp32 scale for each
+// (block, kv_head), K and V apart, always a power of two:
+//     s = 2^e,  e the least integer >= -100 with amax * 2^-e <= 127 (int8) or 448 (e4m3);   value = code * s.
+// A power of two costs at most one bit of int8 (none of e4m3, which carries its own exponent) and makes every step but the
+// one rounding exact: x / s, code * s, and the change of scale when a larger token joins a block.  The codes are then a
+// function of the block's tokens and not of the order of arithmetic, the same whether a prompt came in one call or many,
+// as long as the scale does not change under a token (then that token is rounded once more, to the coarser step).
+//   * Writing slot 0 begins a block: its scale starts from that call's tokens alone.  Otherwise s = max(old, new), and the
+//     codes of the slots below the call's first one are rounded again when s grew.  Slots above its last one keep their bytes.
+//   * A token with a value that is not finite makes the scale NaN until the block begins again: a query that sees any token
+//     of that block and head reads NaN.  Codes themselves are always finite, so masked slots never spread one.
+#pragma once
+#include "common.cuh"
+
+namespace ronn {
+
+constexpr int KV8_BLOCK = 16;
+constexpr uint32_t STATUS_KV8_PAGE = 0x5801;    // a block table, slot or table-row index outside the cache: not accessed
+
+enum Kv8Code { KV8_INT8 = 0, KV8_E4M3 = 1 };
+
+__device__ __forceinline__ void kv8_report(uint32_t* status) {
+  if (status) atomicCAS(status, 0u, STATUS_KV8_PAGE);
+}
+
+// Scale of a block whose largest magnitude has the bits `amax` (of a finite float >= 0).
+template <int CODE>
+__device__ __forceinline__ float kv8_least_scale(uint32_t amax) {
+  // 127 = 1.984375 * 2^6, 448 = 1.75 * 2^8: one more when the significand is above the limit's
+  const int top = CODE == KV8_INT8 ? 6 : 8;
+  const uint32_t frac = CODE == KV8_INT8 ? 0x7E0000u : 0x600000u;
+  int e = int(amax >> 23) - 127 - top + ((amax & 0x7fffffu) > frac ? 1 : 0);
+  e = max(e, -100);
+  return __uint_as_float(uint32_t(e + 127) << 23);
+}
+
+// 1 / s for a scale made above (a power of two between 2^-100 and 2^122); 0 for 0 (a block never written) and for NaN.
+__device__ __forceinline__ float kv8_inverse(float s) {
+  const uint32_t ex = __float_as_uint(s) >> 23;
+  return ex == 0 || ex >= 254 ? 0.f : __uint_as_float((254u - ex) << 23);
+}
+
+// Four values (already divided by the scale) to four codes, round to nearest even.
+template <int CODE>
+__device__ __forceinline__ uint32_t kv8_pack4(float a, float b, float c, float d) {
+  if constexpr (CODE == KV8_INT8) {
+    // |x| <= 127: adding 1.5 * 2^23 rounds to an integer that stands in the low bits
+    const float magic = 12582912.f;
+    const uint32_t x = __float_as_uint(a + magic), y = __float_as_uint(b + magic);
+    const uint32_t z = __float_as_uint(c + magic), w = __float_as_uint(d + magic);
+    return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+  } else {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return uint32_t(lo) | (uint32_t(hi) << 16);
+  }
+}
+
+// Two codes in the low 16 bits of w -> two floats.
+template <int CODE>
+__device__ __forceinline__ float2 kv8_unpack2(uint32_t w) {
+  if constexpr (CODE == KV8_INT8) {
+    return make_float2(float(int(int8_t(w & 0xff))), float(int(int8_t((w >> 8) & 0xff))));
+  } else {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(w)));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+  }
+}
+template <int CODE>
+__device__ __forceinline__ void kv8_unpack4(uint32_t w, float (&f)[4]) {
+  const float2 a = kv8_unpack2<CODE>(w), b = kv8_unpack2<CODE>(w >> 16);
+  f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+}
+
+// Rotary embedding: the angle of pair j at position p is p * base^(-2j/d).  `turns[j]` is base^(-2j/d) / (2 pi) as a
+// 64-bit binary fraction, so p * turns[j] modulo 2^64 is the angle's fraction of a turn, exact to 2^-44 at p = 2^20 (a
+// 32-bit angle is off by 0.004 rad at p = 65536).  Sine and cosine are taken in 64 bits and the rotated value is rounded
+// to 32 bits and then to the activations' type, as a 64-bit tensor is converted: a value next to a rounding border then
+// falls on the same side wherever it is computed.
+constexpr int KV8_MAX_HALF = 64;
+struct Kv8Turns {
+  unsigned long long t[KV8_MAX_HALF];
+};
+__device__ __forceinline__ double2 kv8_cos_sin(unsigned long long turn, int pos) {
+  const unsigned long long f = turn * (unsigned long long)(long long)pos;
+  double s, c;
+  sincospi(double((long long)f) * 1.0842021724855044e-19, &s, &c);       // 2^-63: half turns in [-1, 1)
+  return make_double2(c, s);
+}
+template <class T> __device__ __forceinline__ T kv8_round16(double v);
+template <> __device__ __forceinline__ __half kv8_round16<__half>(double v) { return __float2half_rn(__double2float_rn(v)); }
+template <> __device__ __forceinline__ __nv_bfloat16 kv8_round16<__nv_bfloat16>(double v) { return __float2bfloat16_rn(__double2float_rn(v)); }
+
+// Eight rotated values: `own` the chunk, `oth` the chunk half a head away, `low` whether own is in the first half.
+template <class T>
+__device__ __forceinline__ Vec8 kv8_rotate8(const Vec8& own, const Vec8& oth, bool low, const double2* cs) {
+  float a[8], b[8];
+  unpack8<T>(own, a);
+  unpack8<T>(oth, b);
+  Vec8 r;
+  T* o = reinterpret_cast<T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const double c = cs[i].x, s = low ? -cs[i].y : cs[i].y;
+    o[i] = kv8_round16<T>(fma(double(b[i]), s, double(a[i]) * c));
+  }
+  return r;
+}
+
+// Largest magnitude of eight 16-bit values as 16-bit patterns, two running maxima in one word.
+__device__ __forceinline__ uint32_t kv8_absmax(uint32_t m, const Vec8& v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __vmaxu2(m, v.w[i] & 0x7fff7fffu);
+  return m;
+}
+// ... over the warp, as the bits of a float; values that are not finite give 0x7f800000 or more.
+template <class T>
+__device__ __forceinline__ uint32_t kv8_warp_amax(uint32_t m) {
+  m = max(m & 0xffffu, m >> 16);
+  m = __reduce_max_sync(0xffffffffu, m);
+  float lo, hi;
+  Pair16<T>::unpack(m, lo, hi);
+  return __float_as_uint(lo);
+}
+
+}  // namespace ronn

@@ -81,6 +81,23 @@ def kv_append(qkv, slots, kcache, positions=None) -> None:
         _in_range("positions", positions[:tokens], 0, 1 << 30, "token positions")
 
 
+def kv8_append(qkv, slots, codes, positions=None) -> None:
+    """What the 8-bit append asks of its slots beyond their range: the tokens of one block stand in consecutive rows with
+    rising slots, so a block (whose scale its tokens share) appears once."""
+    kv_append(qkv, slots, codes, positions)
+    s = slots[: qkv.shape[0]].long()
+    at = torch.nonzero(s >= 0).reshape(-1)
+    if at.numel() == 0:
+        return
+    used = s[at]
+    starts = torch.ones_like(used, dtype=torch.bool)
+    starts[1:] = ~((used[1:] == used[:-1] + 1) & (at[1:] == at[:-1] + 1) & (used[1:] % 16 != 0))
+    first = torch.div(used[starts], 16, rounding_mode="floor")
+    order, count = torch.unique(first, return_counts=True)
+    if bool((count > 1).any()):
+        raise IndexCheckError(f"slots: the tokens of cache block {int(order[count > 1][0])} do not stand together in rising order")
+
+
 def embedding(ids, table, positions=None, pos_table=None) -> None:
     _in_range("ids", ids, 0, table.shape[0], "rows of the embedding table")
     if positions is not None and pos_table is not None:

@@ -1,0 +1,117 @@
+"""The 8-bit cache and the log probabilities on the CPU: refusals of their entry points, index checks, the scale's definition."""
+import math
+
+import pytest
+import torch
+
+from kv8_reference import Cache, least_scale
+from ronn_b200 import ops
+from ronn_b200.ops import checks as C
+
+
+def _cache(blocks=6, kvh=2, d=64, precision="int8"):
+    return ops.KV8Cache.alloc(blocks, kvh, d, precision, device="cpu")
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def _q(rows=3, cols=8 * 64, dtype=torch.bfloat16):
+    return torch.zeros(rows, cols, dtype=dtype)
+
+
+def test_cache_shapes_and_types():
+    c = _cache(precision="fp8")
+    assert c.k.dtype == torch.float8_e4m3fn and c.k.shape == (6, 2, 16, 64) and c.k_scale.shape == (6, 2) and c.num_blocks == 6
+    ok = _cache()
+    for args in ((ok.k.to(torch.uint8), ok.v.to(torch.uint8), ok.k_scale, ok.v_scale), (ok.k, c.v, ok.k_scale, ok.v_scale),
+                 (ok.k[:, :, :8], ok.v[:, :, :8], ok.k_scale, ok.v_scale), (ok.k[..., :32], ok.v[..., :32], ok.k_scale, ok.v_scale),
+                 (ok.k, ok.v, ok.k_scale.half(), ok.v_scale), (ok.k, ok.v, ok.k_scale[:5], ok.v_scale),
+                 (ok.k.transpose(0, 1), ok.v.transpose(0, 1), ok.k_scale.t(), ok.v_scale.t()), (ok.k[1:], ok.v, ok.k_scale, ok.v_scale)):
+        with pytest.raises(ops.OperandError):
+            ops.KV8Cache(*args)
+    with pytest.raises(ops.OperandError, match="int4"):
+        _cache(precision="int4")
+
+
+def test_append_refusals():
+    c, qkv, slots = _cache(), _q(), _i32([0, 1, 2])
+    bad = [dict(qkv=_q(dtype=torch.float32)), dict(qkv=_q(cols=8 * 64 - 1)), dict(qkv=_q().t()), dict(qkv=_q(cols=8 * 64 + 3)), dict(qkv=_q()[0]),
+           dict(k_off=4 * 64 + 4), dict(v_off=-8), dict(v_off=7 * 64), dict(slots=slots.long()), dict(slots=slots[:2]), dict(heads=3), dict(heads=0),
+           dict(slots=_i32([0, 1, 2, 3, 4, 5])[::2]), dict(rotated=_q()), dict(positions=slots[:2], rope_base=1e4),
+           dict(positions=slots, rope_base=math.inf), dict(positions=slots, rope_base=1e4, rotated=_q(dtype=torch.float16)),
+           dict(positions=slots, rope_base=1e4, rotated=_q(rows=2)), dict(positions=slots, rope_base=1e4, k_off=3 * 64)]
+    for change in bad:
+        kw = dict(qkv=qkv, k_off=4 * 64, v_off=6 * 64, slots=slots, cache=c, heads=4)
+        kw.update(change)
+        with pytest.raises(ops.OperandError):
+            ops.kv8_append(**kw)
+    with pytest.raises(ops.OperandError, match="CUDA device"):       # all right but for where it is
+        ops.kv8_append(qkv, 4 * 64, 6 * 64, slots, c, 4)
+
+
+def test_read_refusals():
+    c = _cache()
+    for args in ((c, _i32([0]), torch.float32), (c, torch.tensor([0])), (c, _i32([[0, 1]])), (c, _i32([0]))):
+        with pytest.raises(ops.OperandError):
+            ops.kv8_read(*args)
+
+
+def test_attention_refusals():
+    c, tab, ctx = _cache(), _i32([[0, 1, -1]] * 3), _i32([17, 3, 0])
+    good = dict(q=_q(), cache=c, block_tables=tab, ctx_len=ctx, heads=4, max_ctx=32)
+    slots = _i32([16, 2, -1])
+    for change in (dict(q=_q(dtype=torch.float32)), dict(q=_q(cols=3 * 64)), dict(q=_q(cols=8 * 64 + 4)), dict(block_tables=tab.long()),
+                   dict(block_tables=tab[:2]), dict(block_tables=tab.t()), dict(block_tables=tab[0]), dict(ctx_len=ctx[:2]), dict(ctx_len=ctx.long()),
+                   dict(bt_row=_i32([0])), dict(heads=5), dict(max_ctx=-1), dict(scale=math.nan), dict(scale=math.inf), dict(rope=(slots, 1e4)),
+                   dict(append=(4 * 64, 6 * 64, slots[:2])), dict(append=(4 * 64, 7 * 64, slots)), dict(append=(4 * 64 + 1, 6 * 64, slots)),
+                   dict(append=(4 * 64, 6 * 64, slots), rope=(slots, -1.0)), dict(append=(4 * 64, 6 * 64, slots), rope=(slots[:1], 1e4)),
+                   dict(block_tables=torch.empty(3, 0, dtype=torch.int32))):
+        with pytest.raises(ops.OperandError):
+            ops.kv8_attention(**{**good, **change})
+    with pytest.raises(ops.OperandError, match="CUDA device"):
+        ops.kv8_attention(**good)
+
+
+def test_chunk_attention_refusals():
+    c, tab = _cache(), _i32([[0, 1, -1]] * 2)
+    good = dict(q=_q(), q_off=0, cache=c, block_tables=tab, seq_start=_i32([0, 1]), q_len=_i32([1, 2]), kv_len=_i32([5, 20]), max_q_len=2, max_kv_len=20,
+                heads=8)
+    for change in (dict(q_off=8), dict(q_off=-8), dict(q_off=4, heads=4), dict(q_len=_i32([1])), dict(kv_len=torch.tensor([5, 20])),
+                   dict(block_tables=tab[:1]), dict(bt_row=_i32([0])), dict(max_q_len=-1), dict(max_kv_len=-1), dict(heads=7),
+                   dict(q=_q(dtype=torch.float32)), dict(seq_start=_i32([[0, 1]])), dict(scale=-math.inf)):
+        with pytest.raises(ops.OperandError):
+            ops.kv8_prefill_attention(**{**good, **change})
+    with pytest.raises(ops.OperandError, match="CUDA device"):
+        ops.kv8_prefill_attention(**good)
+
+
+def test_logprobs_refuse_the_host():
+    with pytest.raises(ops.OperandError, match="CUDA device"):
+        ops.token_logprobs(torch.zeros(2, 5))
+
+
+def test_index_check_of_the_append():
+    c, qkv = _cache(), _q(5)
+    C.kv8_append(qkv, _i32([5, 6, -1, 31, 32]), c.k)
+    C.kv8_append(qkv, _i32([15, 16, 17, 64, 33]), c.k)
+    for slots in ([0, 1, -1, 2, 3], [3, 2, 1, 0, 16], [0, 0, 16, 32, 48], [7, 16, 8, 32, 48]):
+        with pytest.raises(C.IndexCheckError, match="do not stand together"):
+            C.kv8_append(qkv, _i32(slots), c.k)
+    with pytest.raises(C.IndexCheckError, match=r"slots\[1\] = 96"):
+        C.kv8_append(qkv, _i32([0, 96, -1, -1, -1]), c.k)
+
+
+@pytest.mark.parametrize("code,most", [(torch.int8, 127.0), (torch.float8_e4m3fn, 448.0)])
+def test_the_scale_is_the_least_power_of_two_that_holds_the_largest(code, most):
+    for amax, e in ((most, 0), (most * (1 + 2 ** -7), 1), (most / 2, -1), (1e-40, -100), (0.0, -100), (most * 2.0 ** 20, 20)):
+        assert least_scale(amax, code) == 2.0 ** e
+
+
+def test_reference_rounds_older_codes_again_when_a_larger_token_joins():
+    c = Cache(torch.zeros(1, 1, 16, 2, dtype=torch.int8), torch.zeros(1, 1))
+    c.append(torch.tensor([[[1.0, 127.0]]]), [0])
+    assert c.scale[0, 0] == 1 and c.codes[0, 0, 0].tolist() == [1, 127]
+    c.append(torch.tensor([[[254.0, 3.0]]]), [1])
+    assert c.scale[0, 0] == 2 and c.codes[0, 0, :2].tolist() == [[0, 64], [127, 2]]      # 1/2 and 3/2 round to even
