@@ -1,0 +1,55 @@
+"""Log probabilities of tokens from logits: what a served request that asks for them is answered with, and how texts are scored."""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from .. import _native
+from .kernels import OperandError, _DT, _check, _ptr
+
+MAX_TOP = 32
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row: log probability and rank (1: the most likely) of the given token, entropy of the row in nats, and the ``top``
+    most likely tokens with their log probabilities."""
+    logprob: torch.Tensor          # fp32 [rows]
+    rank: torch.Tensor             # int32 [rows]
+    entropy: torch.Tensor          # fp32 [rows]
+    top_ids: torch.Tensor          # int32 [rows, top]
+    top_logprobs: torch.Tensor     # fp32 [rows, top]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
+    """``logits``: fp32, bf16 or fp16 [rows, vocab], row stride free.  ``tokens``: int32 or int64 [rows]; a token outside
+    [0, vocab), -1 for instance, is none: its log probability and rank are 0 (all are without ``tokens``).  ``top``: up to 32
+    alternatives.  Equal logits rank by index, the lower first.  A row whose logits are all -inf gives every token -inf and
+    an entropy of 0; NaN or +inf among the logits makes the row's figures NaN (ranks count NaN as largest)."""
+    if logits.dim() != 2 or logits.dtype not in _DT or logits.device.type != "cuda":
+        raise OperandError(f"token_logprobs needs a matrix of fp32, bf16 or fp16 logits on a CUDA device, got {logits.dtype} "
+                           f"{tuple(logits.shape)} on {logits.device}")
+    rows, vocab = logits.shape
+    if vocab < 1 or vocab > 2 ** 31 - 1 or (logits.stride(1) != 1 and vocab > 1):
+        raise OperandError(f"logits must have a vocabulary and unit column stride, got {tuple(logits.shape)}, strides {logits.stride()}")
+    if not 0 <= int(top) <= min(MAX_TOP, vocab):
+        raise OperandError(f"top is {top}; up to {min(MAX_TOP, vocab)} alternatives of {vocab} tokens")
+    dev = logits.device
+    if tokens is not None:
+        if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 1 or tokens.numel() != rows or tokens.device != dev:
+            raise OperandError(f"tokens must be {rows} int32 or int64 values on {dev}, got {tokens.dtype} {tuple(tokens.shape)} on "
+                               f"{tokens.device}")
+    with torch.cuda.device(dev):
+        if tokens is not None:
+            if tokens.dtype == torch.int64:          # beyond 32 bits is outside the vocabulary, not inside after a wrap
+                tokens = torch.where((tokens >= 0) & (tokens < vocab), tokens, torch.full_like(tokens, -1)).to(torch.int32)
+            tokens = tokens.contiguous()
+        f = torch.empty((2, rows), dtype=torch.float32, device=dev)
+        rank = torch.empty(rows, dtype=torch.int32, device=dev)
+        ids = torch.empty((rows, int(top)), dtype=torch.int32, device=dev)
+        tops = torch.empty((rows, int(top)), dtype=torch.float32, device=dev)
+        rc = _native.cuda().ronn_token_logprobs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, vocab, rows, _ptr(tokens),
+                                                f[0].data_ptr(), rank.data_ptr(), f[1].data_ptr(), ids.data_ptr(), tops.data_ptr(),
+                                                int(top), _DT[logits.dtype], torch.cuda.current_stream().cuda_stream)
+    _check(rc, "token_logprobs")
+    return TokenLogprobs(f[0], rank, f[1], ids, tops)
