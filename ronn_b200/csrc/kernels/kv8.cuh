@@ -127,4 +127,47 @@ __device__ __forceinline__ uint32_t kv8_warp_amax(uint32_t m) {
   return __float_as_uint(lo);
 }
 
+// One warp puts n tokens of one (block, head) into slots off .. off + n - 1: the block's new scale, older codes rounded again
+// where it grew, the tokens' codes.  x[p] holds 8 channels (from chunk * 8 on) of token p * (tokens a pass) + sub; a lane with
+// chunk < 0 holds a copy and writes nothing.  Tokens from n on are zeros.
+template <class T, int D, int CODE, int PASSES>
+__device__ __forceinline__ void kv8_store_run(const Vec8* x, int chunk, int sub, int n, int off, float* scale, uint8_t* codes) {
+  constexpr int TPW = 256 / D;
+  const int lane = threadIdx.x & 31;
+  const float nan = __uint_as_float(0x7fc00000u);
+  const float old = off > 0 ? *scale : 0.f;
+  uint32_t m = 0;
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) m = kv8_absmax(m, x[p]);
+  m = kv8_warp_amax<T>(m);
+  float s = m >= 0x7f800000u ? nan : kv8_least_scale<CODE>(m);
+  if (!(old <= s)) s = old;                                   // the larger of the two; NaN stays
+  if (m >= 0x7f800000u) s = nan;
+  const float inv = kv8_inverse(s);
+  __syncwarp();                                               // all lanes have read the old scale
+  if (off > 0 && s != old) {
+    const float again = inv == 0.f ? 0.f : old * inv;         // a power of two below 1, or 0
+    uint32_t* c32 = reinterpret_cast<uint32_t*>(codes);
+    for (int i = lane; i < off * (D / 4); i += 32) {
+      float f[4];
+      kv8_unpack4<CODE>(c32[i], f);
+      c32[i] = kv8_pack4<CODE>(f[0] * again, f[1] * again, f[2] * again, f[3] * again);
+    }
+  }
+  if (lane == 0 && (off == 0 || s != old)) *scale = s;
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int t = p * TPW + sub;
+    if (t >= n || chunk < 0) continue;
+    float f[8];
+    unpack8<T>(x[p], f);
+    uint2 c = make_uint2(0u, 0u);
+    if (inv != 0.f) {
+      c.x = kv8_pack4<CODE>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+      c.y = kv8_pack4<CODE>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+    }
+    *reinterpret_cast<uint2*>(codes + (off + t) * D + chunk * 8) = c;
+  }
+}
+
 }  // namespace ronn

@@ -3,115 +3,538 @@
 //   ronn_kv8_attention : query rows grouped by sequence.  Sequence s has q_len[s] queries from row seq_start[s] on (without
 //                        these two: row s, one query) and attends to the kv_len[s] keys its block-table row lists; with
 //                        `causal` its queries are the last positions of that context.  Queries without keys give zeros.
+//                        With append slots (one query per sequence) the row's new K and V join the cache first.
 //
-// First form: one warp per (query, head), one token at a time, statistics and sums in 32 bits.
+// Bound by memory: every code is read once for all the queries that share it.  A warp takes cache blocks of 16 tokens one
+// after the other, straight from global memory into the fragments of mma.sync m16n8k16, without shared memory between:
+//   S = Q K^T     A = up to 16 query rows (heads of the group, queries of a chunk), B = 8 tokens; the head dimension is the
+//                 sum's index, so its order is free: lane (g, c) of the fragment takes 16 consecutive bytes of token g, and
+//                 Q is laid out to match.
+//   O^T = V^T P^T A = 16 channels, B = 8 query rows.  The accumulator of S, (row g, tokens 2c and 2c + 1), is the B fragment
+//                 of P^T as it stands; V's channels are in free order too: lane (g, c) takes 8 or 16 consecutive bytes of
+//                 tokens 2c, 2c + 1, 2c + 8, 2c + 9 and interleaves the bytes of two tokens.
+// Codes become f16 exactly.  Q in bf16 is scaled by a power of two for each row, so that it fits f16 (its 8 significant bits
+// do; what is 2^-34 of the row's largest is lost).  Softmax statistics, sums and O are in 32 bits; P is rounded to f16 as
+// 2^15 p, 2^-12 of it and never more than 2^-40.  The scale of a K block multiplies its scores, that of a V block its P,
+// relative to the largest V scale of the 32 blocks that the warp looks up together.
 #include "kv8.cuh"
 
+#include <type_traits>
+
 namespace ronn {
+
+constexpr int KV8_NW = 4;        // warps of an attention CTA
 
 struct Kv8AttnArgs {
   const void* q;
   void* out;
-  const uint8_t* kcodes;
-  const uint8_t* vcodes;
-  const float* kscale;
-  const float* vscale;
+  uint8_t* kcodes;
+  uint8_t* vcodes;
+  float* kscale;
+  float* vscale;
   const int* tables;
   const int* kv_len;
   const int* bt_row;
   const int* seq_start;
   const int* q_len;
+  const int* slots;           // append: cache slot of each row's new token, or null
+  const int* positions;       // rotary embedding of q and the new k, or null
+  float* part;                // splits > 1: [item][split][rows][D + 2] partial results
   uint32_t* status;
   long ld_q, ld_o, num_blocks, rows, table_ld;
-  int table_rows, max_blocks, heads, kv_heads, causal;
+  int table_rows, max_blocks, heads, kv_heads, causal, splits, part_rows, max_q, k_off, v_off;
   float scale_log2;
 };
 
-template <class T, int D, int CODE>
-__global__ void __launch_bounds__(32) kv8_attention_kernel(Kv8AttnArgs a) {
-  constexpr int PER = D / 32;
+__device__ __forceinline__ void kv8_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float kv8_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t kv8_half2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Weight of a partial result with maximum m and sum l beside others whose maximum is mx: none without keys, NaN for NaN.
+__device__ __forceinline__ float kv8_weight(float m, float l, float mx) { return l == 0.f ? 0.f : l != l ? l : kv8_exp2(m - mx); }
+
+// Four codes in a word -> two f16 pairs.  int8: x + 128 as the low byte of a half with exponent 2^10 is 1024 + 128 + x.
+template <int CODE>
+__device__ __forceinline__ void kv8_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CODE == KV8_INT8) {
+    w ^= 0x80808080u;
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
+  } else {
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(uint16_t(w)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"(uint16_t(w >> 16)));
+  }
+}
+
+// The new K (IS_V: V) of one row into its slot, by one warp: kv8_append for a run of one token.
+template <class T, int D, int CODE, bool IS_V>
+__device__ __forceinline__ void kv8_append_one(const Kv8AttnArgs& a, long row, int slot, int kvh, const double2* cs) {
+  constexpr int CH = D / 8;
+  const int lane = threadIdx.x & 31, chunk = lane % CH;
+  const T* src = static_cast<const T*>(a.q) + row * a.ld_q + (IS_V ? a.v_off : a.k_off) + long(kvh) * D;
+  Vec8 x = *reinterpret_cast<const Vec8*>(src + chunk * 8);       // every CH lanes the same token
+  if (!IS_V && a.positions) {
+    Vec8 oth;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) oth.w[i] = __shfl_xor_sync(0xffffffffu, x.w[i], CH / 2);
+    x = kv8_rotate8<T>(x, oth, chunk < CH / 2, cs + (chunk % (CH / 2)) * 8);
+  }
+  const long unit = long(slot / KV8_BLOCK) * a.kv_heads + kvh;
+  const int off = slot % KV8_BLOCK;
+  float* scale = (IS_V ? a.vscale : a.kscale) + unit;
+  uint8_t* codes = (IS_V ? a.vcodes : a.kcodes) + unit * (KV8_BLOCK * D);
+  kv8_store_run<T, D, CODE, 1>(&x, lane < CH ? chunk : -1, 0, 1, off, scale, codes);
+}
+
+// One CTA of NW warps: a tile of up to 16 query rows of one (sequence, KV head), and one of `splits` shares of its blocks.
+// NT = 1: at most 8 rows.  ST: blocks a warp has in registers, one of them at work and the others on their way.
+template <class T, int D, int CODE, int NT, int NW, int ST>
+__global__ void __launch_bounds__(NW * 32) kv8_attention_kernel(Kv8AttnArgs a, Kv8Turns turns) {
+  constexpr int KW = D / 64;                  // 16-byte loads of K a lane and 8 tokens
+  constexpr int VB = D / 8;                   // bytes of V a lane and token
+  constexpr int VW = VB / 4;
+  constexpr int MT = D / 16;                  // channel tiles of O^T, k steps of S
+  constexpr int R = 8 * NT;
+  __shared__ alignas(16) __half s_q[16][D];
+  __shared__ float s_qs[16];
+  __shared__ double2 s_cs[D / 2];
+  __shared__ float s_m[NW][R], s_l[NW][R];
+  extern __shared__ float s_o[];              // [NW][R][D]
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x;
-  const int seq = blockIdx.x, head = blockIdx.y, qi = blockIdx.z;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int seq = blockIdx.x / a.kv_heads, kvh = blockIdx.x - seq * a.kv_heads;
+  const int group = a.heads / a.kv_heads;
   const int n = a.q_len ? a.q_len[seq] : 1;
-  if (qi >= n) return;
-  const long row = a.seq_start ? long(a.seq_start[seq]) + qi : seq;
-  int table = a.bt_row ? a.bt_row[seq] : seq;
+  const int r0 = blockIdx.y * 16;
+  const int live = min(min(16, a.part_rows), n * group - r0);   // rows of this tile
+  if (n > a.max_q && threadIdx.x == 0) kv8_report(a.status);    // more queries than the launch was sized for: left out
+  if (live <= 0) return;
+  const long row0 = a.seq_start ? long(a.seq_start[seq]) : seq;
+  const int table = a.bt_row ? a.bt_row[seq] : seq;
   int len = min(a.kv_len[seq], a.max_blocks * KV8_BLOCK);
-  if (row < 0 || row >= a.rows) {
-    if (lane == 0) kv8_report(a.status);
+  if (row0 < 0 || row0 + n > a.rows) {
+    if (threadIdx.x == 0) kv8_report(a.status);
     return;
   }
   if (table < 0 || table >= a.table_rows) {
-    if (lane == 0) kv8_report(a.status);
+    if (threadIdx.x == 0) kv8_report(a.status);
     len = 0;
   }
-  if (a.causal) len -= n - 1 - qi;
-  const int kvh = head / (a.heads / a.kv_heads);
-  const T* q = static_cast<const T*>(a.q) + row * a.ld_q + long(head) * D + lane * PER;
-  float qf[PER], acc[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) qf[i] = Cvt<T>::to_f(q[i]) * a.scale_log2, acc[i] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (int t = 0; t < len; ++t) {
-    const int blk = a.tables[long(table) * a.table_ld + t / KV8_BLOCK];
-    if (blk < 0 || blk >= a.num_blocks) {
-      if (lane == 0) kv8_report(a.status);
-      continue;
-    }
-    const long unit = long(blk) * a.kv_heads + kvh;
-    const long at = (unit * KV8_BLOCK + t % KV8_BLOCK) * D + lane * PER;
-    float s = 0.f, kf[PER], vf[PER];
-#pragma unroll
-    for (int i = 0; i < PER; i += 2) {
-      const float2 k = kv8_unpack2<CODE>(*reinterpret_cast<const uint16_t*>(a.kcodes + at + i));
-      const float2 v = kv8_unpack2<CODE>(*reinterpret_cast<const uint16_t*>(a.vcodes + at + i));
-      kf[i] = k.x, kf[i + 1] = k.y, vf[i] = v.x, vf[i + 1] = v.y;
-    }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s += qf[i] * kf[i];
-    s = warp_sum(s) * a.kscale[unit];
-    const float vs = a.vscale[unit];
-    const float mn = fmaxf(m, s);
-    const float c = exp2f(m - mn), p = exp2f(s - mn);
-    l = l * c + p;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = acc[i] * c + p * (vf[i] * vs);
-    m = mn;
+  // keys that the tile's last query sees, and this share's blocks
+  const int seen = a.causal ? len - (n - 1 - (r0 + live - 1) / group) : len;
+  const int nblk = seen > 0 ? (seen + KV8_BLOCK - 1) / KV8_BLOCK : 0;
+  const int b_lo = int(long(nblk) * blockIdx.z / a.splits), b_hi = int(long(nblk) * (blockIdx.z + 1) / a.splits);
+  const int w_lo = b_lo + int(long(b_hi - b_lo) * warp / NW), w_hi = b_lo + int(long(b_hi - b_lo) * (warp + 1) / NW);
+  const int* bt = a.tables + long(table) * a.table_ld;
+
+  // ---- q to shared memory: rotated, scaled to f16
+  const int pos = a.positions ? a.positions[seq] : 0;
+  if (a.positions) {
+    for (int j = threadIdx.x; j < D / 2; j += NW * 32) s_cs[j] = kv8_cos_sin(turns.t[j], pos);
+    __syncthreads();
   }
-  T* o = static_cast<T*>(a.out) + row * a.ld_o + long(head) * D + lane * PER;
+  for (int r = warp; r < 16; r += NW) {
+    constexpr int CH = D / 8;
+    const int chunk = lane % CH;
+    Vec8 x = Vec8{{0u, 0u, 0u, 0u}};
+    if (r < live) {
+      const int t = (r0 + r) / group, h = kvh * group + (r0 + r) % group;
+      x = *reinterpret_cast<const Vec8*>(static_cast<const T*>(a.q) + (row0 + t) * a.ld_q + long(h) * D + chunk * 8);
+    }
+    if (a.positions) {
+      Vec8 oth;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) o[i] = Cvt<T>::from_f(len > 0 ? acc[i] / l : 0.f);
+      for (int i = 0; i < 4; ++i) oth.w[i] = __shfl_xor_sync(0xffffffffu, x.w[i], CH / 2);
+      x = kv8_rotate8<T>(x, oth, chunk < CH / 2, s_cs + (chunk % (CH / 2)) * 8);
+    }
+    float up = 1.f, down = 1.f;
+    if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+      const uint32_t m = kv8_warp_amax<T>(kv8_absmax(0u, x)) >> 23;           // exponent of the largest
+      if (m > 0 && m < 255) {
+        const int e = max(int(m) - 127 - 10, -100);                          // largest to [2^10, 2^11)
+        up = __uint_as_float(uint32_t(127 - e) << 23);
+        down = __uint_as_float(uint32_t(127 + e) << 23);
+      }
+    }
+    if (lane < CH) {
+      float f[8];
+      unpack8<T>(x, f);
+      uint4 h;
+      h.x = kv8_half2(f[0] * up, f[1] * up), h.y = kv8_half2(f[2] * up, f[3] * up);
+      h.z = kv8_half2(f[4] * up, f[5] * up), h.w = kv8_half2(f[6] * up, f[7] * up);
+      *reinterpret_cast<uint4*>(&s_q[r][chunk * 8]) = h;
+    }
+    if (lane == 0) s_qs[r] = down * a.scale_log2;
+  }
+  // ---- the new token joins its block: the warp that reads that block writes it first (one query per sequence here)
+  if (a.slots && w_hi > w_lo && w_hi == nblk) {
+    const int slot = a.slots[seq];
+    if (slot >= long(a.num_blocks) * KV8_BLOCK) {
+      if (lane == 0) kv8_report(a.status);
+    } else if (slot >= 0) {
+      kv8_append_one<T, D, CODE, false>(a, row0, slot, kvh, s_cs);
+      kv8_append_one<T, D, CODE, true>(a, row0, slot, kvh, s_cs);
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  // Q fragments: k step j of lane c is bytes 4 (j % 4) .. + 3 of its 16 in chunk j / 4 of 64 channels
+  uint32_t qa[MT][2 * NT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int ch = (j / 4) * 64 + c * 16 + (j % 4) * 4;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint2 w = *reinterpret_cast<const uint2*>(&s_q[g + 8 * t][ch]);
+      qa[j][t] = w.x;
+      qa[j][NT + t] = w.y;
+    }
+  }
+  float qs[NT];
+  int lim[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = r0 + g + 8 * t;
+    qs[t] = s_qs[g + 8 * t];
+    lim[t] = g + 8 * t < live ? (a.causal ? len - (n - 1 - r / group) : len) : 0;
+  }
+  const int first_lim = a.causal ? len - (n - 1 - r0 / group) : len;        // the fewest keys of a live row
+
+  float o[MT][NT][4], m[NT], l[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t] = -INFINITY, l[t] = 0.f;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[i][t][k] = 0.f;
+  }
+  float vref = 0.f;                            // o is in units of vref * 2^-15
+
+  uint4 kb[ST][2 * KW];
+  uint32_t vb[ST][4][VW];
+  // looked up for 32 blocks at a time, one a lane
+  int page = -1;
+  float kf = 0.f, vf = 0.f;
+  auto look_up = [&](int b0) {
+    const int b = b0 + lane;
+    page = b < w_hi ? bt[b] : -1;
+    const bool ok = page >= 0 && page < a.num_blocks;
+    if (!ok && b < w_hi) kv8_report(a.status);
+    if (!ok) page = -1;
+    const long unit = long(ok ? page : 0) * a.kv_heads + kvh;
+    kf = ok ? a.kscale[unit] : 0.f;
+    vf = ok ? a.vscale[unit] : 0.f;
+    if (vf != vf) kf = vf, vf = 0.f;            // seeing the block's keys is seeing its values: NaN through the scores
+  };
+  auto load = [&](int slot_in, int b) {         // b: index within the 32
+    const int p = __shfl_sync(0xffffffffu, page, b);
+    const long base = (long(max(p, 0)) * a.kv_heads + kvh) * (KV8_BLOCK * D);
+    const uint8_t* kp = a.kcodes + base;
+    const uint8_t* vp = a.vcodes + base;
+#pragma unroll
+    for (int i = 0; i < KW; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        kb[slot_in][2 * i + h] = *reinterpret_cast<const uint4*>(kp + (g + 8 * h) * D + i * 64 + c * 16);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint8_t* src = vp + (2 * c + (k & 1) + 8 * (k >> 1)) * D + g * VB;
+      if constexpr (VW == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(src);
+        vb[slot_in][k][0] = w.x, vb[slot_in][k][1] = w.y;
+      } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(src);
+        vb[slot_in][k][0] = w.x, vb[slot_in][k][1] = w.y, vb[slot_in][k][2] = w.z, vb[slot_in][k][3] = w.w;
+      }
+    }
+  };
+  for (int b0 = w_lo; b0 < w_hi; b0 += 32) {
+    look_up(b0);
+    const int cnt = min(32, w_hi - b0);
+    const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vf)));
+    if (top > vref) {
+      const float down = vref * kv8_inverse(top);          // 0 the first time
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[i][t][k] *= down;
+      vref = top;
+    }
+    vf *= kv8_inverse(vref) * 32768.f;
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s)
+      if (s < cnt) load(s, s);
+    for (int b8 = 0; b8 < cnt; b8 += ST) {
+#pragma unroll
+      for (int s = 0; s < ST; ++s) {
+        const int b = b8 + s;
+        if (b >= cnt) break;
+        if (b + ST - 1 < cnt) load((s + ST - 1) % ST, b + ST - 1);
+        // ---- scores
+        float sc[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            const uint4& w4 = kb[s][2 * (j / 4) + h];
+            const uint32_t w = (j % 4) == 0 ? w4.x : (j % 4) == 1 ? w4.y : (j % 4) == 2 ? w4.z : w4.w;
+            uint32_t b0r, b1r;
+            kv8_halves<CODE>(w, b0r, b1r);
+            kv8_mma(sc[h], qa[j][0], NT == 2 ? qa[j][1] : 0u, qa[j][NT], NT == 2 ? qa[j][NT + 1] : 0u, b0r, b1r);
+          }
+        }
+        const float kfac = __shfl_sync(0xffffffffu, kf, b), vfac = __shfl_sync(0xffffffffu, vf, b);
+        const int t0 = (b0 + b) * KV8_BLOCK;
+        const bool gone = __shfl_sync(0xffffffffu, page, b) < 0;
+        const bool edge = gone || t0 + KV8_BLOCK > first_lim;
+        float x[NT][4];                         // (row g + 8 t; tokens 2c, 2c + 1, 2c + 8, 2c + 9)
+        bool rise = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float f = kfac * qs[t];
+          x[t][0] = sc[0][2 * t] * f, x[t][1] = sc[0][2 * t + 1] * f, x[t][2] = sc[1][2 * t] * f, x[t][3] = sc[1][2 * t + 1] * f;
+          if (edge) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (gone || t0 + 2 * c + (k & 1) + 8 * (k >> 1) >= lim[t]) x[t][k] = -INFINITY;
+          }
+          rise |= fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])) > m[t];
+        }
+        if (edge) {
+          // bytes behind the context are no codes
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (gone || t0 + 2 * c + (k & 1) + 8 * (k >> 1) >= len) {
+#pragma unroll
+              for (int i = 0; i < VW; ++i) vb[s][k][i] = 0u;
+            }
+        }
+        if (__any_sync(0xffffffffu, rise)) {
+          float alpha[NT];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            float mx = fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            mx = fmaxf(mx, m[t]);
+            alpha[t] = mx == -INFINITY ? 1.f : kv8_exp2(m[t] - mx);
+            l[t] *= alpha[t];
+            m[t] = mx;
+          }
+          // o's rows run along c: rows 2c and 2c + 1 of the tile, held for scores by lanes g = 2c and 2c + 1
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const float a0 = __shfl_sync(0xffffffffu, alpha[t], 8 * c), a1 = __shfl_sync(0xffffffffu, alpha[t], 8 * c + 4);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[i][t][0] *= a0, o[i][t][1] *= a1, o[i][t][2] *= a0, o[i][t][3] *= a1;
+          }
+        }
+        uint32_t p[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float mm = m[t] == -INFINITY ? 0.f : m[t];
+          float e[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) e[k] = kv8_exp2(x[t][k] - mm);
+          l[t] += (e[0] + e[1]) + (e[2] + e[3]);
+          p[t][0] = kv8_half2(e[0] * vfac, e[1] * vfac);
+          p[t][1] = kv8_half2(e[2] * vfac, e[3] * vfac);
+        }
+        // ---- values: channel tile i has channels 2 i and 2 i + 1 of the lane's
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int w = i / 2;
+          const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
+          uint32_t a0, a1, a2, a3;
+          kv8_halves<CODE>(__byte_perm(vb[s][0][w], vb[s][1][w], sel), a0, a1);
+          kv8_halves<CODE>(__byte_perm(vb[s][2][w], vb[s][3][w], sel), a2, a3);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) kv8_mma(o[i][t], a0, a1, a2, a3, p[t][0], p[t][1]);
+        }
+      }
+    }
+  }
+
+  // ---- the warps' results together
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
+    l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
+    if (c == 0) s_m[warp][g + 8 * t] = m[t], s_l[warp][g + 8 * t] = l[t];
+  }
+  const float unit = vref * (1.f / 32768.f);
+  // o[i][t][k]: channel g * VB + 2 i + (k >> 1), row 2c + (k & 1) + 8 t
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = 2 * c + k + 8 * t;
+      if (r < live) {
+        float* dst = s_o + (warp * R + r) * D + g * VB;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[i][t][k] * unit, o[i][t][k + 2] * unit);
+      }
+    }
+  __syncthreads();
+  const long item = (long(blockIdx.y) * gridDim.x + blockIdx.x) * a.splits + blockIdx.z;
+  for (int i = threadIdx.x; i < live * (D / 2); i += NW * 32) {
+    const int r = i / (D / 2), ch = (i % (D / 2)) * 2;
+    float mx = s_m[0][r];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, s_m[w][r]);
+    float s0 = 0.f, s1 = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = kv8_weight(s_m[w][r], s_l[w][r], mx);
+      const float2 v = *reinterpret_cast<const float2*>(s_o + (w * R + r) * D + ch);
+      if (f != 0.f) s0 += f * v.x, s1 += f * v.y, sum += f * s_l[w][r];
+    }
+    if (a.splits > 1) {
+      float* dst = a.part + (item * a.part_rows + r) * (D + 2);
+      *reinterpret_cast<float2*>(dst + ch) = make_float2(s0, s1);
+      if (ch == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mx, sum);
+    } else {
+      const int t = (r0 + r) / group, h = kvh * group + (r0 + r) % group;
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      T* dst = static_cast<T*>(a.out) + (row0 + t) * a.ld_o + long(h) * D + ch;
+      *reinterpret_cast<uint32_t*>(dst) = Pair16<T>::pack(s0 * inv, s1 * inv);
+    }
+  }
+}
+
+// The shares of a row together: one warp for each row of each tile.
+template <class T, int D>
+__global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8AttnArgs a, long tiles, int items_x) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const long unit = long(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const long tile = unit / a.part_rows;
+  const int r = int(unit - tile * a.part_rows);
+  if (tile >= tiles) return;
+  const int x = int(tile % items_x), r0 = int(tile / items_x) * 16;
+  const int seq = x / a.kv_heads, kvh = x - seq * a.kv_heads, group = a.heads / a.kv_heads;
+  const int n = a.q_len ? a.q_len[seq] : 1;
+  if (r0 + r >= n * group || r >= 16) return;
+  const long row0 = a.seq_start ? long(a.seq_start[seq]) : seq;
+  if (row0 < 0 || row0 + n > a.rows) return;
+  const float* src = a.part + (tile * a.splits * a.part_rows + r) * (D + 2);
+  const long step = long(a.part_rows) * (D + 2);
+  float mx = -INFINITY;
+  for (int z = 0; z < a.splits; ++z) mx = fmaxf(mx, src[z * step + D]);
+  constexpr int PER = D / 32;
+  float acc[PER], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) acc[k] = 0.f;
+  for (int z = 0; z < a.splits; ++z) {
+    const float l = src[z * step + D + 1], mz = src[z * step + D];
+    const float f = kv8_weight(mz, l, mx);
+    if (f != 0.f) {
+      sum += f * l;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) acc[k] += f * src[z * step + lane * PER + k];
+    }
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  T* dst = static_cast<T*>(a.out) + (row0 + (r0 + r) / group) * a.ld_o + long(kvh * group + (r0 + r) % group) * D + lane * PER;
+#pragma unroll
+  for (int k = 0; k < PER; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = Pair16<T>::pack(acc[k] * inv, acc[k + 1] * inv);
 }
 
 }  // namespace ronn
 
 using namespace ronn;
 
-// q, out: 16-bit [rows, ld]; dtype 0 bf16, 1 fp16; code 0 int8, 1 e4m3; head_dim 64 or 128.  max_q_len bounds q_len.
-extern "C" int ronn_kv8_attention(const void* q, long ld_q, long rows, const void* kcodes, const void* vcodes, const float* kscale,
-                                  const float* vscale, long num_blocks, const int* tables, long table_ld, int table_rows, int max_blocks,
+// How many CTAs share the blocks of one tile: enough for two waves' worth of CTAs, each with at least four blocks a warp.
+static int kv8_splits(long tiles, int max_ctx) {
+  const long want = 2L * device_sm_count();
+  const long by_work = max_ctx / (KV8_BLOCK * KV8_NW * 4);
+  long s = tiles > 0 ? want / tiles : 1;
+  if (s > by_work) s = by_work;
+  return int(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+// Bytes of scratch that ronn_kv8_attention needs for these sizes; 0 where one CTA takes a whole tile.
+extern "C" long ronn_kv8_attention_scratch(int n_seq, int max_q_len, int max_ctx, int heads, int kv_heads, int head_dim) {
+  if (n_seq <= 0 || max_q_len <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  const long rows = long(max_q_len) * (heads / kv_heads), tiles = (rows + 15) / 16 * n_seq * kv_heads;
+  const int s = kv8_splits(tiles, max_ctx);
+  return s <= 1 ? 0 : tiles * s * (rows < 16 ? rows : 16) * (head_dim + 2) * long(sizeof(float));
+}
+
+// q, out: 16-bit [rows, ld]; dtype 0 bf16, 1 fp16; code 0 int8, 1 e4m3; head_dim 64 or 128.  max_q_len bounds q_len, max_ctx
+// sizes the launch.  slots (one query per sequence): the new K and V of row s are at columns k_off and v_off of q's row and
+// join the cache at slots[s]; positions and turns (kv8_append): rotary embedding of q and the new k.
+extern "C" int ronn_kv8_attention(const void* q, long ld_q, long rows, void* kcodes, void* vcodes, float* kscale, float* vscale,
+                                  long num_blocks, const int* tables, long table_ld, int table_rows, int max_blocks,
                                   const int* bt_row, const int* seq_start, const int* q_len, const int* kv_len, void* out,
-                                  long ld_o, int n_seq, int max_q_len, int heads, int kv_heads, int head_dim, int causal,
-                                  float scale, int dtype, int code, uint32_t* status, cudaStream_t stream) {
+                                  long ld_o, int n_seq, int max_q_len, int max_ctx, int heads, int kv_heads, int head_dim, int causal,
+                                  float scale, int dtype, int code, int k_off, int v_off, const int* slots, const int* positions,
+                                  const unsigned long long* turns, void* scratch, long scratch_bytes, uint32_t* status,
+                                  cudaStream_t stream) {
   if (n_seq <= 0 || max_q_len <= 0) return 0;
-  if (heads <= 0 || heads > 65535 || kv_heads <= 0 || heads % kv_heads || max_q_len > 65535 || (ld_q & 7) || (ld_o & 7)) return -2;
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || (ld_q & 7) || (ld_o & 7) || max_ctx < 0) return -2;
   if ((seq_start == nullptr) != (q_len == nullptr)) return -2;
-  Kv8AttnArgs a{q, out, (const uint8_t*)kcodes, (const uint8_t*)vcodes, kscale, vscale, tables, kv_len, bt_row, seq_start, q_len,
-                status, ld_q, ld_o, num_blocks, rows, table_ld, table_rows, max_blocks, heads, kv_heads, causal, scale * 1.4426950408889634f};
-  const dim3 grid{unsigned(n_seq), unsigned(heads), unsigned(max_q_len)};
-#define RONN_KV8T(T, D, C) launch(kv8_attention_kernel<T, D, C>, grid, dim3(32), 0, stream, a)
-#define RONN_KV8T_(T) \
+  if ((slots || positions) && seq_start) return -2;
+  if (positions && (!turns || !slots)) return -2;
+  if (head_dim != 64 && head_dim != 128) return -1;
+  const long group_rows = long(max_q_len) * (heads / kv_heads), mtiles = (group_rows + 15) / 16, xs = long(n_seq) * kv_heads;
+  if (xs > 2147483647L || mtiles > 65535) return -2;
+  const int splits = kv8_splits(xs * mtiles, max_ctx);
+  const int part_rows = int(group_rows < 16 ? group_rows : 16);
+  const long need = ronn_kv8_attention_scratch(n_seq, max_q_len, max_ctx, heads, kv_heads, head_dim);
+  if (splits > 1 && (scratch == nullptr || scratch_bytes < need)) return -4;
+  Kv8Turns tn = {};
+  if (positions)
+    for (int j = 0; j < head_dim / 2; ++j) tn.t[j] = turns[j];
+  Kv8AttnArgs a{q, out, (uint8_t*)kcodes, (uint8_t*)vcodes, kscale, vscale, tables, kv_len, bt_row, seq_start, q_len, slots, positions,
+                (float*)scratch, status, ld_q, ld_o, num_blocks, rows, table_ld, table_rows, max_blocks, heads, kv_heads, causal,
+                splits, part_rows, max_q_len, k_off, v_off, scale * 1.4426950408889634f};
+  const dim3 grid{unsigned(xs), unsigned(mtiles), unsigned(splits)};
+  const bool small = group_rows <= 8;
+#define RONN_KV8T(T, D, C, NT) \
   do { \
-    if (head_dim == 64 && code == 0) RONN_KV8T(T, 64, 0); \
-    else if (head_dim == 64 && code == 1) RONN_KV8T(T, 64, 1); \
-    else if (head_dim == 128 && code == 0) RONN_KV8T(T, 128, 0); \
-    else if (head_dim == 128 && code == 1) RONN_KV8T(T, 128, 1); \
-    else return -1; \
+    constexpr int smem = KV8_NW * 8 * NT * D * 4; \
+    auto* kern = kv8_attention_kernel<T, D, C, NT, KV8_NW, (D == 64 ? 3 : 2)>; \
+    static bool seen[MAX_DEVICES] = {false}; \
+    if (smem > 32768 && first_use_on_device(seen) && \
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3; \
+    launch(kern, grid, dim3(KV8_NW * 32), smem, stream, a, tn); \
   } while (0)
-  if (dtype == 0) RONN_KV8T_(__nv_bfloat16);
-  else if (dtype == 1) RONN_KV8T_(__half);
+#define RONN_KV8T_(T, D) \
+  do { \
+    if (code == 0 && small) RONN_KV8T(T, D, 0, 1); \
+    else if (code == 0) RONN_KV8T(T, D, 0, 2); \
+    else if (code == 1 && small) RONN_KV8T(T, D, 1, 1); \
+    else if (code == 1) RONN_KV8T(T, D, 1, 2); \
+    else return -1; \
+    if (splits > 1) { \
+      const long units = xs * mtiles * part_rows; \
+      launch(kv8_combine_kernel<T, D>, dim3(unsigned((units + 3) / 4)), dim3(128), 0, stream, a, xs * mtiles, int(xs)); \
+    } \
+  } while (0)
+  if (dtype == 0 && head_dim == 64) RONN_KV8T_(__nv_bfloat16, 64);
+  else if (dtype == 0) RONN_KV8T_(__nv_bfloat16, 128);
+  else if (dtype == 1 && head_dim == 64) RONN_KV8T_(__half, 64);
+  else if (dtype == 1) RONN_KV8T_(__half, 128);
   else return -1;
 #undef RONN_KV8T
 #undef RONN_KV8T_

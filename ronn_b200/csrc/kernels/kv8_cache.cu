@@ -108,43 +108,9 @@ kv8_append_kernel(Kv8AppendArgs a, Kv8Turns turns) {
         }
       }
       if (is_q || slot0 < 0) continue;
-      uint32_t m = 0;
-#pragma unroll
-      for (int p = 0; p < PASSES; ++p) m = kv8_absmax(m, x[p]);
-      m = kv8_warp_amax<T>(m);
-      const long blk = slot0 / KV8_BLOCK;
-      const int off = slot0 % KV8_BLOCK;
-      float* scale = (is_v ? a.vscale : a.kscale) + blk * a.kv_heads + h;
-      uint8_t* codes = (is_v ? a.vcodes : a.kcodes) + (blk * a.kv_heads + h) * (KV8_BLOCK * D);
-      const float old = off > 0 ? *scale : 0.f;
-      float s = m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : kv8_least_scale<CODE>(m);
-      if (!(old <= s)) s = old;                               // the larger of the two; NaN stays
-      if (m >= 0x7f800000u) s = __uint_as_float(0x7fc00000u);
-      const float inv = kv8_inverse(s);
-      __syncwarp();                                           // all lanes have read the old scale
-      if (off > 0 && s != old) {
-        const float again = inv == 0.f ? 0.f : old * inv;     // a power of two below 1, or 0
-        uint32_t* c32 = reinterpret_cast<uint32_t*>(codes);
-        for (int i = lane; i < off * (D / 4); i += 32) {
-          float f[4];
-          kv8_unpack4<CODE>(c32[i], f);
-          c32[i] = kv8_pack4<CODE>(f[0] * again, f[1] * again, f[2] * again, f[3] * again);
-        }
-      }
-      if (lane == 0 && (off == 0 || s != old)) *scale = s;
-#pragma unroll
-      for (int p = 0; p < PASSES; ++p) {
-        const int t = p * TPW + sub;
-        if (t >= n) continue;
-        float f[8];
-        unpack8<T>(x[p], f);
-        uint2 c = make_uint2(0u, 0u);
-        if (inv != 0.f) {
-          c.x = kv8_pack4<CODE>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-          c.y = kv8_pack4<CODE>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
-        }
-        *reinterpret_cast<uint2*>(codes + (off + t) * D + chunk * 8) = c;
-      }
+      const long unit = long(slot0 / KV8_BLOCK) * a.kv_heads + h;
+      kv8_store_run<T, D, CODE, PASSES>(x, chunk, sub, n, slot0 % KV8_BLOCK, (is_v ? a.vscale : a.kscale) + unit,
+                                        (is_v ? a.vcodes : a.kcodes) + unit * (KV8_BLOCK * D));
     }
   }
 }

@@ -49,7 +49,8 @@ def declare(lib):
     sig("ronn_gemm_rownorm", [V, V, V, V, V, V, V, V, I, I, I, I, I, I, F, I, I, V, V], optional=True)
     sig("ronn_kv8_append", [V, L, V, L, I, I, V, V, V, V, V, V, V, L, L, I, I, I, I, I, V, V])
     sig("ronn_kv8_read", [V, V, V, V, V, V, V, L, L, I, I, I, I, V, V])
-    sig("ronn_kv8_attention", [V, L, L, V, V, V, V, L, V, L, I, I, V, V, V, V, V, L, I, I, I, I, I, I, F, I, I, V, V])
+    sig("ronn_kv8_attention", [V, L, L, V, V, V, V, L, V, L, I, I, V, V, V, V, V, L, I, I, I, I, I, I, I, F, I, I, I, I, V, V, V, V, L, V, V])
+    sig("ronn_kv8_attention_scratch", [I, I, I, I, I, I], restype=L)
     sig("ronn_token_logprobs", [V, L, I, L, V, V, V, V, V, V, I, I, V])
     sig("ronn_fmha", [V, L, L, I, I, I, V, V, V, V, L, I, I, I, I, I, I, F, I, V, V])
     sig("ronn_fmha_paged", [V, L, L, I, V, V, L, V, I, V, V, V, V, V, L, I, I, I, I, I, I, F, I, V, V])

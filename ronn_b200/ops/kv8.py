@@ -197,6 +197,21 @@ def _scale(scale: Optional[float], d: int) -> float:
     return s
 
 
+def _attention(q_ptr, q, ld, rows, cache, tables, table_ld, bt_row, seq_start, q_len, kv_len, out, ld_o, n_seq, max_q, max_ctx, heads, causal,
+               scale, append=None, rope=None) -> int:
+    lib, dev, d = _native.cuda(), cache.device, cache.head_dim
+    max_ctx = min(max_ctx, tables.shape[1] * _BLOCK)
+    need = lib.ronn_kv8_attention_scratch(n_seq, max_q, max_ctx, heads, cache.kv_heads, d)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None       # this call's own: graphs share none
+    return lib.ronn_kv8_attention(q_ptr, ld, rows, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+                                  cache.num_blocks, tables.data_ptr(), table_ld, tables.shape[0], tables.shape[1], _ptr(bt_row),
+                                  _ptr(seq_start), _ptr(q_len), kv_len.data_ptr(), out.data_ptr(), ld_o, n_seq, max_q, max_ctx, heads,
+                                  cache.kv_heads, d, causal, scale, _DT[q.dtype], cache.code, append[0] if append else 0,
+                                  append[1] if append else 0, append[2].data_ptr() if append else None, rope[0].data_ptr() if rope else None,
+                                  _turns(d, float(rope[1])) if rope else None, _ptr(scratch), need, status_word(dev).data_ptr(),
+                                  torch.cuda.current_stream().cuda_stream)
+
+
 def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, ctx_len: torch.Tensor, heads: int, max_ctx: int,
                   bt_row: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                   append=None, rope=None) -> torch.Tensor:
@@ -231,19 +246,8 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, 
             _run_check(_checks.paged_attention, q, cache.k, block_tables, ctx_len, heads, d, int(max_ctx), bt_row,
                        append[2] if append else None, rope[0] if rope else None)
         out, ld_o = _out(out, q, rows, heads * d)
-        if append is not None:
-            if rope is not None:
-                rotated = torch.empty((rows, append[0] + cache.kv_heads * d), dtype=q.dtype, device=dev)
-                kv8_append(q, append[0], append[1], append[2], cache, heads, rope[0], float(rope[1]), rotated)
-                q, ld = rotated, rotated.stride(0)
-            else:
-                kv8_append(q, append[0], append[1], append[2], cache, heads)
-        rc = _native.cuda().ronn_kv8_attention(q.data_ptr(), ld, rows, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-                                               cache.v_scale.data_ptr(), cache.num_blocks, block_tables.data_ptr(), table_ld,
-                                               block_tables.shape[0], block_tables.shape[1], _ptr(bt_row), None, None,
-                                               ctx_len.data_ptr(), out.data_ptr(), ld_o, rows, 1, heads, cache.kv_heads, d, 0, sc,
-                                               _DT[q.dtype], cache.code, status_word(dev).data_ptr(),
-                                               torch.cuda.current_stream().cuda_stream)
+        rc = _attention(q.data_ptr(), q, ld, rows, cache, block_tables, table_ld, bt_row, None, None, ctx_len, out, ld_o, rows, 1,
+                        int(max_ctx), heads, 0, sc, append, rope)
     _check(rc, "kv8_attention")
     return out
 
@@ -277,12 +281,7 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
             _run_check(_checks.paged_attention, kv_len[:n_seq, None], cache.k, block_tables, kv_len, 0, 0,
                        block_tables.shape[1] * _BLOCK, rows_of)
         out, ld_o = _out(out, q, tokens, heads * d)
-        rc = _native.cuda().ronn_kv8_attention(q.data_ptr() + 2 * q_off, ld, tokens, cache.k.data_ptr(), cache.v.data_ptr(),
-                                               cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.num_blocks,
-                                               block_tables.data_ptr(), table_ld, block_tables.shape[0], block_tables.shape[1],
-                                               _ptr(bt_row), seq_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), out.data_ptr(),
-                                               ld_o, n_seq, int(max_q_len), heads, cache.kv_heads, d, 1 if causal else 0, sc,
-                                               _DT[q.dtype], cache.code, status_word(dev).data_ptr(),
-                                               torch.cuda.current_stream().cuda_stream)
+        rc = _attention(q.data_ptr() + 2 * q_off, q, ld, tokens, cache, block_tables, table_ld, bt_row, seq_start, q_len, kv_len, out, ld_o,
+                        n_seq, int(max_q_len), int(max_kv_len), heads, 1 if causal else 0, sc)
     _check(rc, "kv8_prefill_attention")
     return out
