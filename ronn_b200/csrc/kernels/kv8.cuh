@@ -128,10 +128,10 @@ __device__ __forceinline__ uint32_t kv8_warp_amax(uint32_t m) {
 }
 
 // One warp puts n tokens of one (block, head) into slots off .. off + n - 1: the block's new scale, older codes rounded again
-// where it grew, the tokens' codes.  x[p] holds 8 channels (from chunk * 8 on) of token p * (tokens a pass) + sub; a lane with
+// where it grew, the tokens' codes; returns the scale.  x[p] holds 8 channels (from chunk * 8 on) of token p * (tokens a pass) + sub; a lane with
 // chunk < 0 holds a copy and writes nothing.  Tokens from n on are zeros.
 template <class T, int D, int CODE, int PASSES>
-__device__ __forceinline__ void kv8_store_run(const Vec8* x, int chunk, int sub, int n, int off, float* scale, uint8_t* codes) {
+__device__ __forceinline__ float kv8_store_run(const Vec8* x, int chunk, int sub, int n, int off, float* scale, uint8_t* codes) {
   constexpr int TPW = 256 / D;
   const int lane = threadIdx.x & 31;
   const float nan = __uint_as_float(0x7fc00000u);
@@ -168,6 +168,7 @@ __device__ __forceinline__ void kv8_store_run(const Vec8* x, int chunk, int sub,
     }
     *reinterpret_cast<uint2*>(codes + (off + t) * D + chunk * 8) = c;
   }
+  return s;
 }
 
 }  // namespace ronn

@@ -19,6 +19,7 @@
 // relative to the largest V scale of the 32 blocks that the warp looks up together.
 #include "kv8.cuh"
 
+#include <stdlib.h>
 #include <type_traits>
 
 namespace ronn {
@@ -42,12 +43,12 @@ struct Kv8AttnArgs {
   float* part;                // splits > 1: [item][split][rows][D + 2] partial results
   uint32_t* status;
   long ld_q, ld_o, num_blocks, rows, table_ld;
-  int table_rows, max_blocks, heads, kv_heads, causal, splits, part_rows, max_q, k_off, v_off;
+  int items_x, table_rows, max_blocks, heads, kv_heads, causal, splits, share, part_rows, max_q, k_off, v_off;
   float scale_log2;
 };
 
 __device__ __forceinline__ void kv8_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -79,9 +80,9 @@ __device__ __forceinline__ void kv8_halves(uint32_t w, uint32_t& lo, uint32_t& h
   }
 }
 
-// The new K (IS_V: V) of one row into its slot, by one warp: kv8_append for a run of one token.
+// The new K (IS_V: V) of one row into its slot, by one warp: kv8_append for a run of one token.  Returns the block's scale.
 template <class T, int D, int CODE, bool IS_V>
-__device__ __forceinline__ void kv8_append_one(const Kv8AttnArgs& a, long row, int slot, int kvh, const double2* cs) {
+__device__ __forceinline__ float kv8_append_one(const Kv8AttnArgs& a, long row, int slot, int kvh, const double2* cs) {
   constexpr int CH = D / 8;
   const int lane = threadIdx.x & 31, chunk = lane % CH;
   const T* src = static_cast<const T*>(a.q) + row * a.ld_q + (IS_V ? a.v_off : a.k_off) + long(kvh) * D;
@@ -93,105 +94,165 @@ __device__ __forceinline__ void kv8_append_one(const Kv8AttnArgs& a, long row, i
     x = kv8_rotate8<T>(x, oth, chunk < CH / 2, cs + (chunk % (CH / 2)) * 8);
   }
   const long unit = long(slot / KV8_BLOCK) * a.kv_heads + kvh;
-  const int off = slot % KV8_BLOCK;
-  float* scale = (IS_V ? a.vscale : a.kscale) + unit;
-  uint8_t* codes = (IS_V ? a.vcodes : a.kcodes) + unit * (KV8_BLOCK * D);
-  kv8_store_run<T, D, CODE, 1>(&x, lane < CH ? chunk : -1, 0, 1, off, scale, codes);
+  return kv8_store_run<T, D, CODE, 1>(&x, lane < CH ? chunk : -1, 0, 1, slot % KV8_BLOCK, (IS_V ? a.vscale : a.kscale) + unit,
+                                      (IS_V ? a.vcodes : a.kcodes) + unit * (KV8_BLOCK * D));
 }
 
-// One CTA of NW warps: a tile of up to 16 query rows of one (sequence, KV head), and one of `splits` shares of its blocks.
-// NT = 1: at most 8 rows.  ST: blocks a warp has in registers, one of them at work and the others on their way.
-template <class T, int D, int CODE, int NT, int NW, int ST>
-__global__ void __launch_bounds__(NW * 32) kv8_attention_kernel(Kv8AttnArgs a, Kv8Turns turns) {
+// Barrier of the warps that share an item.
+template <int WPI>
+__device__ __forceinline__ void kv8_item_sync(int item) {
+  if constexpr (WPI == 1) __syncwarp();
+  else if constexpr (WPI == KV8_NW) __syncthreads();
+  else asm volatile("bar.sync %0, %1;" ::"r"(item + 1), "n"(WPI * 32) : "memory");
+}
+
+// An item is a tile of up to 16 query rows of one (sequence, KV head), and one of `splits` shares of its blocks; WPI of the
+// CTA's warps work on it.  NT = 1: at most 8 rows.  ST: blocks a warp has in registers, one at work and the others on their
+// way.  A warp's first loads start before q is fetched: the chain length -> page -> codes is the longer one.
+template <class T, int D, int CODE, int NT, int WPI, int ST>
+__global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64 ? 4 : 3) kv8_attention_kernel(Kv8AttnArgs a, Kv8Turns turns) {
   constexpr int KW = D / 64;                  // 16-byte loads of K a lane and 8 tokens
   constexpr int VB = D / 8;                   // bytes of V a lane and token
   constexpr int VW = VB / 4;
   constexpr int MT = D / 16;                  // channel tiles of O^T, k steps of S
   constexpr int R = 8 * NT;
-  __shared__ alignas(16) __half s_q[16][D];
-  __shared__ float s_qs[16];
-  __shared__ double2 s_cs[D / 2];
-  __shared__ float s_m[NW][R], s_l[NW][R];
-  extern __shared__ float s_o[];              // [NW][R][D]
+  constexpr int IPC = KV8_NW / WPI;           // items of a CTA
+  constexpr int CH = D / 8;
+  __shared__ alignas(16) __half s_q_all[IPC][R][D];
+  __shared__ float s_qs_all[IPC][R];
+  __shared__ double2 s_cs_all[IPC][D / 2];
+  __shared__ float s_m_all[KV8_NW][R], s_l_all[KV8_NW][R];
+  extern __shared__ float s_o_all[];          // [KV8_NW][R][D]
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  const int seq = blockIdx.x / a.kv_heads, kvh = blockIdx.x - seq * a.kv_heads;
+  const int in_cta = warp / WPI, iw = warp % WPI, it = iw * 32 + lane;        // item of the CTA, warp and thread of the item
+  const int x_item = int(blockIdx.x) * IPC + in_cta;
+  if (x_item >= a.items_x) return;
+  auto& s_q = s_q_all[in_cta];
+  auto& s_qs = s_qs_all[in_cta];
+  auto& s_cs = s_cs_all[in_cta];
+  auto* s_m = s_m_all + in_cta * WPI;
+  auto* s_l = s_l_all + in_cta * WPI;
+  float* s_o = s_o_all + in_cta * WPI * R * D;
+  const int seq = x_item / a.kv_heads, kvh = x_item - seq * a.kv_heads;
   const int group = a.heads / a.kv_heads;
   const int n = a.q_len ? a.q_len[seq] : 1;
   const int r0 = blockIdx.y * 16;
   const int live = min(min(16, a.part_rows), n * group - r0);   // rows of this tile
-  if (n > a.max_q && threadIdx.x == 0) kv8_report(a.status);    // more queries than the launch was sized for: left out
+  if (n > a.max_q && it == 0) kv8_report(a.status);             // more queries than the launch was sized for: left out
   if (live <= 0) return;
   const long row0 = a.seq_start ? long(a.seq_start[seq]) : seq;
   const int table = a.bt_row ? a.bt_row[seq] : seq;
+  const int slot = a.slots ? a.slots[seq] : -1;
+  const int pos = a.positions ? a.positions[seq] : 0;
   int len = min(a.kv_len[seq], a.max_blocks * KV8_BLOCK);
   if (row0 < 0 || row0 + n > a.rows) {
-    if (threadIdx.x == 0) kv8_report(a.status);
+    if (it == 0) kv8_report(a.status);
     return;
   }
   if (table < 0 || table >= a.table_rows) {
-    if (threadIdx.x == 0) kv8_report(a.status);
+    if (it == 0) kv8_report(a.status);
     len = 0;
   }
-  // keys that the tile's last query sees, and this share's blocks
+  // keys that the tile's last query sees, this share's blocks, this warp's
   const int seen = a.causal ? len - (n - 1 - (r0 + live - 1) / group) : len;
   const int nblk = seen > 0 ? (seen + KV8_BLOCK - 1) / KV8_BLOCK : 0;
-  const int b_lo = int(long(nblk) * blockIdx.z / a.splits), b_hi = int(long(nblk) * (blockIdx.z + 1) / a.splits);
-  const int w_lo = b_lo + int(long(b_hi - b_lo) * warp / NW), w_hi = b_lo + int(long(b_hi - b_lo) * (warp + 1) / NW);
-  const int* bt = a.tables + long(table) * a.table_ld;
+  const int b_lo = min(nblk, int(blockIdx.z) * a.share), b_hi = blockIdx.z + 1 == a.splits ? nblk : min(nblk, b_lo + a.share);
+  const int w_lo = b_lo + int(long(b_hi - b_lo) * iw / WPI), w_hi = b_lo + int(long(b_hi - b_lo) * (iw + 1) / WPI);
+  const int cnt = w_hi - w_lo;
+  const int* bt = a.tables + long(table) * a.table_ld + w_lo;
+  const bool appends = slot >= 0 && cnt > 0 && w_hi == nblk;    // the warp that reads the last block writes the new token
 
-  // ---- q to shared memory: rotated, scaled to f16
-  const int pos = a.positions ? a.positions[seq] : 0;
-  if (a.positions) {
-    for (int j = threadIdx.x; j < D / 2; j += NW * 32) s_cs[j] = kv8_cos_sin(turns.t[j], pos);
-    __syncthreads();
-  }
-  for (int r = warp; r < 16; r += NW) {
-    constexpr int CH = D / 8;
-    const int chunk = lane % CH;
-    Vec8 x = Vec8{{0u, 0u, 0u, 0u}};
-    if (r < live) {
-      const int t = (r0 + r) / group, h = kvh * group + (r0 + r) % group;
-      x = *reinterpret_cast<const Vec8*>(static_cast<const T*>(a.q) + (row0 + t) * a.ld_q + long(h) * D + chunk * 8);
-    }
-    if (a.positions) {
-      Vec8 oth;
+  uint4 kb[ST][2 * KW];
+  uint32_t vb[ST][4][VW];
+  auto load = [&](int into, int p) {
+    const long base = (long(max(p, 0)) * a.kv_heads + kvh) * (KV8_BLOCK * D);
+    const uint8_t* kp = a.kcodes + base + g * D + c * 16;
+    const uint8_t* vp = a.vcodes + base + 2 * c * D + g * VB;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) oth.w[i] = __shfl_xor_sync(0xffffffffu, x.w[i], CH / 2);
-      x = kv8_rotate8<T>(x, oth, chunk < CH / 2, s_cs + (chunk % (CH / 2)) * 8);
-    }
-    float up = 1.f, down = 1.f;
-    if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
-      const uint32_t m = kv8_warp_amax<T>(kv8_absmax(0u, x)) >> 23;           // exponent of the largest
-      if (m > 0 && m < 255) {
-        const int e = max(int(m) - 127 - 10, -100);                          // largest to [2^10, 2^11)
-        up = __uint_as_float(uint32_t(127 - e) << 23);
-        down = __uint_as_float(uint32_t(127 + e) << 23);
+    for (int i = 0; i < KW; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) kb[into][2 * i + h] = *reinterpret_cast<const uint4*>(kp + 8 * h * D + i * 64);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint8_t* src = vp + ((k & 1) + 8 * (k >> 1)) * D;
+      if constexpr (VW == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(src);
+        vb[into][k][0] = w.x, vb[into][k][1] = w.y;
+      } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(src);
+        vb[into][k][0] = w.x, vb[into][k][1] = w.y, vb[into][k][2] = w.z, vb[into][k][3] = w.w;
       }
     }
-    if (lane < CH) {
+  };
+  // pages and scales are looked up for 32 blocks at a time, one a lane: pages two such groups ahead, scales one
+  auto page_of = [&](int b) {
+    int p = b < cnt ? bt[b] : -1;
+    if (b < cnt && (p < 0 || p >= a.num_blocks)) kv8_report(a.status), p = -1;
+    return p;
+  };
+  auto scale_of = [&](const float* s, int p) { return p >= 0 ? s[long(p) * a.kv_heads + kvh] : 0.f; };
+  int page = page_of(lane), page1 = page_of(32 + lane), page2 = -1;
+  float kf = scale_of(a.kscale, page), vf = scale_of(a.vscale, page), kf1 = 0.f, vf1 = 0.f;
+  const int early = appends ? min(cnt - 1, ST - 1) : min(cnt, ST - 1);        // the last block waits for its new token
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s)
+    if (s < early) load(s, __shfl_sync(0xffffffffu, page, s));
+
+  // ---- q to shared memory: rotated, scaled to f16
+  if (a.positions) {
+    for (int j = it; j < D / 2; j += WPI * 32) s_cs[j] = kv8_cos_sin(turns.t[j], pos);
+    kv8_item_sync<WPI>(in_cta);
+  }
+  for (int r = iw; r < R; r += WPI) {
+    const int chunk = lane % CH;
+    uint4 h = make_uint4(0u, 0u, 0u, 0u);
+    float down = 0.f;
+    if (r < live) {
+      const int t = (r0 + r) / group, head = kvh * group + (r0 + r) % group;
+      Vec8 x = *reinterpret_cast<const Vec8*>(static_cast<const T*>(a.q) + (row0 + t) * a.ld_q + long(head) * D + chunk * 8);
+      if (a.positions) {
+        Vec8 oth;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) oth.w[i] = __shfl_xor_sync(0xffffffffu, x.w[i], CH / 2);
+        x = kv8_rotate8<T>(x, oth, chunk < CH / 2, s_cs + (chunk % (CH / 2)) * 8);
+      }
+      float up = 1.f;
+      down = 1.f;
+      if constexpr (!std::is_same<T, __half>::value) {
+        const uint32_t m = kv8_warp_amax<T>(kv8_absmax(0u, x)) >> 23;           // exponent of the largest
+        if (m > 0 && m < 255) {
+          const int e = max(int(m) - 127 - 10, -100);                          // largest to [2^10, 2^11)
+          up = __uint_as_float(uint32_t(127 - e) << 23);
+          down = __uint_as_float(uint32_t(127 + e) << 23);
+        }
+      }
       float f[8];
       unpack8<T>(x, f);
-      uint4 h;
       h.x = kv8_half2(f[0] * up, f[1] * up), h.y = kv8_half2(f[2] * up, f[3] * up);
       h.z = kv8_half2(f[4] * up, f[5] * up), h.w = kv8_half2(f[6] * up, f[7] * up);
-      *reinterpret_cast<uint4*>(&s_q[r][chunk * 8]) = h;
     }
+    if (lane < CH) *reinterpret_cast<uint4*>(&s_q[r][chunk * 8]) = h;
     if (lane == 0) s_qs[r] = down * a.scale_log2;
   }
-  // ---- the new token joins its block: the warp that reads that block writes it first (one query per sequence here)
-  if (a.slots && w_hi > w_lo && w_hi == nblk) {
-    const int slot = a.slots[seq];
-    if (slot >= long(a.num_blocks) * KV8_BLOCK) {
+  if (appends) {
+    if (slot >= a.num_blocks * KV8_BLOCK) {
       if (lane == 0) kv8_report(a.status);
-    } else if (slot >= 0) {
-      kv8_append_one<T, D, CODE, false>(a, row0, slot, kvh, s_cs);
-      kv8_append_one<T, D, CODE, true>(a, row0, slot, kvh, s_cs);
+    } else {
+      const float ks = kv8_append_one<T, D, CODE, false>(a, row0, slot, kvh, s_cs);
+      const float vs = kv8_append_one<T, D, CODE, true>(a, row0, slot, kvh, s_cs);
       __syncwarp();
+      if (lane == cnt - 1 && page == slot / KV8_BLOCK) kf = ks, vf = vs;
+    }
+    if (early < ST - 1) {
+#pragma unroll
+      for (int s = 0; s < ST - 1; ++s)
+        if (s == early) load(s, __shfl_sync(0xffffffffu, page, s));
     }
   }
-  __syncthreads();
+  if (vf != vf) kf = vf, vf = 0.f;              // seeing the block's keys is seeing its values: NaN through the scores
+  kv8_item_sync<WPI>(in_cta);
   // Q fragments: k step j of lane c is bytes 4 (j % 4) .. + 3 of its 16 in chunk j / 4 of 64 channels
   uint32_t qa[MT][2 * NT];
 #pragma unroll
@@ -208,9 +269,8 @@ __global__ void __launch_bounds__(NW * 32) kv8_attention_kernel(Kv8AttnArgs a, K
   int lim[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int r = r0 + g + 8 * t;
     qs[t] = s_qs[g + 8 * t];
-    lim[t] = g + 8 * t < live ? (a.causal ? len - (n - 1 - r / group) : len) : 0;
+    lim[t] = g + 8 * t < live ? (a.causal ? len - (n - 1 - (r0 + g + 8 * t) / group) : len) : 0;
   }
   const int first_lim = a.causal ? len - (n - 1 - r0 / group) : len;        // the fewest keys of a live row
 
@@ -224,151 +284,114 @@ __global__ void __launch_bounds__(NW * 32) kv8_attention_kernel(Kv8AttnArgs a, K
       for (int k = 0; k < 4; ++k) o[i][t][k] = 0.f;
   }
   float vref = 0.f;                            // o is in units of vref * 2^-15
-
-  uint4 kb[ST][2 * KW];
-  uint32_t vb[ST][4][VW];
-  // looked up for 32 blocks at a time, one a lane
-  int page = -1;
-  float kf = 0.f, vf = 0.f;
-  auto look_up = [&](int b0) {
-    const int b = b0 + lane;
-    page = b < w_hi ? bt[b] : -1;
-    const bool ok = page >= 0 && page < a.num_blocks;
-    if (!ok && b < w_hi) kv8_report(a.status);
-    if (!ok) page = -1;
-    const long unit = long(ok ? page : 0) * a.kv_heads + kvh;
-    kf = ok ? a.kscale[unit] : 0.f;
-    vf = ok ? a.vscale[unit] : 0.f;
-    if (vf != vf) kf = vf, vf = 0.f;            // seeing the block's keys is seeing its values: NaN through the scores
-  };
-  auto load = [&](int slot_in, int b) {         // b: index within the 32
-    const int p = __shfl_sync(0xffffffffu, page, b);
-    const long base = (long(max(p, 0)) * a.kv_heads + kvh) * (KV8_BLOCK * D);
-    const uint8_t* kp = a.kcodes + base;
-    const uint8_t* vp = a.vcodes + base;
+  for (int bs = 0; bs < cnt; bs += ST) {
 #pragma unroll
-    for (int i = 0; i < KW; ++i)
+    for (int s = 0; s < ST; ++s) {
+      const int b = bs + s;
+      if (b >= cnt) break;
+      if ((b & 31) == 0) {
+        if (b > 0) {
+          page = page1, page1 = page2, kf = kf1, vf = vf1;
+          if (vf != vf) kf = vf, vf = 0.f;
+        }
+        kf1 = scale_of(a.kscale, page1), vf1 = scale_of(a.vscale, page1);
+        page2 = page_of(b + 64 + lane);
+        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vf)));
+        if (top > vref) {
+          const float down = vref * kv8_inverse(top);          // 0 the first time
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        kb[slot_in][2 * i + h] = *reinterpret_cast<const uint4*>(kp + (g + 8 * h) * D + i * 64 + c * 16);
+          for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint8_t* src = vp + (2 * c + (k & 1) + 8 * (k >> 1)) * D + g * VB;
-      if constexpr (VW == 2) {
-        const uint2 w = *reinterpret_cast<const uint2*>(src);
-        vb[slot_in][k][0] = w.x, vb[slot_in][k][1] = w.y;
-      } else {
-        const uint4 w = *reinterpret_cast<const uint4*>(src);
-        vb[slot_in][k][0] = w.x, vb[slot_in][k][1] = w.y, vb[slot_in][k][2] = w.z, vb[slot_in][k][3] = w.w;
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) o[i][t][k] *= down;
+          vref = top;
+        }
+        vf *= kv8_inverse(vref) * 32768.f;
       }
-    }
-  };
-  for (int b0 = w_lo; b0 < w_hi; b0 += 32) {
-    look_up(b0);
-    const int cnt = min(32, w_hi - b0);
-    const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vf)));
-    if (top > vref) {
-      const float down = vref * kv8_inverse(top);          // 0 the first time
+      const int nb = b + ST - 1;
+      if (nb < cnt) load((s + ST - 1) % ST, __shfl_sync(0xffffffffu, ((nb ^ b) & 32) ? page1 : page, nb & 31));
+      // ---- scores
+      float sc[2][4];
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int h = 0; h < 2; ++h) {
+        sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int j = 0; j < MT; ++j) {
+          const uint4& w4 = kb[s][2 * (j / 4) + h];
+          const uint32_t w = (j % 4) == 0 ? w4.x : (j % 4) == 1 ? w4.y : (j % 4) == 2 ? w4.z : w4.w;
+          uint32_t b0, b1;
+          kv8_halves<CODE>(w, b0, b1);
+          kv8_mma(sc[h], qa[j][0], NT == 2 ? qa[j][1] : 0u, qa[j][NT], NT == 2 ? qa[j][NT + 1] : 0u, b0, b1);
+        }
+      }
+      const float kfac = __shfl_sync(0xffffffffu, kf, b & 31), vfac = __shfl_sync(0xffffffffu, vf, b & 31);
+      const bool gone = __shfl_sync(0xffffffffu, page, b & 31) < 0;
+      const int t0 = (w_lo + b) * KV8_BLOCK;
+      const bool edge = gone || t0 + KV8_BLOCK > first_lim;
+      float x[NT][4];                         // (row g + 8 t; tokens 2c, 2c + 1, 2c + 8, 2c + 9)
+      bool rise = false;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[i][t][k] *= down;
-      vref = top;
-    }
-    vf *= kv8_inverse(vref) * 32768.f;
+      for (int t = 0; t < NT; ++t) {
+        const float f = kfac * qs[t];
+        x[t][0] = sc[0][2 * t] * f, x[t][1] = sc[0][2 * t + 1] * f, x[t][2] = sc[1][2 * t] * f, x[t][3] = sc[1][2 * t + 1] * f;
+      }
+      if (edge) {
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s)
-      if (s < cnt) load(s, s);
-    for (int b8 = 0; b8 < cnt; b8 += ST) {
+        for (int k = 0; k < 4; ++k) {
+          const int tok = t0 + 2 * c + (k & 1) + 8 * (k >> 1);
 #pragma unroll
-      for (int s = 0; s < ST; ++s) {
-        const int b = b8 + s;
-        if (b >= cnt) break;
-        if (b + ST - 1 < cnt) load((s + ST - 1) % ST, b + ST - 1);
-        // ---- scores
-        float sc[2][4];
+          for (int t = 0; t < NT; ++t)
+            if (gone || tok >= lim[t]) x[t][k] = -INFINITY;
+          if (gone || tok >= len) {           // bytes behind the context are no codes
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            const uint4& w4 = kb[s][2 * (j / 4) + h];
-            const uint32_t w = (j % 4) == 0 ? w4.x : (j % 4) == 1 ? w4.y : (j % 4) == 2 ? w4.z : w4.w;
-            uint32_t b0r, b1r;
-            kv8_halves<CODE>(w, b0r, b1r);
-            kv8_mma(sc[h], qa[j][0], NT == 2 ? qa[j][1] : 0u, qa[j][NT], NT == 2 ? qa[j][NT + 1] : 0u, b0r, b1r);
+            for (int i = 0; i < VW; ++i) vb[s][k][i] = 0u;
           }
         }
-        const float kfac = __shfl_sync(0xffffffffu, kf, b), vfac = __shfl_sync(0xffffffffu, vf, b);
-        const int t0 = (b0 + b) * KV8_BLOCK;
-        const bool gone = __shfl_sync(0xffffffffu, page, b) < 0;
-        const bool edge = gone || t0 + KV8_BLOCK > first_lim;
-        float x[NT][4];                         // (row g + 8 t; tokens 2c, 2c + 1, 2c + 8, 2c + 9)
-        bool rise = false;
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) rise |= fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])) > m[t];
+      if (__any_sync(0xffffffffu, rise)) {
+        float alpha[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const float f = kfac * qs[t];
-          x[t][0] = sc[0][2 * t] * f, x[t][1] = sc[0][2 * t + 1] * f, x[t][2] = sc[1][2 * t] * f, x[t][3] = sc[1][2 * t + 1] * f;
-          if (edge) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (gone || t0 + 2 * c + (k & 1) + 8 * (k >> 1) >= lim[t]) x[t][k] = -INFINITY;
-          }
-          rise |= fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])) > m[t];
+          float mx = fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          mx = fmaxf(mx, m[t]);
+          alpha[t] = mx == -INFINITY ? 1.f : kv8_exp2(m[t] - mx);
+          l[t] *= alpha[t];
+          m[t] = mx;
         }
-        if (edge) {
-          // bytes behind the context are no codes
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (gone || t0 + 2 * c + (k & 1) + 8 * (k >> 1) >= len) {
-#pragma unroll
-              for (int i = 0; i < VW; ++i) vb[s][k][i] = 0u;
-            }
-        }
-        if (__any_sync(0xffffffffu, rise)) {
-          float alpha[NT];
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            float mx = fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            mx = fmaxf(mx, m[t]);
-            alpha[t] = mx == -INFINITY ? 1.f : kv8_exp2(m[t] - mx);
-            l[t] *= alpha[t];
-            m[t] = mx;
-          }
-          // o's rows run along c: rows 2c and 2c + 1 of the tile, held for scores by lanes g = 2c and 2c + 1
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const float a0 = __shfl_sync(0xffffffffu, alpha[t], 8 * c), a1 = __shfl_sync(0xffffffffu, alpha[t], 8 * c + 4);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) o[i][t][0] *= a0, o[i][t][1] *= a1, o[i][t][2] *= a0, o[i][t][3] *= a1;
-          }
-        }
-        uint32_t p[NT][2];
+        // o's rows run along c: rows 2c and 2c + 1 of the tile, held for scores by lanes g = 2c and 2c + 1
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const float mm = m[t] == -INFINITY ? 0.f : m[t];
-          float e[4];
+          const float a0 = __shfl_sync(0xffffffffu, alpha[t], 8 * c), a1 = __shfl_sync(0xffffffffu, alpha[t], 8 * c + 4);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) e[k] = kv8_exp2(x[t][k] - mm);
-          l[t] += (e[0] + e[1]) + (e[2] + e[3]);
-          p[t][0] = kv8_half2(e[0] * vfac, e[1] * vfac);
-          p[t][1] = kv8_half2(e[2] * vfac, e[3] * vfac);
+          for (int i = 0; i < MT; ++i) o[i][t][0] *= a0, o[i][t][1] *= a1, o[i][t][2] *= a0, o[i][t][3] *= a1;
         }
-        // ---- values: channel tile i has channels 2 i and 2 i + 1 of the lane's
+      }
+      uint32_t p[NT][2];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const int w = i / 2;
-          const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
-          uint32_t a0, a1, a2, a3;
-          kv8_halves<CODE>(__byte_perm(vb[s][0][w], vb[s][1][w], sel), a0, a1);
-          kv8_halves<CODE>(__byte_perm(vb[s][2][w], vb[s][3][w], sel), a2, a3);
+      for (int t = 0; t < NT; ++t) {
+        const float mm = m[t] == -INFINITY ? 0.f : m[t];
+        float e[4];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) kv8_mma(o[i][t], a0, a1, a2, a3, p[t][0], p[t][1]);
-        }
+        for (int k = 0; k < 4; ++k) e[k] = kv8_exp2(x[t][k] - mm);
+        l[t] += (e[0] + e[1]) + (e[2] + e[3]);
+        p[t][0] = kv8_half2(e[0] * vfac, e[1] * vfac);
+        p[t][1] = kv8_half2(e[2] * vfac, e[3] * vfac);
+      }
+      // ---- values: channel tile i has channels 2 i and 2 i + 1 of the lane's
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int w = i / 2;
+        const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
+        uint32_t a0, a1, a2, a3;
+        kv8_halves<CODE>(__byte_perm(vb[s][0][w], vb[s][1][w], sel), a0, a1);
+        kv8_halves<CODE>(__byte_perm(vb[s][2][w], vb[s][3][w], sel), a2, a3);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) kv8_mma(o[i][t], a0, a1, a2, a3, p[t][0], p[t][1]);
       }
     }
   }
@@ -378,7 +401,7 @@ __global__ void __launch_bounds__(NW * 32) kv8_attention_kernel(Kv8AttnArgs a, K
   for (int t = 0; t < NT; ++t) {
     l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
     l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
-    if (c == 0) s_m[warp][g + 8 * t] = m[t], s_l[warp][g + 8 * t] = l[t];
+    if (c == 0) s_m[iw][g + 8 * t] = m[t], s_l[iw][g + 8 * t] = l[t];
   }
   const float unit = vref * (1.f / 32768.f);
   // o[i][t][k]: channel g * VB + 2 i + (k >> 1), row 2c + (k & 1) + 8 t
@@ -388,27 +411,27 @@ __global__ void __launch_bounds__(NW * 32) kv8_attention_kernel(Kv8AttnArgs a, K
     for (int k = 0; k < 2; ++k) {
       const int r = 2 * c + k + 8 * t;
       if (r < live) {
-        float* dst = s_o + (warp * R + r) * D + g * VB;
+        float* dst = s_o + (iw * R + r) * D + g * VB;
 #pragma unroll
         for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[i][t][k] * unit, o[i][t][k + 2] * unit);
       }
     }
-  __syncthreads();
-  const long item = (long(blockIdx.y) * gridDim.x + blockIdx.x) * a.splits + blockIdx.z;
-  for (int i = threadIdx.x; i < live * (D / 2); i += NW * 32) {
+  kv8_item_sync<WPI>(in_cta);
+  const long share = (long(blockIdx.y) * a.items_x + x_item) * a.splits + blockIdx.z;
+  for (int i = it; i < live * (D / 2); i += WPI * 32) {
     const int r = i / (D / 2), ch = (i % (D / 2)) * 2;
     float mx = s_m[0][r];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) mx = fmaxf(mx, s_m[w][r]);
+    for (int w = 1; w < WPI; ++w) mx = fmaxf(mx, s_m[w][r]);
     float s0 = 0.f, s1 = 0.f, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
+    for (int w = 0; w < WPI; ++w) {
       const float f = kv8_weight(s_m[w][r], s_l[w][r], mx);
       const float2 v = *reinterpret_cast<const float2*>(s_o + (w * R + r) * D + ch);
       if (f != 0.f) s0 += f * v.x, s1 += f * v.y, sum += f * s_l[w][r];
     }
     if (a.splits > 1) {
-      float* dst = a.part + (item * a.part_rows + r) * (D + 2);
+      float* dst = a.part + (share * a.part_rows + r) * (D + 2);
       *reinterpret_cast<float2*>(dst + ch) = make_float2(s0, s1);
       if (ch == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mx, sum);
     } else {
@@ -422,7 +445,7 @@ __global__ void __launch_bounds__(NW * 32) kv8_attention_kernel(Kv8AttnArgs a, K
 
 // The shares of a row together: one warp for each row of each tile.
 template <class T, int D>
-__global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8AttnArgs a, long tiles, int items_x) {
+__global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8AttnArgs a, long tiles) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31;
@@ -430,7 +453,7 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8AttnArgs a, long ti
   const long tile = unit / a.part_rows;
   const int r = int(unit - tile * a.part_rows);
   if (tile >= tiles) return;
-  const int x = int(tile % items_x), r0 = int(tile / items_x) * 16;
+  const int x = int(tile % a.items_x), r0 = int(tile / a.items_x) * 16;
   const int seq = x / a.kv_heads, kvh = x - seq * a.kv_heads, group = a.heads / a.kv_heads;
   const int n = a.q_len ? a.q_len[seq] : 1;
   if (r0 + r >= n * group || r >= 16) return;
@@ -463,33 +486,58 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8AttnArgs a, long ti
 
 using namespace ronn;
 
-// How many CTAs share the blocks of one tile: enough for two waves' worth of CTAs, each with at least four blocks a warp.
-static int kv8_splits(long tiles, int max_ctx) {
-  const long want = 2L * device_sm_count();
-  const long by_work = max_ctx / (KV8_BLOCK * KV8_NW * 4);
-  long s = tiles > 0 ? want / tiles : 1;
-  if (s > by_work) s = by_work;
-  return int(s < 1 ? 1 : s > 64 ? 64 : s);
+struct Kv8Plan {
+  int wpi, splits, share;      // warps of an item, CTAs along a context, cache blocks each of them takes
+};
+
+// Warps of an item: two where that gives every SM's schedulers at least two rounds of warps, else four.  A context is cut
+// into equal shares, whatever its row's length, so that long rows give more CTAs and not longer ones; shares are taken for
+// about six CTAs an SM at the longest context, of 64 blocks at least.
+static Kv8Plan kv8_plan(long tiles, int max_ctx) {
+  const int sms = device_sm_count(), nblk = (max_ctx + KV8_BLOCK - 1) / KV8_BLOCK;
+  const char* e = getenv("KV8_WPI");
+  Kv8Plan p{tiles >= 8L * sms ? 2 : 4, 1, nblk > 0 ? nblk : 1};
+  if (e) p.wpi = atoi(e);
+  const long want = tiles > 0 ? 6L * sms / tiles : 1;
+  if (want > 1 && nblk > 64) {
+    const long share = (nblk + want - 1) / want;
+    p.share = int(share < 64 ? 64 : share);
+    p.splits = (nblk + p.share - 1) / p.share;
+    if (p.splits > 1) p.wpi = 4;
+  }
+  return p;
 }
 
 // Bytes of scratch that ronn_kv8_attention needs for these sizes; 0 where one CTA takes a whole tile.
 extern "C" long ronn_kv8_attention_scratch(int n_seq, int max_q_len, int max_ctx, int heads, int kv_heads, int head_dim) {
   if (n_seq <= 0 || max_q_len <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
   const long rows = long(max_q_len) * (heads / kv_heads), tiles = (rows + 15) / 16 * n_seq * kv_heads;
-  const int s = kv8_splits(tiles, max_ctx);
+  const int s = kv8_plan(tiles, max_ctx).splits;
   return s <= 1 ? 0 : tiles * s * (rows < 16 ? rows : 16) * (head_dim + 2) * long(sizeof(float));
 }
 
-// q, out: 16-bit [rows, ld]; dtype 0 bf16, 1 fp16; code 0 int8, 1 e4m3; head_dim 64 or 128.  max_q_len bounds q_len, max_ctx
-// sizes the launch.  slots (one query per sequence): the new K and V of row s are at columns k_off and v_off of q's row and
-// join the cache at slots[s]; positions and turns (kv8_append): rotary embedding of q and the new k.
-extern "C" int ronn_kv8_attention(const void* q, long ld_q, long rows, void* kcodes, void* vcodes, float* kscale, float* vscale,
-                                  long num_blocks, const int* tables, long table_ld, int table_rows, int max_blocks,
-                                  const int* bt_row, const int* seq_start, const int* q_len, const int* kv_len, void* out,
-                                  long ld_o, int n_seq, int max_q_len, int max_ctx, int heads, int kv_heads, int head_dim, int causal,
-                                  float scale, int dtype, int code, int k_off, int v_off, const int* slots, const int* positions,
-                                  const unsigned long long* turns, void* scratch, long scratch_bytes, uint32_t* status,
-                                  cudaStream_t stream) {
+// One call.  q, out: 16-bit [rows, ld]; dtype 0 bf16, 1 fp16; code 0 int8, 1 e4m3; head_dim 64 or 128.  max_q_len bounds
+// q_len, max_ctx sizes the launch.  slots (one query per sequence): the new K and V of row s are at columns k_off and v_off of
+// q's row and join the cache at slots[s]; positions and turns (kv8_append): rotary embedding of q and the new k.
+struct Kv8AttnCall {
+  const void* q;
+  void *kcodes, *vcodes;
+  float *kscale, *vscale;
+  const int *tables, *bt_row, *seq_start, *q_len, *kv_len;
+  void* out;
+  const int *slots, *positions;
+  const unsigned long long* turns;
+  void* scratch;
+  uint32_t* status;
+  long ld_q, rows, num_blocks, table_ld, ld_o, scratch_bytes;
+  int table_rows, max_blocks, n_seq, max_q_len, max_ctx, heads, kv_heads, head_dim, causal, dtype, code, k_off, v_off;
+  float scale;
+};
+
+extern "C" int ronn_kv8_attention(const Kv8AttnCall* call, cudaStream_t stream) {
+  const auto& [q, kcodes, vcodes, kscale, vscale, tables, bt_row, seq_start, q_len, kv_len, out, slots, positions, turns, scratch, status,
+               ld_q, rows, num_blocks, table_ld, ld_o, scratch_bytes, table_rows, max_blocks, n_seq, max_q_len, max_ctx, heads, kv_heads,
+               head_dim, causal, dtype, code, k_off, v_off, scale] = *call;
   if (n_seq <= 0 || max_q_len <= 0) return 0;
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || (ld_q & 7) || (ld_o & 7) || max_ctx < 0) return -2;
   if ((seq_start == nullptr) != (q_len == nullptr)) return -2;
@@ -498,24 +546,32 @@ extern "C" int ronn_kv8_attention(const void* q, long ld_q, long rows, void* kco
   if (head_dim != 64 && head_dim != 128) return -1;
   const long group_rows = long(max_q_len) * (heads / kv_heads), mtiles = (group_rows + 15) / 16, xs = long(n_seq) * kv_heads;
   if (xs > 2147483647L || mtiles > 65535) return -2;
-  const int splits = kv8_splits(xs * mtiles, max_ctx);
+  const Kv8Plan plan = kv8_plan(xs * mtiles, max_ctx);
+  const int splits = plan.splits, wpi = plan.wpi;
   const int part_rows = int(group_rows < 16 ? group_rows : 16);
   const long need = ronn_kv8_attention_scratch(n_seq, max_q_len, max_ctx, heads, kv_heads, head_dim);
-  if (splits > 1 && (scratch == nullptr || scratch_bytes < need)) return -4;
+  if (splits > 65535 || (splits > 1 && (scratch == nullptr || scratch_bytes < need))) return -4;
   Kv8Turns tn = {};
   if (positions)
     for (int j = 0; j < head_dim / 2; ++j) tn.t[j] = turns[j];
   Kv8AttnArgs a{q, out, (uint8_t*)kcodes, (uint8_t*)vcodes, kscale, vscale, tables, kv_len, bt_row, seq_start, q_len, slots, positions,
-                (float*)scratch, status, ld_q, ld_o, num_blocks, rows, table_ld, table_rows, max_blocks, heads, kv_heads, causal,
-                splits, part_rows, max_q_len, k_off, v_off, scale * 1.4426950408889634f};
-  const dim3 grid{unsigned(xs), unsigned(mtiles), unsigned(splits)};
+                (float*)scratch, status, ld_q, ld_o, num_blocks, rows, table_ld, int(xs), table_rows, max_blocks, heads, kv_heads, causal,
+                plan.splits, plan.share, part_rows, max_q_len, k_off, v_off, scale * 1.4426950408889634f};
+  const long per_cta = KV8_NW / wpi;
+  const dim3 grid{unsigned((xs + per_cta - 1) / per_cta), unsigned(mtiles), unsigned(splits)};
   const bool small = group_rows <= 8;
 #define RONN_KV8T(T, D, C, NT) \
   do { \
+    if (wpi == 1) RONN_KV8W(T, D, C, NT, 1); \
+    else if (wpi == 2) RONN_KV8W(T, D, C, NT, 2); \
+    else RONN_KV8W(T, D, C, NT, 4); \
+  } while (0)
+#define RONN_KV8W(T, D, C, NT, W) \
+  do { \
     constexpr int smem = KV8_NW * 8 * NT * D * 4; \
-    auto* kern = kv8_attention_kernel<T, D, C, NT, KV8_NW, (D == 64 ? 3 : 2)>; \
+    auto* kern = kv8_attention_kernel<T, D, C, NT, W, (D == 64 ? 3 : 2)>; \
     static bool seen[MAX_DEVICES] = {false}; \
-    if (smem > 32768 && first_use_on_device(seen) && \
+    if (first_use_on_device(seen) && \
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3; \
     launch(kern, grid, dim3(KV8_NW * 32), smem, stream, a, tn); \
   } while (0)
@@ -528,7 +584,7 @@ extern "C" int ronn_kv8_attention(const void* q, long ld_q, long rows, void* kco
     else return -1; \
     if (splits > 1) { \
       const long units = xs * mtiles * part_rows; \
-      launch(kv8_combine_kernel<T, D>, dim3(unsigned((units + 3) / 4)), dim3(128), 0, stream, a, xs * mtiles, int(xs)); \
+      launch(kv8_combine_kernel<T, D>, dim3(unsigned((units + 3) / 4)), dim3(128), 0, stream, a, xs * mtiles); \
     } \
   } while (0)
   if (dtype == 0 && head_dim == 64) RONN_KV8T_(__nv_bfloat16, 64);
@@ -537,6 +593,7 @@ extern "C" int ronn_kv8_attention(const void* q, long ld_q, long rows, void* kco
   else if (dtype == 1) RONN_KV8T_(__half, 128);
   else return -1;
 #undef RONN_KV8T
+#undef RONN_KV8W
 #undef RONN_KV8T_
   return cudaGetLastError() == cudaSuccess ? 0 : -100;
 }

@@ -165,10 +165,21 @@ static int launch_status() { return cudaGetLastError() == cudaSuccess ? 0 : -100
 
 // turns: head_dim / 2 fractions of a turn per position (kv8.cuh) or null without rotary embedding; positions null likewise.
 // dtype 0 bf16, 1 fp16; code 0 int8, 1 e4m3; head_dim 64 or 128.
-extern "C" int ronn_kv8_append(const void* qkv, long ld, void* rotated, long ld_rot, int k_off, int v_off, const int* slots,
-                               const int* positions, const unsigned long long* turns, void* kcodes, void* vcodes, float* kscale,
-                               float* vscale, long num_blocks, long tokens, int heads, int kv_heads, int head_dim, int dtype,
-                               int code, uint32_t* status, cudaStream_t stream) {
+struct Kv8AppendCall {
+  const void* qkv;
+  void* rotated;
+  const int *slots, *positions;
+  const unsigned long long* turns;
+  void *kcodes, *vcodes;
+  float *kscale, *vscale;
+  uint32_t* status;
+  long ld, ld_rot, num_blocks, tokens;
+  int k_off, v_off, heads, kv_heads, head_dim, dtype, code, pad;
+};
+
+extern "C" int ronn_kv8_append(const Kv8AppendCall* call, cudaStream_t stream) {
+  const auto& [qkv, rotated, slots, positions, turns, kcodes, vcodes, kscale, vscale, status, ld, ld_rot, num_blocks, tokens, k_off, v_off,
+               heads, kv_heads, head_dim, dtype, code, pad] = *call;
   if (tokens <= 0) return 0;
   if ((ld & 7) || (ld_rot & 7) || (k_off & 7) || (v_off & 7) || kv_heads <= 0 || heads < 0 || num_blocks < 0) return -2;
   if (positions && (!turns || !rotated)) return -2;
@@ -202,9 +213,18 @@ extern "C" int ronn_kv8_append(const void* qkv, long ld, void* rotated, long ld_
 }
 
 // blocks: [n] cache blocks; kout, vout: [n, kv_heads, 16, head_dim].  A block outside the cache gives zeros and a status code.
-extern "C" int ronn_kv8_read(const void* kcodes, const void* vcodes, const float* kscale, const float* vscale, const int* blocks,
-                             void* kout, void* vout, long n, long num_blocks, int kv_heads, int head_dim, int dtype, int code,
-                             uint32_t* status, cudaStream_t stream) {
+struct Kv8ReadCall {
+  const void *kcodes, *vcodes;
+  const float *kscale, *vscale;
+  const int* blocks;
+  void *kout, *vout;
+  uint32_t* status;
+  long n, num_blocks;
+  int kv_heads, head_dim, dtype, code;
+};
+
+extern "C" int ronn_kv8_read(const Kv8ReadCall* call, cudaStream_t stream) {
+  const auto& [kcodes, vcodes, kscale, vscale, blocks, kout, vout, status, n, num_blocks, kv_heads, head_dim, dtype, code] = *call;
   if (n <= 0) return 0;
   if (kv_heads <= 0 || num_blocks <= 0) return -2;
   const long ctas = (2 * n * kv_heads + 7) / 8;

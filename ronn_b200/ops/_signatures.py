@@ -47,11 +47,11 @@ def declare(lib):
     sig("ronn_kv_append", [V, L, I, I, V, V, V, V, L, I, I, I, F, I, I, V])
     sig("ronn_paged_attention", [V, L, V, V, V, I, V, V, V, L, L, I, I, I, I, F, I, I, I, V, V, F, I, V, V, V])
     sig("ronn_gemm_rownorm", [V, V, V, V, V, V, V, V, I, I, I, I, I, I, F, I, I, V, V], optional=True)
-    sig("ronn_kv8_append", [V, L, V, L, I, I, V, V, V, V, V, V, V, L, L, I, I, I, I, I, V, V])
-    sig("ronn_kv8_read", [V, V, V, V, V, V, V, L, L, I, I, I, I, V, V])
-    sig("ronn_kv8_attention", [V, L, L, V, V, V, V, L, V, L, I, I, V, V, V, V, V, L, I, I, I, I, I, I, I, F, I, I, I, I, V, V, V, V, L, V, V])
+    sig("ronn_kv8_append", [C.c_char_p, V])                     # packed call records (ops/kv8.py)
+    sig("ronn_kv8_read", [C.c_char_p, V])
+    sig("ronn_kv8_attention", [C.c_char_p, V])
     sig("ronn_kv8_attention_scratch", [I, I, I, I, I, I], restype=L)
-    sig("ronn_token_logprobs", [V, L, I, L, V, V, V, V, V, V, I, I, V])
+    sig("ronn_token_logprobs", [V, L, I, L, V, L, I, V, V, V, V, V, I, I, V])
     sig("ronn_fmha", [V, L, L, I, I, I, V, V, V, V, L, I, I, I, I, I, I, F, I, V, V])
     sig("ronn_fmha_paged", [V, L, L, I, V, V, L, V, I, V, V, V, V, V, L, I, I, I, I, I, I, F, I, V, V])
     sig("ronn_conv2d", [V, V, V, V, V, I, I, I, I, I, I, I, I, I, I, I, I, I, I, V, L, V, V], optional=True)

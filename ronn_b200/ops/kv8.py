@@ -10,9 +10,9 @@ stands for is left out, the kernel sets the device's status word, and ``check_st
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
+import struct
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -20,20 +20,25 @@ import torch
 
 from .. import _native
 from . import checks as _checks
-from .kernels import KernelError, OperandError, _DT, _check, _ptr, _run_check, status_word
+from .kernels import OperandError, _check, _run_check, status_word
 
 _CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _PRECISIONS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 _BLOCK = 16
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    return t.data_ptr() % 16 == 0
+# the launchers' call records (kv8_attention.cu, kv8_cache.cu), packed: a decode step is made of calls of a few microseconds, and
+# three dozen arguments one by one cost as much as the kernel
+_APPEND_CALL = struct.Struct("=10Q4q8i")
+_READ_CALL = struct.Struct("=8Q2q4i")
+_ATTENTION_CALL = struct.Struct("=16Q6q13if")
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 class KV8Cache:
     """Codes and scales of one layer's keys and values, or of one rank's share of them."""
-    __slots__ = ("k", "v", "k_scale", "v_scale", "num_blocks", "kv_heads", "head_dim", "code")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_blocks", "kv_heads", "head_dim", "code", "_index", "_pointers", "_status")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dtype not in _CODES or v.dtype != k.dtype:
@@ -45,13 +50,16 @@ class KV8Cache:
                 raise OperandError(f"cache scales must be contiguous fp32 {tuple(k.shape[:2])} on {k.device}, got {s.dtype} "
                                    f"{tuple(s.shape)} on {s.device}")
         for c in (k, v):
-            if not c.is_contiguous() or not _aligned(c) or c.device != k.device:
+            if not c.is_contiguous() or c.data_ptr() % 16 or c.device != k.device:
                 raise OperandError("cache codes must be contiguous from a 16-byte boundary, keys and values on one device")
         if k.shape[0] * _BLOCK > 2 ** 31 - 1:
             raise OperandError(f"cache slots are 32-bit numbers; {k.shape[0]} blocks have more")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_blocks, self.kv_heads, _, self.head_dim = k.shape
         self.code = _CODES[k.dtype]
+        self._index = k.get_device()                        # -1 on the host
+        self._pointers = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        self._status = None
 
     @classmethod
     def alloc(cls, num_blocks: int, kv_heads: int, head_dim: int, precision: str = "int8", device="cuda") -> "KV8Cache":
@@ -71,39 +79,54 @@ class KV8Cache:
         return self.k.dtype
 
 
-def _guard(device: torch.device):
-    """The operands' device for the launch, where it is not the current one."""
-    if device.type != "cuda":
-        raise OperandError(f"the 8-bit cache kernels run on a CUDA device, got a cache on {device}")
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _launch(cache: KV8Cache, fn) -> None:
+    """``fn(library, status word, raw stream)`` on the cache's device, current or not, and that device's current stream."""
+    index = cache._index
+    if index < 0:
+        raise OperandError(f"the 8-bit cache kernels run on a CUDA device, got a cache on {cache.device}")
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _launch(cache, fn)
+    if cache._status is None:
+        cache._status = status_word(cache.device).data_ptr()
+    fn(_native.cuda(), cache._status, _raw_stream(index))
 
 
-def _rows16(what: str, t: torch.Tensor, cols: int, device: torch.device, dtype: Optional[torch.dtype] = None) -> int:
+def _rows16(what: str, t: torch.Tensor, cols: int, index: int, dtype: Optional[torch.dtype] = None) -> int:
     """Row stride of a 16-bit matrix whose rows the kernels read or write in 16-byte pieces."""
-    if t.dim() != 2 or t.dtype not in (torch.bfloat16, torch.float16) or t.device != device or (dtype is not None and t.dtype != dtype):
-        raise OperandError(f"{what} must be a matrix of {dtype or 'bf16 or fp16'} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if t.shape[1] < cols:
-        raise OperandError(f"{what} has {t.shape[1]} columns, {cols} are read or written")
-    ld = t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
-    if t.stride(1) != 1 and t.shape[1] > 1 or ld % 8 or ld < cols or not _aligned(t):
+    if t.dim() != 2 or t.get_device() != index or (t.dtype not in _DTYPES if dtype is None else t.dtype is not dtype):
+        raise OperandError(f"{what} must be a matrix of {dtype or 'bf16 or fp16'} on device {index}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    rows, width = t.shape
+    if width < cols:
+        raise OperandError(f"{what} has {width} columns, {cols} are read or written")
+    ld, unit = t.stride()
+    if rows <= 1:
+        ld = -(-width // 8) * 8
+    if unit != 1 and width > 1 or ld % 8 or ld < cols or t.data_ptr() % 16:
         raise OperandError(f"{what} must have unit column stride and rows that start on 16-byte boundaries and do not overlap, got "
                            f"strides {t.stride()}")
     return ld
 
 
-def _ints(what: str, t: Optional[torch.Tensor], n: int, device: torch.device) -> None:
-    if t is not None and (t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or t.dim() != 1 or t.numel() < n):
-        raise OperandError(f"{what} must be {n} contiguous int32 values on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _ints(what: str, t: torch.Tensor, n: int, index: int) -> int:
+    """Address of n int32 values."""
+    if t.dtype is not torch.int32 or t.get_device() != index or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
+        raise OperandError(f"{what} must be {n} contiguous int32 values on device {index}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
-def _table(block_tables: torch.Tensor, device: torch.device) -> int:
-    t = block_tables
-    if t.dim() != 2 or t.dtype != torch.int32 or t.device != device or (t.stride(1) != 1 and t.shape[1] > 1) or t.shape[1] < 1:
-        raise OperandError(f"block_tables must be an int32 matrix with unit column stride on {device}, got {t.dtype} {tuple(t.shape)}")
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if ld < t.shape[1]:
-        raise OperandError(f"rows of block_tables overlap (strides {t.stride()})")
-    return ld
+def _table(t: torch.Tensor, rows: int, index: int) -> Tuple[int, int, int]:
+    """(row stride, rows, columns) of block tables that need ``rows`` rows (0: are indexed by a vector)."""
+    if t.dim() != 2 or t.dtype is not torch.int32 or t.get_device() != index:
+        raise OperandError(f"block_tables must be an int32 matrix on device {index}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    (n, width), (ld, unit) = t.shape, t.stride()
+    if n <= 1:
+        ld = max(ld, width)
+    if width < 1 or (unit != 1 and width > 1) or ld < width:
+        raise OperandError(f"block_tables must have columns, in unit stride, and rows that do not overlap, got {tuple(t.shape)}, strides {t.stride()}")
+    if n < rows:
+        raise OperandError(f"block_tables has {n} rows for {rows}")
+    return ld, n, width
 
 
 def _heads(heads: int, cache: KV8Cache) -> None:
@@ -118,11 +141,12 @@ def _offset(what: str, off: int) -> None:
 
 @lru_cache(maxsize=64)
 def _turns(head_dim: int, base: float):
-    """base^(-2j/d) / (2 pi) for each channel pair, as 64-bit fractions of a turn."""
+    """base^(-2j/d) / (2 pi) for each channel pair, as 64-bit fractions of a turn: the array, which must live, and its address."""
     if not (base > 0.0 and math.isfinite(base)):
         raise OperandError(f"rotary base must be a positive number, got {base}")
     f = [int(base ** (-2.0 * j / head_dim) / (2.0 * math.pi) * 2.0 ** 64) & (2 ** 64 - 1) for j in range(head_dim // 2)]
-    return (ctypes.c_ulonglong * len(f))(*f)
+    arr = (ctypes.c_ulonglong * len(f))(*f)
+    return arr, ctypes.addressof(arr)
 
 
 def kv8_append(qkv: torch.Tensor, k_off: int, v_off: int, slots: torch.Tensor, cache: KV8Cache, heads: int,
@@ -130,86 +154,91 @@ def kv8_append(qkv: torch.Tensor, k_off: int, v_off: int, slots: torch.Tensor, c
     """Put the K and V columns of a fused QKV activation [tokens, ld] into their cache slots (int32 [tokens], -1: not cached).
     The tokens of one block stand in consecutive rows with rising slots, as a scheduler lists them.  With ``positions`` and
     ``rope_base`` > 0, q and k are rotated first; the rotated columns go to ``rotated`` (laid out as qkv; default: qkv itself)."""
-    d, kvh, dev = cache.head_dim, cache.kv_heads, cache.device
+    d, kvh, index = cache.head_dim, cache.kv_heads, cache._index
     _heads(heads, cache)
     rope = positions is not None and rope_base > 0
     if not rope and rotated is not None:
         raise OperandError("rotated needs positions and a rotary base")
     _offset("k_off", k_off)
     _offset("v_off", v_off)
-    ld = _rows16("qkv", qkv, max(k_off, v_off) + kvh * d, dev)
-    rot = qkv if rotated is None else rotated
-    ld_rot = _rows16("rotated", rot, max(heads * d, k_off + kvh * d), dev, qkv.dtype) if rope else 0
-    if rope and k_off < heads * d:
-        raise OperandError(f"k_off {k_off} lies inside the {heads} heads of q")
-    tokens = qkv.shape[0]
-    if rope and rot.shape[0] < tokens:
-        raise OperandError(f"rotated has {rot.shape[0]} rows for {tokens} tokens")
-    _ints("slots", slots, tokens, dev)
+    ld = _rows16("qkv", qkv, max(k_off, v_off) + kvh * d, index)
+    tokens, rot, ld_rot, pos, turns = qkv.shape[0], 0, 0, 0, 0
+    slot_ptr = _ints("slots", slots, tokens, index)
     if rope:
-        _ints("positions", positions, tokens, dev)
-    with _guard(dev):
+        if k_off < heads * d:
+            raise OperandError(f"k_off {k_off} lies inside the {heads} heads of q")
+        to = qkv if rotated is None else rotated
+        ld_rot = _rows16("rotated", to, k_off + kvh * d, index, qkv.dtype)
+        if to.shape[0] < tokens:
+            raise OperandError(f"rotated has {to.shape[0]} rows for {tokens} tokens")
+        rot, pos, turns = to.data_ptr(), _ints("positions", positions, tokens, index), _turns(d, float(rope_base))[1]
+
+    def go(lib, status, stream):
         if _checks.enabled():
             _run_check(_checks.kv8_append, qkv, slots, cache.k, positions)
-        rc = _native.cuda().ronn_kv8_append(qkv.data_ptr(), ld, rot.data_ptr() if rope else None, ld_rot, k_off, v_off,
-                                            slots.data_ptr(), positions.data_ptr() if rope else None,
-                                            _turns(d, float(rope_base)) if rope else None, cache.k.data_ptr(), cache.v.data_ptr(),
-                                            cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.num_blocks, tokens, heads, kvh,
-                                            d, _DT[qkv.dtype], cache.code, status_word(dev).data_ptr(),
-                                            torch.cuda.current_stream().cuda_stream)
-    _check(rc, "kv8_append")
+        _check(lib.ronn_kv8_append(_APPEND_CALL.pack(qkv.data_ptr(), rot, slot_ptr, pos, turns, *cache._pointers, status, ld, ld_rot,
+                                                     cache.num_blocks, tokens, k_off, v_off, heads, kvh, d, _DTYPES[qkv.dtype],
+                                                     cache.code, 0), stream), "kv8_append")
+    _launch(cache, go)
 
 
 def kv8_read(cache: KV8Cache, blocks: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of whole cache blocks (int32 [n]) as two [n, kv_heads, 16, head_dim] tensors."""
-    dev = cache.device
-    if dtype not in (torch.bfloat16, torch.float16):
+    if dtype not in _DTYPES:
         raise OperandError(f"kv8_read gives bf16 or fp16, not {dtype}")
     n = blocks.numel()
-    _ints("blocks", blocks, n, dev)
-    with _guard(dev):
+    ptr = _ints("blocks", blocks, n, cache._index)
+    out = []
+
+    def go(lib, status, stream):
         if _checks.enabled():
             _run_check(_checks._in_range, "blocks", blocks, 0, cache.num_blocks, "cache blocks")
-        k = torch.empty((n, cache.kv_heads, _BLOCK, cache.head_dim), dtype=dtype, device=dev)
-        v = torch.empty_like(k)
-        rc = _native.cuda().ronn_kv8_read(cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-                                          blocks.data_ptr(), k.data_ptr(), v.data_ptr(), n, cache.num_blocks, cache.kv_heads,
-                                          cache.head_dim, _DT[dtype], cache.code, status_word(dev).data_ptr(),
-                                          torch.cuda.current_stream().cuda_stream)
-    _check(rc, "kv8_read")
-    return k, v
+        both = torch.empty((2, n, cache.kv_heads, _BLOCK, cache.head_dim), dtype=dtype, device=blocks.device)
+        out.extend(both.unbind(0))
+        _check(lib.ronn_kv8_read(_READ_CALL.pack(*cache._pointers, ptr, out[0].data_ptr(), out[1].data_ptr(), status, n, cache.num_blocks,
+                                                 cache.kv_heads, cache.head_dim, _DTYPES[dtype], cache.code), stream), "kv8_read")
+    _launch(cache, go)
+    return out[0], out[1]
 
 
-def _out(out: Optional[torch.Tensor], q: torch.Tensor, rows: int, cols: int) -> Tuple[torch.Tensor, int]:
+def _out(out: Optional[torch.Tensor], q: torch.Tensor, rows: int, cols: int, index: int) -> int:
+    """Row stride of the result, 0 where it is still to be made."""
     if out is None:
-        out = torch.empty((rows, cols), dtype=q.dtype, device=q.device)
-        return out, cols
-    ld = _rows16("out", out, cols, q.device, q.dtype)
+        return 0
+    ld = _rows16("out", out, cols, index, q.dtype)
     if out.shape[0] < rows:
         raise OperandError(f"out has {out.shape[0]} rows for {rows} of q")
-    return out, ld
+    return ld
 
 
 def _scale(scale: Optional[float], d: int) -> float:
-    s = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not math.isfinite(s):
-        raise OperandError(f"scale must be finite, got {s}")
-    return s
+    if scale is None:
+        return d ** -0.5
+    if not math.isfinite(scale):
+        raise OperandError(f"scale must be finite, got {scale}")
+    return float(scale)
 
 
-def _attention(q_ptr, q, ld, rows, cache, tables, table_ld, bt_row, seq_start, q_len, kv_len, out, ld_o, n_seq, max_q, max_ctx, heads, causal,
-               scale, append=None, rope=None) -> int:
-    lib, dev, d = _native.cuda(), cache.device, cache.head_dim
-    max_ctx = min(max_ctx, tables.shape[1] * _BLOCK)
-    need = lib.ronn_kv8_attention_scratch(n_seq, max_q, max_ctx, heads, cache.kv_heads, d)
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None       # this call's own: graphs share none
-    return lib.ronn_kv8_attention(q_ptr, ld, rows, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-                                  cache.num_blocks, tables.data_ptr(), table_ld, tables.shape[0], tables.shape[1], _ptr(bt_row),
-                                  _ptr(seq_start), _ptr(q_len), kv_len.data_ptr(), out.data_ptr(), ld_o, n_seq, max_q, max_ctx, heads,
-                                  cache.kv_heads, d, causal, scale, _DT[q.dtype], cache.code, append[0] if append else 0,
-                                  append[1] if append else 0, append[2].data_ptr() if append else None, rope[0].data_ptr() if rope else None,
-                                  _turns(d, float(rope[1])) if rope else None, _ptr(scratch), need, status_word(dev).data_ptr(),
-                                  torch.cuda.current_stream().cuda_stream)
+def _attention(what, cache, q, q_off, ld, tables, table, bt_row, seq_start, q_len, kv_len, out, ld_o, n_seq, max_q, max_ctx, heads, causal,
+               scale, check, k_off=0, v_off=0, slots=0, positions=0, turns=0) -> torch.Tensor:
+    table_ld, table_rows, width = table
+    result = [out]
+
+    def go(lib, status, stream):
+        if _checks.enabled():
+            check()
+        kvh, d, longest = cache.kv_heads, cache.head_dim, min(max_ctx, width * _BLOCK)
+        if out is None:
+            result[0] = torch.empty((q.shape[0], heads * d), dtype=q.dtype, device=q.device)
+        need = lib.ronn_kv8_attention_scratch(n_seq, max_q, longest, heads, kvh, d)
+        # this call's own: captured graphs and other streams share none
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _check(lib.ronn_kv8_attention(_ATTENTION_CALL.pack(
+            q.data_ptr() + 2 * q_off, *cache._pointers, tables.data_ptr(), bt_row, seq_start, q_len, kv_len, result[0].data_ptr(), slots,
+            positions, turns, scratch.data_ptr() if need else 0, status, ld, q.shape[0], cache.num_blocks, table_ld, ld_o or heads * d, need,
+            table_rows, width, n_seq, max_q, longest, heads, kvh, d, causal, _DTYPES[q.dtype], cache.code, k_off, v_off, scale), stream), what)
+    _launch(cache, go)
+    return result[0]
 
 
 def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, ctx_len: torch.Tensor, heads: int, max_ctx: int,
@@ -221,35 +250,34 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, 
     ``append=(k_off, v_off, slots)`` (decode, one row per sequence): q is the fused QKV activation, and each row's new K and V
     first join the cache at the row's slot, which is that of key ``ctx_len[r] - 1``.  ``rope=(positions, base)`` with
     ``append``: q and the new k are rotated (q in memory stays as it is)."""
-    d, dev, rows = cache.head_dim, cache.device, q.shape[0] if q.dim() else 0
+    d, index = cache.head_dim, cache._index
     _heads(heads, cache)
-    if rope is not None and append is None:
-        raise OperandError("rope needs append: without it q is taken as it is")
-    ld = _rows16("q", q, heads * d if append is None else max(heads * d, max(append[0], append[1]) + cache.kv_heads * d), dev)
-    table_ld = _table(block_tables, dev)
-    _ints("ctx_len", ctx_len, rows, dev)
-    _ints("bt_row", bt_row, rows, dev)
-    if bt_row is None and block_tables.shape[0] < rows:
-        raise OperandError(f"block_tables has {block_tables.shape[0]} rows for {rows} of q")
+    more = {}
+    cols = heads * d
     if append is not None:
-        _ints("slots", append[2], rows, dev)
-        _offset("k_off", append[0])
-        _offset("v_off", append[1])
-    if rope is not None:
-        _ints("positions", rope[0], rows, dev)
-        _turns(d, float(rope[1]))
-    if int(max_ctx) < 0:
+        k_off, v_off, slots = append
+        _offset("k_off", k_off)
+        _offset("v_off", v_off)
+        cols = max(cols, max(k_off, v_off) + cache.kv_heads * d)
+    elif rope is not None:
+        raise OperandError("rope needs append: without it q is taken as it is")
+    ld = _rows16("q", q, cols, index)
+    rows = q.shape[0]
+    table = _table(block_tables, rows if bt_row is None else 0, index)
+    ctx = _ints("ctx_len", ctx_len, rows, index)
+    at = 0 if bt_row is None else _ints("bt_row", bt_row, rows, index)
+    if append is not None:
+        more = dict(k_off=k_off, v_off=v_off, slots=_ints("slots", slots, rows, index))
+        if rope is not None:
+            more.update(positions=_ints("positions", rope[0], rows, index), turns=_turns(d, float(rope[1]))[1])
+    if max_ctx < 0:
         raise OperandError(f"max_ctx is {max_ctx}")
-    sc = _scale(scale, d)
-    with _guard(dev):
-        if _checks.enabled():
-            _run_check(_checks.paged_attention, q, cache.k, block_tables, ctx_len, heads, d, int(max_ctx), bt_row,
-                       append[2] if append else None, rope[0] if rope else None)
-        out, ld_o = _out(out, q, rows, heads * d)
-        rc = _attention(q.data_ptr(), q, ld, rows, cache, block_tables, table_ld, bt_row, None, None, ctx_len, out, ld_o, rows, 1,
-                        int(max_ctx), heads, 0, sc, append, rope)
-    _check(rc, "kv8_attention")
-    return out
+
+    def check():
+        _run_check(_checks.paged_attention, q, cache.k, block_tables, ctx_len, heads, d, int(max_ctx), bt_row,
+                   append[2] if append else None, rope[0] if rope else None)
+    return _attention("kv8_attention", cache, q, 0, ld, block_tables, table, at, 0, 0, ctx, out, _out(out, q, rows, heads * d, index), rows,
+                      1, int(max_ctx), heads, 0, _scale(scale, d), check, **more)
 
 
 def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_tables: torch.Tensor, seq_start: torch.Tensor,
@@ -260,28 +288,22 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
     on ([tokens, ld], head h at column q_off + h * head_dim) and attends to the ``kv_len[s]`` keys that row ``bt_row[s]``
     (default s) of the block tables lists; with ``causal`` its queries are the last positions of that context, and a query in
     front of the first key gives zeros.  The new tokens' K and V are in the cache already.  Returns [tokens, heads * head_dim];
-    rows that belong to no sequence are not written.  ``max_q_len`` and ``max_kv_len`` bound the lengths."""
-    d, dev, tokens = cache.head_dim, cache.device, q.shape[0] if q.dim() else 0
+    rows that belong to no sequence are not written.  ``max_q_len`` bounds the queries of a sequence, ``max_kv_len`` its keys."""
+    d, index = cache.head_dim, cache._index
     _heads(heads, cache)
     _offset("q_off", q_off)
-    ld = _rows16("q", q, q_off + heads * d, dev)
-    table_ld = _table(block_tables, dev)
-    n_seq = seq_start.numel()
-    for name, t in (("seq_start", seq_start), ("q_len", q_len), ("kv_len", kv_len), ("bt_row", bt_row)):
-        _ints(name, t, n_seq, dev)
-    if bt_row is None and block_tables.shape[0] < n_seq:
-        raise OperandError(f"block_tables has {block_tables.shape[0]} rows for {n_seq} sequences")
-    if int(max_q_len) < 0 or int(max_kv_len) < 0:
+    ld = _rows16("q", q, q_off + heads * d, index)
+    tokens, n_seq = q.shape[0], seq_start.numel()
+    table = _table(block_tables, n_seq if bt_row is None else 0, index)
+    start, count, keys = (_ints(name, t, n_seq, index) for name, t in (("seq_start", seq_start), ("q_len", q_len), ("kv_len", kv_len)))
+    at = 0 if bt_row is None else _ints("bt_row", bt_row, n_seq, index)
+    if max_q_len < 0 or max_kv_len < 0:
         raise OperandError(f"max_q_len is {max_q_len}, max_kv_len {max_kv_len}")
-    sc = _scale(scale, d)
-    with _guard(dev):
-        if _checks.enabled():
-            _run_check(_checks.sequences, tokens, seq_start, q_len, kv_len, False, block_tables.shape[1] * _BLOCK)
-            rows_of = bt_row if bt_row is not None else torch.arange(n_seq, device=dev, dtype=torch.int32)
-            _run_check(_checks.paged_attention, kv_len[:n_seq, None], cache.k, block_tables, kv_len, 0, 0,
-                       block_tables.shape[1] * _BLOCK, rows_of)
-        out, ld_o = _out(out, q, tokens, heads * d)
-        rc = _attention(q.data_ptr() + 2 * q_off, q, ld, tokens, cache, block_tables, table_ld, bt_row, seq_start, q_len, kv_len, out, ld_o,
-                        n_seq, int(max_q_len), int(max_kv_len), heads, 1 if causal else 0, sc)
-    _check(rc, "kv8_prefill_attention")
-    return out
+
+    def check():
+        _run_check(_checks.sequences, tokens, seq_start, q_len, kv_len, False, block_tables.shape[1] * _BLOCK)
+        rows_of = bt_row if bt_row is not None else torch.arange(n_seq, device=q.device, dtype=torch.int32)
+        _run_check(_checks.paged_attention, kv_len[:n_seq, None], cache.k, block_tables, kv_len, 0, 0, block_tables.shape[1] * _BLOCK, rows_of)
+    return _attention("kv8_prefill_attention", cache, q, q_off, ld, block_tables, table, at, start, count, keys, out,
+                      _out(out, q, tokens, heads * d, index), n_seq, int(max_q_len), int(max_kv_len), heads, 1 if causal else 0,
+                      _scale(scale, d), check)

@@ -30,26 +30,26 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         raise OperandError(f"token_logprobs needs a matrix of fp32, bf16 or fp16 logits on a CUDA device, got {logits.dtype} "
                            f"{tuple(logits.shape)} on {logits.device}")
     rows, vocab = logits.shape
-    if vocab < 1 or vocab > 2 ** 31 - 1 or (logits.stride(1) != 1 and vocab > 1):
+    if vocab < 1 or vocab > 2 ** 30 or (logits.stride(1) != 1 and vocab > 1):
         raise OperandError(f"logits must have a vocabulary and unit column stride, got {tuple(logits.shape)}, strides {logits.stride()}")
     if not 0 <= int(top) <= min(MAX_TOP, vocab):
         raise OperandError(f"top is {top}; up to {min(MAX_TOP, vocab)} alternatives of {vocab} tokens")
-    dev = logits.device
+    dev, index = logits.device, logits.get_device()
     if tokens is not None:
-        if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 1 or tokens.numel() != rows or tokens.device != dev:
+        if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 1 or tokens.numel() != rows or tokens.get_device() != index:
             raise OperandError(f"tokens must be {rows} int32 or int64 values on {dev}, got {tokens.dtype} {tuple(tokens.shape)} on "
                                f"{tokens.device}")
-    with torch.cuda.device(dev):
-        if tokens is not None:
-            if tokens.dtype == torch.int64:          # beyond 32 bits is outside the vocabulary, not inside after a wrap
-                tokens = torch.where((tokens >= 0) & (tokens < vocab), tokens, torch.full_like(tokens, -1)).to(torch.int32)
-            tokens = tokens.contiguous()
-        f = torch.empty((2, rows), dtype=torch.float32, device=dev)
-        rank = torch.empty(rows, dtype=torch.int32, device=dev)
-        ids = torch.empty((rows, int(top)), dtype=torch.int32, device=dev)
-        tops = torch.empty((rows, int(top)), dtype=torch.float32, device=dev)
-        rc = _native.cuda().ronn_token_logprobs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, vocab, rows, _ptr(tokens),
-                                                f[0].data_ptr(), rank.data_ptr(), f[1].data_ptr(), ids.data_ptr(), tops.data_ptr(),
-                                                int(top), _DT[logits.dtype], torch.cuda.current_stream().cuda_stream)
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return token_logprobs(logits, tokens, top)
+    top = int(top)
+    f = torch.empty((2 + top, rows) if rows else (2, 0), dtype=torch.float32, device=dev)
+    i = torch.empty(((1 + top) * rows,), dtype=torch.int32, device=dev)
+    rank, ids, tops = i[:rows], i[rows:].view(rows, top), f[2:].view(rows, top)
+    wide = tokens is not None and tokens.dtype is torch.int64
+    rc = _native.cuda().ronn_token_logprobs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, vocab, rows, _ptr(tokens),
+                                            (tokens.stride(0) if rows > 1 else 1) if tokens is not None else 0, 1 if wide else 0,
+                                            f.data_ptr(), rank.data_ptr(), f.data_ptr() + 4 * rows, ids.data_ptr(), tops.data_ptr(), top,
+                                            _DT[logits.dtype], torch._C._cuda_getCurrentRawStream(index))
     _check(rc, "token_logprobs")
     return TokenLogprobs(f[0], rank, f[1], ids, tops)
