@@ -19,7 +19,6 @@
 // relative to the largest V scale of the 32 blocks that the warp looks up together.
 #include "kv8.cuh"
 
-#include <stdlib.h>
 #include <type_traits>
 
 namespace ronn {
@@ -495,9 +494,7 @@ struct Kv8Plan {
 // about six CTAs an SM at the longest context, of 64 blocks at least.
 static Kv8Plan kv8_plan(long tiles, int max_ctx) {
   const int sms = device_sm_count(), nblk = (max_ctx + KV8_BLOCK - 1) / KV8_BLOCK;
-  const char* e = getenv("KV8_WPI");
   Kv8Plan p{tiles >= 8L * sms ? 2 : 4, 1, nblk > 0 ? nblk : 1};
-  if (e) p.wpi = atoi(e);
   const long want = tiles > 0 ? 6L * sms / tiles : 1;
   if (want > 1 && nblk > 64) {
     const long share = (nblk + want - 1) / want;
