@@ -171,4 +171,22 @@ __device__ __forceinline__ float kv8_store_run(const Vec8* x, int chunk, int sub
   return s;
 }
 
+// One call.  q, out: 16-bit [rows, ld]; dtype 0 bf16, 1 fp16; code 0 int8, 1 e4m3; head_dim 64 or 128.  max_q_len bounds
+// q_len, max_ctx sizes the launch.  slots (one query per sequence): the new K and V of row s are at columns k_off and v_off of
+// q's row and join the cache at slots[s]; positions and turns (kv8_append): rotary embedding of q and the new k.
+struct Kv8AttnCall {
+  const void* q;
+  void *kcodes, *vcodes;
+  float *kscale, *vscale;
+  const int *tables, *bt_row, *seq_start, *q_len, *kv_len;
+  void* out;
+  const int *slots, *positions;
+  const unsigned long long* turns;
+  void* scratch;
+  uint32_t* status;
+  long ld_q, rows, num_blocks, table_ld, ld_o, scratch_bytes;
+  int table_rows, max_blocks, n_seq, max_q_len, max_ctx, heads, kv_heads, head_dim, causal, dtype, code, k_off, v_off;
+  float scale;
+};
+
 }  // namespace ronn

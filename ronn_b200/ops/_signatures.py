@@ -50,6 +50,9 @@ def declare(lib):
     sig("ronn_kv8_append", [C.c_char_p, V])                     # packed call records (ops/kv8.py)
     sig("ronn_kv8_read", [C.c_char_p, V])
     sig("ronn_kv8_attention", [C.c_char_p, V])
+    sig("ronn_kv8_chunk_attention", [C.c_char_p, V])
+    sig("ronn_kv8_chunk_scratch", [I, I, I, I], restype=L)
+    sig("ronn_kv8_chunk_form", [I, I, I, I, I, I])
     sig("ronn_kv8_attention_scratch", [I, I, I, I, I, I], restype=L)
     sig("ronn_token_logprobs", [V, L, I, L, V, L, I, V, V, V, V, V, I, I, V])
     sig("ronn_fmha", [V, L, L, I, I, I, V, V, V, V, L, I, I, I, I, I, I, F, I, V, V])

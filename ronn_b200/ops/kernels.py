@@ -31,7 +31,7 @@ _STATUS = {}
 _STATUS_NAMES = {1: "TMA stage never arrived", 2: "pipeline stage never released", 3: "accumulator never committed",
                  4: "peer flag never raised", 5: "epilogue never drained",
                  0x5201: "row load of a streaming row-wise kernel never completed",
-                 0x5801: "a cache page, slot or table row outside the 8-bit KV cache was skipped"}
+                 0x5801: "a page, slot, row or length outside the 8-bit KV cache or its call was skipped"}
 
 
 def _stream():

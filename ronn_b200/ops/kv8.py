@@ -220,7 +220,7 @@ def _scale(scale: Optional[float], d: int) -> float:
 
 
 def _attention(what, cache, q, q_off, ld, tables, table, bt_row, seq_start, q_len, kv_len, out, ld_o, n_seq, max_q, max_ctx, heads, causal,
-               scale, check, k_off=0, v_off=0, slots=0, positions=0, turns=0) -> torch.Tensor:
+               scale, check, k_off=0, v_off=0, slots=0, positions=0, turns=0, form=None) -> torch.Tensor:
     table_ld, table_rows, width = table
     result = [out]
 
@@ -230,10 +230,14 @@ def _attention(what, cache, q, q_off, ld, tables, table, bt_row, seq_start, q_le
         kvh, d, longest = cache.kv_heads, cache.head_dim, min(max_ctx, width * _BLOCK)
         if out is None:
             result[0] = torch.empty((q.shape[0], heads * d), dtype=q.dtype, device=q.device)
-        need = lib.ronn_kv8_attention_scratch(n_seq, max_q, longest, heads, kvh, d)
+        chunked = seq_start != 0 and scale > 0 and longest > 0 and (lib.ronn_kv8_chunk_form(n_seq, max_q, longest, heads, kvh, d) if form is None
+                                                                    else form == "expanded")
+        need = (lib.ronn_kv8_chunk_scratch(n_seq, longest, kvh, d) if chunked else
+                lib.ronn_kv8_attention_scratch(n_seq, max_q, longest, heads, kvh, d))
         # this call's own: captured graphs and other streams share none
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        _check(lib.ronn_kv8_attention(_ATTENTION_CALL.pack(
+        call = lib.ronn_kv8_chunk_attention if chunked else lib.ronn_kv8_attention
+        _check(call(_ATTENTION_CALL.pack(
             q.data_ptr() + 2 * q_off, *cache._pointers, tables.data_ptr(), bt_row, seq_start, q_len, kv_len, result[0].data_ptr(), slots,
             positions, turns, scratch.data_ptr() if need else 0, status, ld, q.shape[0], cache.num_blocks, table_ld, ld_o or heads * d, need,
             table_rows, width, n_seq, max_q, longest, heads, kvh, d, causal, _DTYPES[q.dtype], cache.code, k_off, v_off, scale), stream), what)
@@ -283,12 +287,14 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, 
 def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_tables: torch.Tensor, seq_start: torch.Tensor,
                           q_len: torch.Tensor, kv_len: torch.Tensor, max_q_len: int, max_kv_len: int, heads: int,
                           causal: bool = True, bt_row: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-                          scale: Optional[float] = None) -> torch.Tensor:
+                          scale: Optional[float] = None, form: Optional[str] = None) -> torch.Tensor:
     """Attention of query chunks (chunked prompts, prefix hits): sequence s has ``q_len[s]`` queries from row ``seq_start[s]`` of q
     on ([tokens, ld], head h at column q_off + h * head_dim) and attends to the ``kv_len[s]`` keys that row ``bt_row[s]``
     (default s) of the block tables lists; with ``causal`` its queries are the last positions of that context, and a query in
     front of the first key gives zeros.  The new tokens' K and V are in the cache already.  Returns [tokens, heads * head_dim];
-    rows that belong to no sequence are not written.  ``max_q_len`` bounds the queries of a sequence, ``max_kv_len`` its keys."""
+    rows that belong to no sequence are not written.  ``max_q_len`` bounds the queries of a sequence, ``max_kv_len`` its keys.
+    Few queries read the codes as they are ("direct"); for many the contexts are expanded to 16-bit values first and the
+    tensor-core attention runs over those ("expanded", for a positive scale).  ``form`` names one, for measurements."""
     d, index = cache.head_dim, cache._index
     _heads(heads, cache)
     _offset("q_off", q_off)
@@ -297,6 +303,8 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
     table = _table(block_tables, n_seq if bt_row is None else 0, index)
     start, count, keys = (_ints(name, t, n_seq, index) for name, t in (("seq_start", seq_start), ("q_len", q_len), ("kv_len", kv_len)))
     at = 0 if bt_row is None else _ints("bt_row", bt_row, n_seq, index)
+    if form not in (None, "direct", "expanded"):
+        raise OperandError(f"form is 'direct' or 'expanded', not {form!r}")
     if max_q_len < 0 or max_kv_len < 0:
         raise OperandError(f"max_q_len is {max_q_len}, max_kv_len {max_kv_len}")
 
@@ -306,4 +314,4 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
         _run_check(_checks.paged_attention, kv_len[:n_seq, None], cache.k, block_tables, kv_len, 0, 0, block_tables.shape[1] * _BLOCK, rows_of)
     return _attention("kv8_prefill_attention", cache, q, q_off, ld, block_tables, table, at, start, count, keys, out,
                       _out(out, q, tokens, heads * d, index), n_seq, int(max_q_len), int(max_kv_len), heads, 1 if causal else 0,
-                      _scale(scale, d), check)
+                      _scale(scale, d), check, form=form)
