@@ -78,38 +78,48 @@ __device__ __forceinline__ void kv8_unpack4(uint32_t w, float (&f)[4]) {
 
 // Rotary embedding: the angle of pair j at position p is p * base^(-2j/d).  `turns[j]` is base^(-2j/d) / (2 pi) as a
 // 64-bit binary fraction, so p * turns[j] modulo 2^64 is the angle's fraction of a turn, exact to 2^-44 at p = 2^20 (a
-// 32-bit angle is off by 0.004 rad at p = 65536).  Sine and cosine are taken in 64 bits and the rotated value is rounded
-// to 32 bits and then to the activations' type, as a 64-bit tensor is converted: a value next to a rounding border then
+// 32-bit angle is off by 0.004 rad at p = 65536).  Sine and cosine are taken in 64 bits and the rotated value is formed to 44,
+// then rounded to 32 bits and to the activations' type, as a 64-bit tensor is converted: a value next to a rounding border
 // falls on the same side wherever it is computed.
 constexpr int KV8_MAX_HALF = 64;
 struct Kv8Turns {
   unsigned long long t[KV8_MAX_HALF];
 };
-__device__ __forceinline__ double2 kv8_cos_sin(unsigned long long turn, int pos) {
+// Cosine and sine, each as a float and the float that it leaves over: 48 bits.
+__device__ __forceinline__ float4 kv8_cos_sin(unsigned long long turn, int pos) {
   const unsigned long long f = turn * (unsigned long long)(long long)pos;
   double s, c;
   sincospi(double((long long)f) * 1.0842021724855044e-19, &s, &c);       // 2^-63: half turns in [-1, 1)
-  return make_double2(c, s);
+  const float ch = __double2float_rn(c), sh = __double2float_rn(s);
+  return make_float4(ch, __double2float_rn(c - double(ch)), sh, __double2float_rn(s - double(sh)));
 }
-template <class T> __device__ __forceinline__ T kv8_round16(double v);
-template <> __device__ __forceinline__ __half kv8_round16<__half>(double v) { return __float2half_rn(__double2float_rn(v)); }
-template <> __device__ __forceinline__ __nv_bfloat16 kv8_round16<__nv_bfloat16>(double v) { return __float2bfloat16_rn(__double2float_rn(v)); }
 
-// Eight rotated values: `own` the chunk, `oth` the chunk half a head away, `low` whether own is in the first half.
-template <class T>
-__device__ __forceinline__ Vec8 kv8_rotate8(const Vec8& own, const Vec8& oth, bool low, const double2* cs) {
+// a c + b s rounded to 32 bits as if its products and their sum were exact to 2^-44: the products of 16-bit values with the
+// upper parts are a float and the float left over, so is their sum.  (Conversions to and from 64 bits cost four times this:
+// they run at a quarter of a multiplication's rate at best.)
+__device__ __forceinline__ float kv8_turned(float a, float ch, float cl, float b, float sh, float sl) {
+  const float p = __fmul_rn(a, ch), pe = __fmaf_rn(a, ch, -p), q = __fmul_rn(b, sh), qe = __fmaf_rn(b, sh, -q);
+  const float r = __fadd_rn(p, q), z = __fadd_rn(r, -p), e = __fadd_rn(__fadd_rn(p, -__fadd_rn(r, -z)), __fadd_rn(q, -z));
+  return __fadd_rn(r, __fadd_rn(e, __fadd_rn(__fadd_rn(pe, qe), __fmaf_rn(a, cl, __fmul_rn(b, sl)))));
+}
+
+// Eight rotated values: `own` the chunk, `oth` the chunk half a head away, `low` whether own is in the first half.  cs: the
+// pair's angle, the eight of a chunk STEP apart, so that the lanes of a token read neighbouring places.
+template <class T, int STEP>
+__device__ __forceinline__ Vec8 kv8_rotate8(const Vec8& own, const Vec8& oth, bool low, const float4* cs) {
   float a[8], b[8];
   unpack8<T>(own, a);
   unpack8<T>(oth, b);
-  Vec8 r;
-  T* o = reinterpret_cast<T*>(&r);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const double c = cs[i].x, s = low ? -cs[i].y : cs[i].y;
-    o[i] = kv8_round16<T>(fma(double(b[i]), s, double(a[i]) * c));
+    const float4 k = cs[i * STEP];
+    a[i] = kv8_turned(a[i], k.x, k.y, b[i], low ? -k.z : k.z, low ? -k.w : k.w);
   }
-  return r;
+  return pack8<T>(a);
 }
+// Place of pair j of a head of D channels in a table of angles.
+template <int D>
+__device__ __forceinline__ int kv8_angle_at(int j) { return (j % 8) * (D / 16) + j / 8; }
 
 // Largest magnitude of eight 16-bit values as 16-bit patterns, two running maxima in one word.
 __device__ __forceinline__ uint32_t kv8_absmax(uint32_t m, const Vec8& v) {

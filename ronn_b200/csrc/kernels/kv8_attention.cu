@@ -81,7 +81,7 @@ __device__ __forceinline__ void kv8_halves(uint32_t w, uint32_t& lo, uint32_t& h
 
 // The new K (IS_V: V) of one row into its slot, by one warp: kv8_append for a run of one token.  Returns the block's scale.
 template <class T, int D, int CODE, bool IS_V>
-__device__ __forceinline__ float kv8_append_one(const Kv8AttnArgs& a, long row, int slot, int kvh, const double2* cs) {
+__device__ __forceinline__ float kv8_append_one(const Kv8AttnArgs& a, long row, int slot, int kvh, const float4* cs) {
   constexpr int CH = D / 8;
   const int lane = threadIdx.x & 31, chunk = lane % CH;
   const T* src = static_cast<const T*>(a.q) + row * a.ld_q + (IS_V ? a.v_off : a.k_off) + long(kvh) * D;
@@ -90,7 +90,7 @@ __device__ __forceinline__ float kv8_append_one(const Kv8AttnArgs& a, long row, 
     Vec8 oth;
 #pragma unroll
     for (int i = 0; i < 4; ++i) oth.w[i] = __shfl_xor_sync(0xffffffffu, x.w[i], CH / 2);
-    x = kv8_rotate8<T>(x, oth, chunk < CH / 2, cs + (chunk % (CH / 2)) * 8);
+    x = kv8_rotate8<T, CH / 2>(x, oth, chunk < CH / 2, cs + chunk % (CH / 2));
   }
   const long unit = long(slot / KV8_BLOCK) * a.kv_heads + kvh;
   return kv8_store_run<T, D, CODE, 1>(&x, lane < CH ? chunk : -1, 0, 1, slot % KV8_BLOCK, (IS_V ? a.vscale : a.kscale) + unit,
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
   constexpr int CH = D / 8;
   __shared__ alignas(16) __half s_q_all[IPC][R][D];
   __shared__ float s_qs_all[IPC][R];
-  __shared__ double2 s_cs_all[IPC][D / 2];
+  __shared__ float4 s_cs_all[IPC][D / 2];
   __shared__ float s_m_all[KV8_NW][R], s_l_all[KV8_NW][R];
   extern __shared__ float s_o_all[];          // [KV8_NW][R][D]
   pdl_wait();
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
 
   // ---- q to shared memory: rotated, scaled to f16
   if (a.positions) {
-    for (int j = it; j < D / 2; j += WPI * 32) s_cs[j] = kv8_cos_sin(turns.t[j], pos);
+    for (int j = it; j < D / 2; j += WPI * 32) s_cs[kv8_angle_at<D>(j)] = kv8_cos_sin(turns.t[j], pos);
     kv8_item_sync<WPI>(in_cta);
   }
   for (int r = iw; r < R; r += WPI) {
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
         Vec8 oth;
 #pragma unroll
         for (int i = 0; i < 4; ++i) oth.w[i] = __shfl_xor_sync(0xffffffffu, x.w[i], CH / 2);
-        x = kv8_rotate8<T>(x, oth, chunk < CH / 2, s_cs + (chunk % (CH / 2)) * 8);
+        x = kv8_rotate8<T, CH / 2>(x, oth, chunk < CH / 2, s_cs + chunk % (CH / 2));
       }
       float up = 1.f;
       down = 1.f;

@@ -34,19 +34,18 @@ struct Kv8AppendArgs {
 // share of the heads (grid.y).
 constexpr int KV8_AP_WARPS = 8;
 
-template <class T, int D, int CODE>
-__global__ void __launch_bounds__(KV8_AP_WARPS * 32)
+template <class T, int D, int CODE, bool ROPE>
+__global__ void __launch_bounds__(KV8_AP_WARPS * 32, ROPE ? 3 : 4)
 kv8_append_kernel(Kv8AppendArgs a, Kv8Turns turns) {
   constexpr int CH = D / 8;                 // 16-byte chunks (lanes) per token
   constexpr int TPW = 32 / CH;              // tokens per warp pass
   constexpr int PASSES = KV8_BLOCK / TPW;
   constexpr int HALF = D / 2;
-  extern __shared__ double2 s_cs[];         // [16][HALF], with rotary embedding
+  extern __shared__ float4 s_cs[];          // [16][HALF], with rotary embedding
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane / CH, chunk = lane % CH;
-  const bool rope = a.positions != nullptr;
   // the window's 16 rows and the 15 behind them, one per lane
   const long w0 = long(blockIdx.x) * KV8_BLOCK;
   const long row = w0 + lane;
@@ -66,7 +65,7 @@ kv8_append_kernel(Kv8AppendArgs a, Kv8Turns turns) {
                                  : slot == -1 && before == -1 && (row & (KV8_BLOCK - 1)) != 0;
   const uint32_t starts = __ballot_sync(0xffffffffu, !goes_on);          // rows past the end count as starts
   const uint32_t live = __ballot_sync(0xffffffffu, slot != -2);
-  const int q_units = rope ? a.heads : 0;
+  const int q_units = ROPE ? a.heads : 0;
   const int units = q_units + 2 * a.kv_heads;
   const int u0 = blockIdx.y * a.per_cta, u1 = min(units, u0 + a.per_cta);
   const T* qkv = static_cast<const T*>(a.qkv);
@@ -77,10 +76,10 @@ kv8_append_kernel(Kv8AppendArgs a, Kv8Turns turns) {
     const int n = min(later ? __ffs(later) : 32 - first, KV8_BLOCK);     // rows of the run (a block's end ends it)
     const int slot0 = __shfl_sync(0xffffffffu, slot, first);
     const long t0 = w0 + first;
-    if (rope) {
+    if constexpr (ROPE) {
       __syncthreads();                       // the table of the run before has been read
       for (int i = threadIdx.x; i < n * HALF; i += KV8_AP_WARPS * 32)
-        s_cs[i] = kv8_cos_sin(turns.t[i % HALF], a.positions[t0 + i / HALF]);
+        s_cs[i / HALF * HALF + kv8_angle_at<D>(i % HALF)] = kv8_cos_sin(turns.t[i % HALF], a.positions[t0 + i / HALF]);
       __syncthreads();
     }
     for (int u = u0 + warp; u < u1; u += KV8_AP_WARPS) {
@@ -89,7 +88,7 @@ kv8_append_kernel(Kv8AppendArgs a, Kv8Turns turns) {
       const bool is_v = !is_q && kvu >= a.kv_heads;
       const int h = is_q ? u : is_v ? kvu - a.kv_heads : kvu;
       const long col = (is_q ? 0 : is_v ? a.v_off : a.k_off) + long(h) * D + chunk * 8;
-      if (!is_q && slot0 < 0 && (is_v || !rope)) continue;
+      if (!is_q && slot0 < 0 && (is_v || !ROPE)) continue;
       Vec8 x[PASSES];
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {
@@ -97,7 +96,7 @@ kv8_append_kernel(Kv8AppendArgs a, Kv8Turns turns) {
         if (t < n) x[p] = *reinterpret_cast<const Vec8*>(qkv + (t0 + t) * a.ld + col);
         else x[p] = Vec8{{0u, 0u, 0u, 0u}};
       }
-      if (rope && !is_v) {
+      if (ROPE && !is_v) {
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
           const int t = p * TPW + sub;
@@ -105,7 +104,7 @@ kv8_append_kernel(Kv8AppendArgs a, Kv8Turns turns) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) oth.w[i] = __shfl_xor_sync(0xffffffffu, x[p].w[i], CH / 2);
           if (t < n) {
-            x[p] = kv8_rotate8<T>(x[p], oth, chunk < CH / 2, s_cs + t * HALF + (chunk % (CH / 2)) * 8);
+            x[p] = kv8_rotate8<T, CH / 2>(x[p], oth, chunk < CH / 2, s_cs + t * HALF + chunk % (CH / 2));
             *reinterpret_cast<Vec8*>(static_cast<T*>(a.rotated) + (t0 + t) * a.ld_rot + col) = x[p];
           }
         }
@@ -280,8 +279,10 @@ extern "C" int ronn_kv8_append(const Kv8AppendCall* call, cudaStream_t stream) {
   Kv8AppendArgs a{qkv, rotated, slots, positions, (uint8_t*)kcodes, (uint8_t*)vcodes, kscale, vscale, status, ld, ld_rot, tokens,
                   num_blocks * KV8_BLOCK, k_off, v_off, heads, kv_heads, per_cta};
   const dim3 grid{unsigned(windows), unsigned(ys), 1u};
-  const size_t smem = positions ? size_t(KV8_BLOCK) * (head_dim / 2) * sizeof(double2) : 0;
-#define RONN_KV8A(T, D, C) launch(kv8_append_kernel<T, D, C>, grid, dim3(KV8_AP_WARPS * 32), smem, stream, a, tn)
+  const size_t smem = positions ? size_t(KV8_BLOCK) * (head_dim / 2) * sizeof(float4) : 0;
+#define RONN_KV8A(T, D, C) \
+  (positions ? launch(kv8_append_kernel<T, D, C, true>, grid, dim3(KV8_AP_WARPS * 32), smem, stream, a, tn) \
+             : launch(kv8_append_kernel<T, D, C, false>, grid, dim3(KV8_AP_WARPS * 32), smem, stream, a, tn))
 #define RONN_KV8A_(T) \
   do { \
     if (head_dim == 64 && code == 0) RONN_KV8A(T, 64, 0); \
