@@ -5,8 +5,8 @@ the device pool, the host pool and the memory budget.
 
 The state itself lives in the native scheduler (``csrc/serving/scheduler.cc``: block pool, reference counts, page tables,
 host-pool assignments of swapped-out sequences) and in the engine (the cache tensors); nothing is duplicated here.
-Blocks hold 16 tokens.  Cache precision is the engine's compute dtype: the quantised cache precisions of the design are
-listed for parity of the vocabulary, and asking for one raises.
+Blocks hold 16 tokens.  Cache precision is the engine's compute dtype, or 8 bits with ``EngineConfig.kv_cache_dtype``; the
+narrower precisions of the design are listed for parity of the vocabulary, and asking for one raises.
 """
 from __future__ import annotations
 
@@ -30,6 +30,7 @@ class CachePrecision(enum.Enum):
     FP16 = "fp16"
     BF16 = "bf16"
     INT8 = "int8"
+    FP8 = "fp8"
     INT4 = "int4"
     INT2 = "int2"
     INT1 = "int1"
@@ -37,14 +38,14 @@ class CachePrecision(enum.Enum):
     @staticmethod
     def of(dtype: torch.dtype) -> "CachePrecision":
         table = {torch.float32: CachePrecision.FP32, torch.float16: CachePrecision.FP16,
-                 torch.bfloat16: CachePrecision.BF16}
+                 torch.bfloat16: CachePrecision.BF16, torch.int8: CachePrecision.INT8, torch.float8_e4m3fn: CachePrecision.FP8}
         if dtype not in table:
             raise SessionError(f"no cache precision for {dtype}")
         return table[dtype]
 
     def require_supported(self) -> "CachePrecision":
-        if self in (CachePrecision.INT8, CachePrecision.INT4, CachePrecision.INT2, CachePrecision.INT1):
-            raise SessionError(f"KV cache precision {self.value} is not implemented (quantised caches are out of scope)")
+        if self in (CachePrecision.INT4, CachePrecision.INT2, CachePrecision.INT1):
+            raise SessionError(f"KV cache precision {self.value} is not implemented (8 bits are the fewest)")
         return self
 
 
@@ -95,9 +96,8 @@ class BlockManager:
 
     @property
     def block_bytes(self) -> int:
-        """Bytes of one block over all layers, keys and values."""
-        k = self._e.runner.kcache[0]
-        return 2 * len(self._e.runner.kcache) * k[0].numel() * k.element_size()
+        """Bytes of one block over all layers, keys and values, with their scales."""
+        return sum(t[0].numel() * t.element_size() for t in self._e.runner.cache_tensors())
 
     @property
     def gpu_pool(self) -> Dict[str, int]:

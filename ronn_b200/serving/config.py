@@ -23,6 +23,7 @@ class EngineConfig:
     eos_token_id: int = -1              # -1 = never stop on a token
     use_cuda_graph: bool = True
     dtype: str = "bf16"
+    kv_cache_dtype: str = "auto"        # "auto" (dtype) | "int8" | "fp8": 8-bit codes with a scale for each block and KV head
     tp_size: int = 1
     backend: str = "kernels"            # "kernels" (hand-written sm_100a) | "torch" (library baseline / CPU)
     tp_comm: str = "fused"              # "fused" (in-kernel NVLink) | "nccl" (library collectives baseline)
@@ -37,6 +38,8 @@ class EngineConfig:
     def __post_init__(self):
         if self.block_size != 16:
             raise ValueError("the paged attention kernels are built for 16-token blocks")
+        if self.kv_cache_dtype not in ("auto", "int8", "fp8"):
+            raise ValueError(f"kv_cache_dtype is 'auto', 'int8' or 'fp8', not '{self.kv_cache_dtype}'")
         for k in ("max_num_seqs", "max_batch_tokens", "max_model_len", "decode_streams", "cluster_norm"):
             env = os.environ.get("RONN_" + k.upper())
             if env:

@@ -20,9 +20,12 @@ from ..api.errors import SessionError
 from .config import EngineConfig
 from .metrics import EngineMetrics
 from .model_runner import DecoderArch, DecoderRunner, NoComm
-from .request import FinishReason, Priority, Request, RequestState, SamplingParams
+from .request import FinishReason, Priority, Request, RequestState, SamplingParams, TokenLogprob
 from .sampler import sample_tokens
 from .scheduler import PLAN_DECODE, PLAN_NONE, PLAN_PREFILL, HostBatchBuffers, Scheduler
+
+MAX_LOGPROBS = 32       # alternatives a request can ask for
+
 
 class StepOutput:
     """What one iteration produced: ids of the requests that got a token, the tokens, and finish codes
@@ -46,13 +49,13 @@ class StepOutput:
 _BUCKETS = [1, 2, 4, 8, 16, 32, 64, 96, 128, 160, 192, 224, 256, 320, 384, 448, 512, 768, 1024]
 
 
-def classify_prefill_step(token_item: np.ndarray, positions: np.ndarray, n_items: int):
+def classify_prefill_step(token_item: np.ndarray, positions: np.ndarray, n_items: int, min_tokens: int = 32):
     """Which attention kernel a prefill step takes, from the item index and the position of each of its tokens (items
     occupy consecutive token ranges).  ``("dense", lens)``: every item is a whole prompt from position 0, attention
     reads K and V from the fused qkv buffer.  ``("paged", starts, lens, first_pos)``: some item continues a chunked
     prompt or starts behind a prefix-cache hit, the tensor-core kernel reads the paged cache; its 128-query tiles do
-    not pay for a handful of tokens per item, so steps under 32 tokens per item on average return None (per-row
-    kernel), as do steps whose tokens are not grouped by item."""
+    not pay for a handful of tokens per item, so steps under ``min_tokens`` tokens per item on average return None
+    (per-row kernel), as do steps whose tokens are not grouped by item."""
     n_tokens = len(token_item)
     starts = np.flatnonzero(np.diff(token_item, prepend=-1))
     if n_tokens == 0 or len(starts) != n_items:
@@ -61,7 +64,7 @@ def classify_prefill_step(token_item: np.ndarray, positions: np.ndarray, n_items
     first_pos = positions[starts]
     if not first_pos.any():
         return ("dense", lens)
-    if n_tokens < 32 * n_items:
+    if n_tokens < min_tokens * n_items:
         return None
     return ("paged", starts, lens, first_pos)
 
@@ -96,6 +99,9 @@ class LLMEngine:
             shape = (n_cpu,) + tuple(self.runner.kcache[0].shape[1:])
             self._cpu_k = [torch.empty(shape, dtype=self.runner.kcache[0].dtype) for _ in self.runner.kcache]
             self._cpu_v = [torch.empty(shape, dtype=self.runner.kcache[0].dtype) for _ in self.runner.kcache]
+            if self.runner.kv8 is not None:              # the blocks' scales go with their codes
+                shape = shape[:2]
+                self._cpu_scales = [[torch.empty(shape) for _ in self.runner.kv8] for _ in range(2)]
         max_tokens = max(self.cfg.max_batch_tokens, self.cfg.max_num_seqs)
         self.host = HostBatchBuffers(max_tokens, self.cfg.max_num_seqs, self.max_blocks, pin=self.device.type == "cuda")
         self.dev_buf = torch.zeros(self.host.total, dtype=torch.int32, device=self.device)
@@ -120,6 +126,7 @@ class LLMEngine:
         self.kernel_launches_last = 0
         self.on_token: Optional[Callable[[Request, int], None]] = None
         self._non_greedy = 0
+        self._logprob_tops: Dict[int, int] = {}          # unfinished requests that ask for log probabilities: their alternatives
         self._watch_count = 0
         self._replayed_launches = 0
         self._h2d_sampling = 0
@@ -161,6 +168,8 @@ class LLMEngine:
         if len(toks) + params.max_new_tokens > self.cfg.max_model_len:
             raise SessionError(f"prompt ({len(toks)}) + max_new_tokens ({params.max_new_tokens}) exceeds "
                                f"max_model_len ({self.cfg.max_model_len})")
+        if params.logprobs is not None and not 0 <= int(params.logprobs) <= min(MAX_LOGPROBS, self.arch.vocab):
+            raise SessionError(f"logprobs is {params.logprobs}; up to {min(MAX_LOGPROBS, self.arch.vocab)} alternatives")
         rid = self._next_id if request_id is None else int(request_id)
         self._next_id = max(self._next_id, rid) + 1
         self.sched.add(rid, toks, params.max_new_tokens, int(priority))
@@ -171,6 +180,9 @@ class LLMEngine:
             self._non_greedy += 1
         if params.stop_sequences:
             self._watch_count += 1
+        if params.logprobs is not None:
+            r.output_logprobs = []
+            self._logprob_tops[rid] = int(params.logprobs)
         self.metrics.requests_added += 1
         return rid
 
@@ -197,6 +209,7 @@ class LLMEngine:
             self._non_greedy -= 1
         if r.params.stop_sequences:
             self._watch_count -= 1
+        self._logprob_tops.pop(r.id, None)
         if not cancel:
             self.metrics.requests_finished += 1
         self._finished_order.append(r.id)
@@ -258,16 +271,21 @@ class LLMEngine:
         if self._cpu_k is None:
             return
         o_src, o_dst, i_src, i_dst = self.sched.swaps()
+        pools = [(self.runner.kcache, self._cpu_k), (self.runner.vcache, self._cpu_v)]
+        if self.runner.kv8 is not None:
+            raw = lambda ts: [t.view(torch.uint8) for t in ts]
+            pools = [(raw(d), raw(c)) for d, c in pools] + [([c.k_scale for c in self.runner.kv8], self._cpu_scales[0]),
+                                                             ([c.v_scale for c in self.runner.kv8], self._cpu_scales[1])]
         if len(o_src):
             src = torch.as_tensor(o_src, dtype=torch.long, device=self.device)
             dst = torch.as_tensor(o_dst, dtype=torch.long)
-            for dev_c, cpu_c in ((self.runner.kcache, self._cpu_k), (self.runner.vcache, self._cpu_v)):
+            for dev_c, cpu_c in pools:
                 for l in range(len(dev_c)):
                     cpu_c[l].index_copy_(0, dst, dev_c[l].index_select(0, src).cpu())
         if len(i_src):
             src = torch.as_tensor(i_src, dtype=torch.long)
             dst = torch.as_tensor(i_dst, dtype=torch.long, device=self.device)
-            for dev_c, cpu_c in ((self.runner.kcache, self._cpu_k), (self.runner.vcache, self._cpu_v)):
+            for dev_c, cpu_c in pools:
                 for l in range(len(dev_c)):
                     dev_c[l].index_copy_(0, dst, cpu_c[l].index_select(0, src).to(self.device))
         self.metrics.swapped_blocks += len(o_src) + len(i_src)
@@ -296,17 +314,22 @@ class LLMEngine:
         n_launch0 = lib.launches if lib is not None else 0
         self._replayed_launches = 0
         try:
+            top = self._logprob_top(sb.req_ids[:n_items])
+            scores = None
             if decode and self.use_graph and self._non_greedy == 0:
-                toks = self._decode_graph(n_items)
+                toks = self._decode_graph(n_items, top=top)
             elif decode and self.use_graph and self.device_sampling:
                 self._stage_sampling(sb.req_ids[:n_items], self._bucket(n_items))
-                toks = self._decode_graph(n_items, sample=True)
+                toks = self._decode_graph(n_items, sample=True, top=top)
             else:
                 self._upload(n_tokens, n_items)
                 b = self._batch_views(n_tokens, n_items)
                 if not decode:
                     b["dense_plan"] = self._dense_prefill_plan(n_tokens, n_items)
-                toks = self._run_and_sample(b, decode, n_tokens, n_items, sb.req_ids)
+                toks = self._run_and_sample(b, decode, n_tokens, n_items, sb.req_ids, top)
+            if top is not None:
+                toks, scores = toks
+                scores = [t[:n_items].to("cpu", non_blocking=False) for t in scores]
             self.sampled_host[:n_items].copy_(toks[:n_items], non_blocking=True)
             status = self.runner.ops.status_tensor()
             if status is not None:                       # rides the same synchronisation as the sampled tokens
@@ -327,6 +350,8 @@ class LLMEngine:
         req_ids = sb.req_ids.copy()
         fin = self.sched.commit(sampled, self.cfg.eos_token_id)
         now = time.perf_counter()
+        if scores is not None:
+            self._record_logprobs(req_ids, sampled, samples_mask, scores)
         if not decode:                                   # first tokens are born in prefill steps
             for i in np.nonzero(samples_mask)[0]:
                 r = self.requests[int(req_ids[i])]
@@ -368,7 +393,9 @@ class LLMEngine:
         if self.cfg.backend != "kernels" or self.device.type != "cuda" or not self.cfg.dense_prefill:
             return None
         h = self.host
-        kind = classify_prefill_step(h.field("token_item")[:n_tokens], h.field("positions")[:n_tokens], n_items)
+        # the 8-bit cache's kernel shares a block's codes among a sequence's queries, however few
+        kind = classify_prefill_step(h.field("token_item")[:n_tokens], h.field("positions")[:n_tokens], n_items,
+                                     1 if self.runner.kv8 is not None else 32)
         if kind is None:
             return None
         from ..ops import kernels as K
@@ -377,18 +404,44 @@ class LLMEngine:
         _, starts, lens, first_pos = kind
         mk = lambda v: torch.tensor(np.asarray(v, dtype=np.int32), device=self.device)
         return {"paged": True, "seq_start": mk(starts), "q_len": mk(lens), "kv_len": mk(first_pos + lens),
-                "max_q_len": int(lens.max()), "n_seq": n_items}
+                "max_q_len": int(lens.max()), "max_kv_len": int((first_pos + lens).max()), "n_seq": n_items}
 
-    def _run_and_sample(self, b, decode, n_tokens, n_items, req_ids) -> torch.Tensor:
+    def _run_and_sample(self, b, decode, n_tokens, n_items, req_ids, top=None):
+        """The step's tokens, and with ``top`` their log probabilities and that many alternatives."""
         greedy = self._non_greedy == 0 or all(self.requests[int(i)].params.temperature <= 0 for i in req_ids)
-        if greedy:
+        if greedy and top is None:
             return self.runner.forward(b, decode, n_tokens, n_items)
         logits = self.runner.forward(b, decode, n_tokens, n_items, want_logits=True)
+        if greedy:
+            return self._with_logprobs(self.runner.ops.argmax(logits), logits, top)
+        own = logits if top is None else logits.clone()              # the sampler's penalties change what it is given
         if self.device_sampling:
             self._stage_sampling(req_ids[:n_items], n_items)
-            return self._sample_on_device(logits, n_items)
-        reqs = [self.requests[int(i)] for i in req_ids]
-        return sample_tokens(logits, reqs, base_seed=self._samp_seed if self.runner.tp > 1 else None)
+            toks = self._sample_on_device(own, n_items)
+        else:
+            reqs = [self.requests[int(i)] for i in req_ids]
+            toks = sample_tokens(own, reqs, base_seed=self._samp_seed if self.runner.tp > 1 else None)
+        return toks if top is None else self._with_logprobs(toks, logits, top)
+
+    # ------------------------------------------------------------------ log probabilities
+    def _logprob_top(self, req_ids) -> Optional[int]:
+        """Alternatives that this step's requests ask for, in few sizes so that few decode graphs are captured; None: no
+        request asks for log probabilities."""
+        if not self._logprob_tops:
+            return None
+        most = max((self._logprob_tops.get(int(i), -1) for i in req_ids), default=-1)
+        return None if most < 0 else min(next(n for n in (0, 5, 20, MAX_LOGPROBS) if n >= most), self.arch.vocab)
+
+    def _with_logprobs(self, toks: torch.Tensor, logits: torch.Tensor, top: int):
+        return toks, self.runner.ops.token_logprobs(logits[:, :self.arch.vocab], toks, top)
+
+    def _record_logprobs(self, req_ids, sampled, samples_mask, scores) -> None:
+        lp, rank, ent, ids, tops = (t.tolist() for t in scores)
+        for i in np.nonzero(samples_mask)[0]:
+            r = self.requests[int(req_ids[i])]
+            n = r.params.logprobs
+            if n is not None:
+                r.output_logprobs.append(TokenLogprob(int(sampled[i]), lp[i], rank[i], ent[i], list(zip(ids[i][:n], tops[i][:n]))))
 
     # ------------------------------------------------------------------ device-side sampling
     def _stage_sampling(self, req_ids, rows: int) -> None:
@@ -431,7 +484,7 @@ class LLMEngine:
                 return bsz
         return self.cfg.max_num_seqs
 
-    def _decode_graph(self, n_items: int, sample: bool = False) -> torch.Tensor:
+    def _decode_graph(self, n_items: int, sample: bool = False, top: Optional[int] = None):
         bsz = self._bucket(n_items)
         h = self.host
         if bsz > n_items:       # pad rows: no cache slot, no context
@@ -441,11 +494,18 @@ class LLMEngine:
             h.field("seq_lens")[n_items:bsz] = 0
             h.field("block_tables")[n_items * self.max_blocks: bsz * self.max_blocks] = 0
         self._upload(bsz, bsz)
-        key = (bsz, self.runner.step_ctx, sample)
+        key = (bsz, self.runner.step_ctx, sample, top)
         entry = self._graphs.get(key)
         if entry is None:
-            parts = None if sample else self._split_rows(bsz)
-            if sample:
+            parts = None if sample or top is not None else self._split_rows(bsz)
+            if top is not None:
+                b = self._batch_views(bsz, bsz)
+
+                def run():
+                    logits = self.runner.forward(b, True, bsz, bsz, want_logits=True)
+                    toks = self._sample_on_device(logits.clone(), bsz) if sample else self.runner.ops.argmax(logits)
+                    return self._with_logprobs(toks, logits, top)
+            elif sample:
                 b = self._batch_views(bsz, bsz)
                 run = lambda: self._sample_on_device(self.runner.forward(b, True, bsz, bsz, want_logits=True), bsz)
             elif parts is None:

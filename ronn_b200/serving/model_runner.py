@@ -172,10 +172,20 @@ class DecoderRunner:
             from ..models.bitnet_llama import load_decoder_weights
             load_decoder_weights(self, init)
 
+    def cache_tensors(self) -> List[torch.Tensor]:
+        """Everything a cache block consists of, over all layers; the first dimension is the block."""
+        if self.kv8 is None:
+            return [*self.kcache, *self.vcache]
+        return [t for c in self.kv8 for t in (c.k, c.v, c.k_scale, c.v_scale)]
+
     def _alloc_cache(self) -> None:
         a = self.arch
+        self.kv8 = None if self.cfg.kv_cache_dtype == "auto" else []       # one KV8Cache a layer
+        if self.kv8 is not None and a.head_dim not in (64, 128):
+            raise SessionError(f"an 8-bit KV cache needs heads of 64 or 128 channels, this model has {a.head_dim}")
         if self.num_blocks <= 0:
-            per_block = a.n_layer * 2 * self.n_kv_local * KV_BLOCK * a.head_dim * torch.finfo(self.dtype).bits // 8
+            bits = torch.finfo(self.dtype).bits if self.kv8 is None else 8
+            per_block = a.n_layer * 2 * self.n_kv_local * (KV_BLOCK * a.head_dim * bits // 8 + (0 if self.kv8 is None else 4))
             want = self.cfg.max_num_seqs * self.max_blocks_per_seq
             if self.device.type == "cuda":
                 free, _ = torch.cuda.mem_get_info(self.device)
@@ -184,6 +194,11 @@ class DecoderRunner:
             self.num_blocks = max(want, 1)
         # one spare block past the pool: padded rows of the library backend scatter there
         shape = (self.num_blocks + 1, self.n_kv_local, KV_BLOCK, a.head_dim)
+        if self.kv8 is not None:
+            from ..ops import KV8Cache
+            self.kv8 = [KV8Cache.alloc(shape[0], shape[1], a.head_dim, self.cfg.kv_cache_dtype, self.device) for _ in range(a.n_layer)]
+            self.kcache, self.vcache = [c.k for c in self.kv8], [c.v for c in self.kv8]
+            return
         self.kcache = [torch.zeros(shape, dtype=self.dtype, device=self.device) for _ in range(a.n_layer)]
         self.vcache = [torch.zeros(shape, dtype=self.dtype, device=self.device) for _ in range(a.n_layer)]
 
@@ -311,7 +326,9 @@ class DecoderRunner:
             else:
                 h = h_next if h_next is not None else self._norm(x, L["ln1"])
                 qkv = self._linear(h, L["qkv"])
-            if decode and ops.name == "kernels":
+            if self.kv8 is not None:
+                att = self._attend_kv8(qkv, li, b, decode, slots, pos, ctx, bt_row, max_ctx, dense_plan)
+            elif decode and ops.name == "kernels":
                 att = ops.append_attention(qkv, hn, hn + kn, slots, self.kcache[li], self.vcache[li], b["block_tables"],
                                            ctx, self.n_head_local, self.n_kv_local, d, max_ctx, pos, a.rope_base)
             else:
@@ -376,6 +393,20 @@ class DecoderRunner:
         if local_argmax:
             return idx, mx
         return self.combine_argmax(idx, mx, comm)
+
+    def _attend_kv8(self, qkv, li, b, decode, slots, pos, ctx, bt_row, max_ctx, dense_plan):
+        """One layer's append and attention with the 8-bit cache: a decode step in one launch; whole prompts attend to the
+        fused qkv buffer as they do with a 16-bit cache, continuations and tails to the cache."""
+        a, ops, d, cache = self.arch, self.ops, self.arch.head_dim, self.kv8[li]
+        hn, kn = self.n_head_local * d, self.n_kv_local * d
+        if decode and ops.name == "kernels":
+            return ops.kv8_append_attention(qkv, hn, hn + kn, slots, cache, b["block_tables"], ctx, self.n_head_local, max_ctx, pos, a.rope_base)
+        ops.kv8_append(qkv, hn, hn + kn, slots, cache, self.n_head_local, pos, a.rope_base)
+        if dense_plan is not None and dense_plan.get("paged"):
+            return ops.kv8_prefill_attention(qkv, cache, b["block_tables"], dense_plan, self.n_head_local, self.cfg.max_model_len)
+        if dense_plan is not None:
+            return ops.dense_attention(qkv, 0, hn, hn + kn, dense_plan, self.n_head_local, self.n_kv_local, d, True)
+        return ops.kv8_attention(qkv, cache, b["block_tables"], ctx, self.n_head_local, max_ctx, bt_row)
 
     def gather_vocab(self, logits: torch.Tensor, comm=None) -> torch.Tensor:
         """Full-vocabulary fp32 logits on every rank from the vocabulary shards: [rows, world * shard] where column

@@ -18,6 +18,37 @@ from ..onnx.registry import rotary
 KV_BLOCK = 16
 
 
+def kv8_store(x, slots, codes, scale):
+    """Tokens x [T, kv_heads, d] into an 8-bit cache, as the append kernel defines it (``csrc/kernels/kv8.cuh``), over the whole
+    cache at once and without data-dependent shapes; rows without a slot go to the spare last block."""
+    nb, most = codes.shape[0], 127.0 if codes.dtype == torch.int8 else 448.0
+    def to_codes(v):
+        v = torch.nan_to_num(v)
+        return torch.round(v).clamp(-127, 127).to(torch.int8) if codes.dtype == torch.int8 else v.to(codes.dtype)
+    s = torch.where(slots >= 0, slots, torch.full_like(slots, (nb - 1) * KV_BLOCK)).long()
+    blk, off = s // KV_BLOCK, s % KV_BLOCK
+    xf = x.float()
+    begins = torch.full((nb,), KV_BLOCK, dtype=torch.long, device=x.device).scatter_reduce(0, blk, off, "amin")
+    size = xf.abs().amax(2)
+    finite = torch.isfinite(size)
+    at = blk[:, None].expand(-1, x.shape[1])
+    amax = torch.zeros_like(scale).scatter_reduce(0, at, torch.where(finite, size, torch.zeros_like(size)), "amax")
+    bad = torch.zeros_like(scale).scatter_reduce(0, at, (~finite).float(), "amax") > 0
+    frac, e = torch.frexp(amax)
+    top_frac, top_e = math.frexp(most)
+    e = torch.where(amax > 0, e - top_e + (frac > top_frac).to(e.dtype), torch.full_like(e, -100)).clamp(min=-100)
+    least = ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+    old = torch.where((begins == 0)[:, None], torch.zeros_like(scale), scale)
+    new = torch.where(bad, torch.full_like(scale, math.nan), torch.maximum(old, least))
+    touched = (begins < KV_BLOCK)[:, None]
+    again = to_codes(codes.float() * (old / new)[:, :, None, None])
+    older = (torch.arange(KV_BLOCK, device=x.device)[None, :] < begins[:, None])[:, None, :, None] & (begins < KV_BLOCK)[:, None, None, None]
+    raw = codes.view(torch.uint8)
+    raw.copy_(torch.where(older, again.view(torch.uint8), raw))
+    raw[blk, :, off, :] = to_codes(xf / new[blk][:, :, None]).view(torch.uint8)
+    scale.copy_(torch.where(touched, new, scale))
+
+
 class TorchOps:
     name = "torch"
 
@@ -94,6 +125,30 @@ class TorchOps:
         out = F.scaled_dot_product_attention(qh, k, v, attn_mask=keep[:, None, None, :])
         out = torch.where(empty[:, None, None, None], torch.zeros((), device=out.device, dtype=cdt), out)
         return out.reshape(rows, heads * d).to(q.dtype)
+
+    def kv8_append(self, qkv, k_off, v_off, slots, cache, heads, positions=None, rope_base=0.0):
+        T, d, kvh = qkv.shape[0], cache.head_dim, cache.kv_heads
+        if rope_base > 0 and positions is not None:
+            for off, n in ((0, heads), (k_off, kvh)):
+                qkv[:, off:off + n * d] = rotary(qkv[:, off:off + n * d], positions, rope_base, n)
+        for off, codes, scale in ((k_off, cache.k, cache.k_scale), (v_off, cache.v, cache.v_scale)):
+            kv8_store(qkv[:, off:off + kvh * d].reshape(T, kvh, d), slots, codes, scale)
+
+    def kv8_attention(self, q, cache, block_tables, ctx_len, heads, max_ctx, bt_row=None):
+        cdt = torch.float32 if q.device.type == "cpu" else q.dtype
+        k, v = ((c.float() * s[:, :, None, None]).to(cdt) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+        return self.paged_attention(q, k, v, block_tables, ctx_len, heads, cache.kv_heads, cache.head_dim, max_ctx, bt_row)
+
+    def token_logprobs(self, logits, tokens, top):
+        from ..ops import TokenLogprobs
+        lp = torch.log_softmax(logits.float(), -1)
+        t = tokens.long()[:, None]
+        own = logits.gather(1, t)
+        ahead = (logits > own) | ((logits == own) & (torch.arange(logits.shape[1], device=logits.device)[None, :] < t))
+        p = lp.exp()
+        ids = torch.sort(logits, dim=1, descending=True, stable=True).indices[:, :top]
+        return TokenLogprobs(lp.gather(1, t)[:, 0], ahead.sum(1).to(torch.int32) + 1, -torch.where(p > 0, p * lp, torch.zeros_like(p)).sum(1),
+                             ids.to(torch.int32), lp.gather(1, ids))
 
     def argmax(self, logits, col_offset=0, return_max=False):
         m, i = logits.float().max(dim=-1)
@@ -189,6 +244,25 @@ class KernelOps:
         """Causal attention of this step's query chunks over the paged cache, on the tensor cores."""
         return self.K.paged_prefill_attention(q, 0, kcache, vcache, block_tables, plan["seq_start"], plan["q_len"],
                                               plan["kv_len"], plan["max_q_len"], heads, kv_heads, d, causal=True)
+
+    def kv8_append(self, qkv, k_off, v_off, slots, cache, heads, positions=None, rope_base=0.0):
+        self.K.kv8_append(qkv, k_off, v_off, slots, cache, heads, positions if rope_base > 0 else None, rope_base)
+
+    def kv8_append_attention(self, qkv, k_off, v_off, slots, cache, block_tables, ctx_len, heads, max_ctx, positions=None, rope_base=0.0):
+        """Decode step with the 8-bit cache: (rotary embedding,) append and attention in one launch."""
+        return self.K.kv8_attention(qkv, cache, block_tables, ctx_len, heads, max_ctx, append=(k_off, v_off, slots),
+                                    rope=(positions, rope_base) if rope_base > 0 and positions is not None else None)
+
+    def kv8_attention(self, q, cache, block_tables, ctx_len, heads, max_ctx, bt_row=None):
+        return self.K.kv8_attention(q, cache, block_tables, ctx_len, heads, max_ctx, bt_row)
+
+    def kv8_prefill_attention(self, q, cache, block_tables, plan, heads, max_ctx):
+        """Causal attention of this step's query chunks over the 8-bit cache."""
+        return self.K.kv8_prefill_attention(q, 0, cache, block_tables, plan["seq_start"], plan["q_len"], plan["kv_len"], plan["max_q_len"],
+                                            plan.get("max_kv_len", max_ctx), heads, causal=True)
+
+    def token_logprobs(self, logits, tokens, top):
+        return self.K.token_logprobs(logits, tokens, top)
 
     def argmax(self, logits, col_offset=0, return_max=False):
         return self.K.argmax(logits, col_offset, return_max)

@@ -5,7 +5,7 @@ from __future__ import annotations
 import enum
 import time
 from dataclasses import dataclass, field
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 
 class RequestState(enum.IntEnum):
@@ -41,6 +41,17 @@ class SamplingParams:
     repeat_penalty: float = 1.0
     stop_sequences: List[List[int]] = field(default_factory=list)
     seed: Optional[int] = None
+    logprobs: Optional[int] = None     # log probabilities of the generated tokens, with this many alternatives (0 to 32)
+
+
+@dataclass(frozen=True)
+class TokenLogprob:
+    """How likely a generated token was under the model's own scores, before penalties and temperature."""
+    token: int
+    logprob: float
+    rank: int                          # 1: the most likely
+    entropy: float                     # of the whole distribution, nats
+    top: List[Tuple[int, float]]       # the most likely tokens, best first
 
 
 @dataclass
@@ -54,6 +65,7 @@ class Request:
     first_token_at: Optional[float] = None
     finished_at: Optional[float] = None
     error: Optional[str] = None
+    output_logprobs: Optional[List[TokenLogprob]] = None       # one of each generated token, where the request asks for them
     _final_tokens: Optional[List[int]] = None
     _sample_record: Optional[tuple] = None               # (sampling parameters, their packed record): see the engine
     _token_source: Optional[object] = None       # callable returning prompt + generated tokens while the request is live

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import asyncio
 import json
+import math
 import threading
 import time
 from typing import Dict, List, Optional
@@ -38,6 +39,7 @@ class CompletionRequest(BaseModel):
     repeat_penalty: float = 1.0
     seed: Optional[int] = None
     stop_token_sequences: List[List[int]] = []
+    logprobs: Optional[int] = None
     stream: bool = False
     priority: str = "normal"
 
@@ -56,6 +58,8 @@ class ChatRequest(BaseModel):
     repeat_penalty: float = 1.0
     seed: Optional[int] = None
     stop: List[str] = []
+    logprobs: bool = False
+    top_logprobs: int = 0
     stream: bool = False
     priority: str = "normal"
 
@@ -219,11 +223,22 @@ def create_app(engine: LLMEngine, tokenizer=None, admission=None):
             raise HTTPException(status_code=410, detail="request record is gone")
         if r.error:
             raise HTTPException(status_code=400 if r.finish_reason is None or not r.output_tokens else 500, detail=r.error)
-        return {"id": rid, "object": "text_completion",
-                "choices": [{"index": 0, "token_ids": r.output_tokens,
-                             "text": tokenizer.decode(r.output_tokens) if tokenizer is not None else None,
-                             "finish_reason": r.finish_reason.value if r.finish_reason else None}],
+        choice = {"index": 0, "token_ids": r.output_tokens,
+                  "text": tokenizer.decode(r.output_tokens) if tokenizer is not None else None,
+                  "finish_reason": r.finish_reason.value if r.finish_reason else None}
+        if r.output_logprobs is not None:
+            choice["logprobs"] = {"token_logprobs": [_number(p.logprob) for p in r.output_logprobs], "ranks": [p.rank for p in r.output_logprobs],
+                                  "entropy": [_number(p.entropy) for p in r.output_logprobs],
+                                  "top_logprobs": [[{"token_id": i, "logprob": _number(v)} for i, v in p.top] for p in r.output_logprobs]}
+        return {"id": rid, "object": "text_completion", "choices": [choice],
                 "usage": {"prompt_tokens": len(r.prompt_tokens), "completion_tokens": len(r.output_tokens)}}
+
+    def _number(v: float) -> Optional[float]:
+        return v if math.isfinite(v) else None                   # JSON has neither infinities nor NaN
+
+    def _logprob(p) -> dict:
+        return {"token_id": p.token, "logprob": _number(p.logprob), "rank": p.rank,
+                "top_logprobs": [{"token_id": i, "logprob": _number(v)} for i, v in p.top]}
 
     def _priority(name: str) -> Priority:
         try:
@@ -244,7 +259,8 @@ def create_app(engine: LLMEngine, tokenizer=None, admission=None):
         prompt = tokenizer.encode(render_chat([m.model_dump() for m in req.messages]))
         params = SamplingParams(max_new_tokens=req.max_tokens, temperature=req.temperature, top_k=req.top_k,
                                 top_p=req.top_p, repeat_penalty=req.repeat_penalty, seed=req.seed,
-                                stop_sequences=[tokenizer.encode(s_) for s_ in req.stop if s_])
+                                stop_sequences=[tokenizer.encode(s_) for s_ in req.stop if s_],
+                                logprobs=req.top_logprobs if req.logprobs else None)
         prio = _priority(req.priority)
         ticket = _admit(http)
         rid = loop.submit(prompt, params, prio)
@@ -254,10 +270,11 @@ def create_app(engine: LLMEngine, tokenizer=None, admission=None):
                 r = loop.result(rid)
                 if r is None or r.error:
                     raise HTTPException(status_code=400, detail=r.error if r is not None else "request record is gone")
+                more = {} if r.output_logprobs is None else {"logprobs": {"content": [_logprob(p) for p in r.output_logprobs]}}
                 return {"id": rid, "object": "chat.completion",
                         "choices": [{"index": 0, "message": {"role": "assistant", "content": tokenizer.decode(r.output_tokens)},
                                      "token_ids": r.output_tokens,
-                                     "finish_reason": r.finish_reason.value if r.finish_reason else None}],
+                                     "finish_reason": r.finish_reason.value if r.finish_reason else None, **more}],
                         "usage": {"prompt_tokens": len(r.prompt_tokens), "completion_tokens": len(r.output_tokens)}}
             finally:
                 loop.release(rid)
@@ -301,7 +318,7 @@ def create_app(engine: LLMEngine, tokenizer=None, admission=None):
             raise HTTPException(status_code=400, detail="prompt_token_ids must not be empty")
         params = SamplingParams(max_new_tokens=req.max_tokens, temperature=req.temperature, top_k=req.top_k,
                                 top_p=req.top_p, repeat_penalty=req.repeat_penalty, seed=req.seed,
-                                stop_sequences=req.stop_token_sequences)
+                                stop_sequences=req.stop_token_sequences, logprobs=req.logprobs)
         prio = _priority(req.priority)
         ticket = _admit(http)
         rid = loop.submit(list(req.prompt_token_ids), params, prio)
@@ -314,11 +331,17 @@ def create_app(engine: LLMEngine, tokenizer=None, admission=None):
                 adm.release(ticket)
 
         async def events():
+            sent = 0
             try:
                 while True:
                     done = await _wait(rid, 0.01)
                     for tok in loop.drain_stream(rid):
-                        yield f"data: {json.dumps({'id': rid, 'token_id': tok})}\n\n"
+                        event = {"id": rid, "token_id": tok}
+                        r = loop.result(rid)
+                        if r is not None and r.output_logprobs is not None and sent < len(r.output_logprobs):
+                            event["logprobs"] = _logprob(r.output_logprobs[sent])
+                        sent += 1
+                        yield f"data: {json.dumps(event)}\n\n"
                     if done or adm.expired(ticket):
                         r = loop.result(rid)
                         reason = r.finish_reason.value if r is not None and r.finish_reason else ("deadline" if not done else None)
