@@ -137,48 +137,54 @@ __device__ __forceinline__ uint32_t kv8_warp_amax(uint32_t m) {
   return __float_as_uint(lo);
 }
 
+// Scale of a block after tokens whose largest magnitude has the bits `m` (not finite: 0x7f800000 or more) have joined one of
+// scale `old`: the larger of the two; NaN stays.
+template <int CODE>
+__device__ __forceinline__ float kv8_new_scale(uint32_t m, float old) {
+  const float nan = __uint_as_float(0x7fc00000u);
+  if (m >= 0x7f800000u) return nan;
+  const float s = kv8_least_scale<CODE>(m);
+  return old <= s ? s : old;
+}
+// The first `words` words of codes to a coarser step, by `lanes` lanes.
+template <int CODE>
+__device__ __forceinline__ void kv8_round_again(uint8_t* codes, int words, int lane, int lanes, float old, float inv) {
+  const float again = inv == 0.f ? 0.f : old * inv;           // a power of two below 1, or 0
+  uint32_t* c32 = reinterpret_cast<uint32_t*>(codes);
+  for (int i = lane; i < words; i += lanes) {
+    float f[4];
+    kv8_unpack4<CODE>(c32[i], f);
+    c32[i] = kv8_pack4<CODE>(f[0] * again, f[1] * again, f[2] * again, f[3] * again);
+  }
+}
+template <class T, int CODE>
+__device__ __forceinline__ uint2 kv8_pack8(const Vec8& x, float inv) {
+  float f[8];
+  unpack8<T>(x, f);
+  if (inv == 0.f) return make_uint2(0u, 0u);                  // also for what is not finite
+  return make_uint2(kv8_pack4<CODE>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                    kv8_pack4<CODE>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+}
+
 // One warp puts n tokens of one (block, head) into slots off .. off + n - 1: the block's new scale, older codes rounded again
-// where it grew, the tokens' codes; returns the scale.  x[p] holds 8 channels (from chunk * 8 on) of token p * (tokens a pass) + sub; a lane with
-// chunk < 0 holds a copy and writes nothing.  Tokens from n on are zeros.
+// where it grew, the tokens' codes.  x[p] holds 8 channels (from chunk * 8 on) of token p * (tokens a pass) + sub.  Tokens from
+// n on are zeros.
 template <class T, int D, int CODE, int PASSES>
-__device__ __forceinline__ float kv8_store_run(const Vec8* x, int chunk, int sub, int n, int off, float* scale, uint8_t* codes) {
+__device__ __forceinline__ void kv8_store_run(const Vec8* x, int chunk, int sub, int n, int off, float* scale, uint8_t* codes) {
   constexpr int TPW = 256 / D;
   const int lane = threadIdx.x & 31;
-  const float nan = __uint_as_float(0x7fc00000u);
   const float old = off > 0 ? *scale : 0.f;
   uint32_t m = 0;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) m = kv8_absmax(m, x[p]);
-  m = kv8_warp_amax<T>(m);
-  float s = m >= 0x7f800000u ? nan : kv8_least_scale<CODE>(m);
-  if (!(old <= s)) s = old;                                   // the larger of the two; NaN stays
-  if (m >= 0x7f800000u) s = nan;
-  const float inv = kv8_inverse(s);
-  __syncwarp();                                               // all lanes have read the old scale
-  if (off > 0 && s != old) {
-    const float again = inv == 0.f ? 0.f : old * inv;         // a power of two below 1, or 0
-    uint32_t* c32 = reinterpret_cast<uint32_t*>(codes);
-    for (int i = lane; i < off * (D / 4); i += 32) {
-      float f[4];
-      kv8_unpack4<CODE>(c32[i], f);
-      c32[i] = kv8_pack4<CODE>(f[0] * again, f[1] * again, f[2] * again, f[3] * again);
-    }
-  }
+  const float s = kv8_new_scale<CODE>(kv8_warp_amax<T>(m), old), inv = kv8_inverse(s);       // all lanes have read the old scale
+  if (off > 0 && s != old) kv8_round_again<CODE>(codes, off * (D / 4), lane, 32, old, inv);
   if (lane == 0 && (off == 0 || s != old)) *scale = s;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     const int t = p * TPW + sub;
-    if (t >= n || chunk < 0) continue;
-    float f[8];
-    unpack8<T>(x[p], f);
-    uint2 c = make_uint2(0u, 0u);
-    if (inv != 0.f) {
-      c.x = kv8_pack4<CODE>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-      c.y = kv8_pack4<CODE>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
-    }
-    *reinterpret_cast<uint2*>(codes + (off + t) * D + chunk * 8) = c;
+    if (t < n) *reinterpret_cast<uint2*>(codes + (off + t) * D + chunk * 8) = kv8_pack8<T, CODE>(x[p], inv);
   }
-  return s;
 }
 
 // One call.  q, out: 16-bit [rows, ld]; dtype 0 bf16, 1 fp16; code 0 int8, 1 e4m3; head_dim 64 or 128.  max_q_len bounds

@@ -6,13 +6,16 @@
 //                        With append slots (one query per sequence) the row's new K and V join the cache first.
 //
 // Bound by memory: every code is read once for all the queries that share it.  A warp takes cache blocks of 16 tokens one
-// after the other, straight from global memory into the fragments of mma.sync m16n8k16, without shared memory between:
+// after the other, by asynchronous 16-byte copies into a ring of its own in shared memory and from there into the fragments
+// of mma.sync m16n8k16:
 //   S = Q K^T     A = up to 16 query rows (heads of the group, queries of a chunk), B = 8 tokens; the head dimension is the
-//                 sum's index, so its order is free: lane (g, c) of the fragment takes 16 consecutive bytes of token g, and
+//                 sum's index, so its order is free: lane (g, c) of the fragment takes 16 consecutive bytes of one token, and
 //                 Q is laid out to match.
-//   O^T = V^T P^T A = 16 channels, B = 8 query rows.  The accumulator of S, (row g, tokens 2c and 2c + 1), is the B fragment
-//                 of P^T as it stands; V's channels are in free order too: lane (g, c) takes 8 or 16 consecutive bytes of
-//                 tokens 2c, 2c + 1, 2c + 8, 2c + 9 and interleaves the bytes of two tokens.
+//   O^T = V^T P^T A = 16 channels, B = 8 query rows.  The accumulator of S, (row g, two tokens of c), is the B fragment of P^T
+//                 as it stands; V's channels are in free order too: lane (g, c) takes 8 or 16 consecutive bytes of c's four
+//                 tokens and interleaves the bytes of two.
+// The 16-byte pieces of a row stand in the ring in an order that depends on the row (Kv8Ring), so that neither read meets a
+// bank twice.  Blocks held in registers instead cost 48 of them and with them a third of the warps an SM can hold.
 // Codes become f16 exactly.  Q in bf16 is scaled by a power of two for each row, so that it fits f16 (its 8 significant bits
 // do; what is 2^-34 of the row's largest is lost).  Softmax statistics, sums and O are in 32 bits; P is rounded to f16 as
 // 2^15 p, 2^-12 of it and never more than 2^-40.  The scale of a K block multiplies its scores, that of a V block its P,
@@ -42,7 +45,7 @@ struct Kv8AttnArgs {
   float* part;                // splits > 1: [item][split][rows][D + 2] partial results
   uint32_t* status;
   long ld_q, ld_o, num_blocks, rows, table_ld;
-  int items_x, table_rows, max_blocks, heads, kv_heads, causal, splits, share, part_rows, max_q, k_off, v_off;
+  int group, items_x, table_rows, max_blocks, heads, kv_heads, causal, splits, share, part_rows, max_q, k_off, v_off;
   float scale_log2;
 };
 
@@ -79,22 +82,61 @@ __device__ __forceinline__ void kv8_halves(uint32_t w, uint32_t& lo, uint32_t& h
   }
 }
 
-// The new K (IS_V: V) of one row into its slot, by one warp: kv8_append for a run of one token.  Returns the block's scale.
-template <class T, int D, int CODE, bool IS_V>
-__device__ __forceinline__ float kv8_append_one(const Kv8AttnArgs& a, long row, int slot, int kvh, const float4* cs) {
+// Places in a block of codes in shared memory: row t's 16-byte pieces are permuted by an exclusive or with `turn(t)`.  A token
+// of fragment column n is `token(n)`: for rows of 64 bytes, two rows to a line of banks, c's tokens are 2c and 2c + 1 in an order
+// that gives the four c of one load rows of both parities.
+template <int D> struct Kv8Ring {
+  static constexpr int PIECES = D / 16;                                  // of a row
+  static __device__ __forceinline__ int turn(int t) { return D == 64 ? ((t >> 2) & 1) * 2 : (((t >> 1) & 3) * 2) ^ ((t & 1) * 4); }
+  static __device__ __forceinline__ int token(int n) { return D == 64 ? n ^ ((n >> 1) & 1) : n; }
+  static __device__ __forceinline__ int at(int t, int piece) { return t * D + ((piece ^ turn(t)) << 4); }
+};
+__device__ __forceinline__ uint4 kv8_shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 kv8_shared8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void kv8_copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
+// The new K and V of one row into its slot, by one warp: kv8_append for a run of one token, K in lanes 0 to 15 and V in the
+// others.  `ks` and `vs` become the block's scales.
+template <class T, int D, int CODE>
+__device__ __forceinline__ void kv8_append_one(const Kv8AttnArgs& a, long row, int slot, int kvh, const float4* cs, float& ks, float& vs) {
   constexpr int CH = D / 8;
   const int lane = threadIdx.x & 31, chunk = lane % CH;
-  const T* src = static_cast<const T*>(a.q) + row * a.ld_q + (IS_V ? a.v_off : a.k_off) + long(kvh) * D;
-  Vec8 x = *reinterpret_cast<const Vec8*>(src + chunk * 8);       // every CH lanes the same token
-  if (!IS_V && a.positions) {
+  const bool is_v = lane >= 16;
+  const T* src = static_cast<const T*>(a.q) + row * a.ld_q + (is_v ? a.v_off : a.k_off) + long(kvh) * D;
+  Vec8 x = *reinterpret_cast<const Vec8*>(src + chunk * 8);
+  const long unit = long(slot / KV8_BLOCK) * a.kv_heads + kvh;
+  const int off = slot % KV8_BLOCK;
+  float* scale = (is_v ? a.vscale : a.kscale) + unit;
+  const float old = off > 0 ? *scale : 0.f;
+  if (a.positions) {
     Vec8 oth;
 #pragma unroll
     for (int i = 0; i < 4; ++i) oth.w[i] = __shfl_xor_sync(0xffffffffu, x.w[i], CH / 2);
-    x = kv8_rotate8<T, CH / 2>(x, oth, chunk < CH / 2, cs + chunk % (CH / 2));
+    const Vec8 turned = kv8_rotate8<T, CH / 2>(x, oth, chunk < CH / 2, cs + chunk % (CH / 2));
+    if (!is_v) x = turned;
   }
-  const long unit = long(slot / KV8_BLOCK) * a.kv_heads + kvh;
-  return kv8_store_run<T, D, CODE, 1>(&x, lane < CH ? chunk : -1, 0, 1, slot % KV8_BLOCK, (IS_V ? a.vscale : a.kscale) + unit,
-                                      (IS_V ? a.vcodes : a.kcodes) + unit * (KV8_BLOCK * D));
+  uint32_t m = kv8_absmax(0u, x);
+#pragma unroll
+  for (int o = 8; o; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));       // over each half of the warp
+  m = max(m & 0xffffu, m >> 16);
+  float lo, hi;
+  Pair16<T>::unpack(m, lo, hi);
+  const float s = kv8_new_scale<CODE>(__float_as_uint(lo), old), inv = kv8_inverse(s);
+  uint8_t* codes = (is_v ? a.vcodes : a.kcodes) + unit * (KV8_BLOCK * D);
+  if (off > 0 && s != old) kv8_round_again<CODE>(codes, off * (D / 4), lane & 15, 16, old, inv);
+  if ((lane & 15) == 0 && (off == 0 || s != old)) *scale = s;
+  if ((lane & 15) < CH) *reinterpret_cast<uint2*>(codes + off * D + chunk * 8) = kv8_pack8<T, CODE>(x, inv);
+  ks = __shfl_sync(0xffffffffu, s, 0), vs = __shfl_sync(0xffffffffu, s, 16);
 }
 
 // Barrier of the warps that share an item.
@@ -106,10 +148,10 @@ __device__ __forceinline__ void kv8_item_sync(int item) {
 }
 
 // An item is a tile of up to 16 query rows of one (sequence, KV head), and one of `splits` shares of its blocks; WPI of the
-// CTA's warps work on it.  NT = 1: at most 8 rows.  ST: blocks a warp has in registers, one at work and the others on their
-// way.  A warp's first loads start before q is fetched: the chain length -> page -> codes is the longer one.
+// CTA's warps work on it.  NT = 1: at most 8 rows.  ST: blocks in a warp's ring, one at work and the others on their way.
+// A warp's first loads start before q is fetched: the chain length -> page -> codes is the longer one.
 template <class T, int D, int CODE, int NT, int WPI, int ST>
-__global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64 ? 4 : 3) kv8_attention_kernel(Kv8AttnArgs a, Kv8Turns turns) {
+__global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT == 1 ? 4 : 3)) kv8_attention_kernel(Kv8AttnArgs a, Kv8Turns turns) {
   constexpr int KW = D / 64;                  // 16-byte loads of K a lane and 8 tokens
   constexpr int VB = D / 8;                   // bytes of V a lane and token
   constexpr int VW = VB / 4;
@@ -121,7 +163,8 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
   __shared__ float s_qs_all[IPC][R];
   __shared__ float4 s_cs_all[IPC][D / 2];
   __shared__ float s_m_all[KV8_NW][R], s_l_all[KV8_NW][R];
-  extern __shared__ float s_o_all[];          // [KV8_NW][R][D]
+  constexpr int STAGE = 2 * KV8_BLOCK * D;    // bytes of a block: keys, values
+  extern __shared__ __align__(128) uint8_t s_ring_all[];           // [KV8_NW][ST][STAGE], later [KV8_NW][R][D] floats
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
@@ -133,9 +176,12 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
   auto& s_cs = s_cs_all[in_cta];
   auto* s_m = s_m_all + in_cta * WPI;
   auto* s_l = s_l_all + in_cta * WPI;
-  float* s_o = s_o_all + in_cta * WPI * R * D;
-  const int seq = x_item / a.kv_heads, kvh = x_item - seq * a.kv_heads;
-  const int group = a.heads / a.kv_heads;
+  const uint32_t ring_at = uint32_t(__cvta_generic_to_shared(s_ring_all)) + warp * (ST * STAGE);
+  // this lane's results start its warp's part of the ring
+  static_assert(R * D * 4 <= ST * STAGE, "a warp's results fit its ring");
+  auto s_o = [&](int w, int r) { return reinterpret_cast<float*>(s_ring_all + (in_cta * WPI + w) * (ST * STAGE)) + r * D; };
+  const int seq = a.kv_heads == 1 ? x_item : x_item / a.kv_heads, kvh = x_item - seq * a.kv_heads;
+  const int group = a.group;
   const int n = a.q_len ? a.q_len[seq] : 1;
   const int r0 = blockIdx.y * 16;
   const int live = min(min(16, a.part_rows), n * group - r0);   // rows of this tile
@@ -155,7 +201,8 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
     len = 0;
   }
   // keys that the tile's last query sees, this share's blocks, this warp's
-  const int seen = a.causal ? len - (n - 1 - (r0 + live - 1) / group) : len;
+  auto query_of = [&](int r) { return n == 1 ? 0 : r / group; };          // of row r: a decode step has one
+  const int seen = a.causal ? len - (n - 1 - query_of(r0 + live - 1)) : len;
   const int nblk = seen > 0 ? (seen + KV8_BLOCK - 1) / KV8_BLOCK : 0;
   const int b_lo = min(nblk, int(blockIdx.z) * a.share), b_hi = blockIdx.z + 1 == a.splits ? nblk : min(nblk, b_lo + a.share);
   const int w_lo = b_lo + int(long(b_hi - b_lo) * iw / WPI), w_hi = b_lo + int(long(b_hi - b_lo) * (iw + 1) / WPI);
@@ -163,28 +210,21 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
   const int* bt = a.tables + long(table) * a.table_ld + w_lo;
   const bool appends = slot >= 0 && cnt > 0 && w_hi == nblk;    // the warp that reads the last block writes the new token
 
-  uint4 kb[ST][2 * KW];
-  uint32_t vb[ST][4][VW];
+  using Ring = Kv8Ring<D>;
+  // this lane's pieces of a block: piece lane + 32 i, for keys and for values
   auto load = [&](int into, int p) {
-    const long base = (long(max(p, 0)) * a.kv_heads + kvh) * (KV8_BLOCK * D);
-    const uint8_t* kp = a.kcodes + base + g * D + c * 16;
-    const uint8_t* vp = a.vcodes + base + 2 * c * D + g * VB;
+    const long base = (long(max(p, 0)) * a.kv_heads + kvh) * (KV8_BLOCK * D) + lane * 16;
+    const uint8_t* kp = a.kcodes + base;
+    const uint8_t* vp = a.vcodes + base;
 #pragma unroll
-    for (int i = 0; i < KW; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) kb[into][2 * i + h] = *reinterpret_cast<const uint4*>(kp + 8 * h * D + i * 64);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint8_t* src = vp + ((k & 1) + 8 * (k >> 1)) * D;
-      if constexpr (VW == 2) {
-        const uint2 w = *reinterpret_cast<const uint2*>(src);
-        vb[into][k][0] = w.x, vb[into][k][1] = w.y;
-      } else {
-        const uint4 w = *reinterpret_cast<const uint4*>(src);
-        vb[into][k][0] = w.x, vb[into][k][1] = w.y, vb[into][k][2] = w.z, vb[into][k][3] = w.w;
-      }
+    for (int i = 0; i < D / 32; ++i) {
+      const int piece = lane + 32 * i;
+      const uint32_t to = ring_at + into * STAGE + Ring::at(piece / Ring::PIECES, piece % Ring::PIECES);
+      kv8_copy16(to, kp + i * 512);
+      kv8_copy16(to + KV8_BLOCK * D, vp + i * 512);
     }
   };
+  auto commit = [&] { asm volatile("cp.async.commit_group;" ::: "memory"); };
   // pages and scales are looked up for 32 blocks at a time, one a lane: pages two such groups ahead, scales one
   auto page_of = [&](int b) {
     int p = b < cnt ? bt[b] : -1;
@@ -196,8 +236,10 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
   float kf = scale_of(a.kscale, page), vf = scale_of(a.vscale, page), kf1 = 0.f, vf1 = 0.f;
   const int early = appends ? min(cnt - 1, ST - 1) : min(cnt, ST - 1);        // the last block waits for its new token
 #pragma unroll
-  for (int s = 0; s < ST - 1; ++s)
+  for (int s = 0; s < ST - 1; ++s) {                                          // one group a block, empty ones among them
     if (s < early) load(s, __shfl_sync(0xffffffffu, page, s));
+    if (!appends || s < early) commit();
+  }
 
   // ---- q to shared memory: rotated, scaled to f16
   if (a.positions) {
@@ -209,7 +251,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
     uint4 h = make_uint4(0u, 0u, 0u, 0u);
     float down = 0.f;
     if (r < live) {
-      const int t = (r0 + r) / group, head = kvh * group + (r0 + r) % group;
+      const int t = query_of(r0 + r), head = kvh * group + r0 + r - t * group;
       Vec8 x = *reinterpret_cast<const Vec8*>(static_cast<const T*>(a.q) + (row0 + t) * a.ld_q + long(head) * D + chunk * 8);
       if (a.positions) {
         Vec8 oth;
@@ -239,15 +281,14 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
     if (slot >= a.num_blocks * KV8_BLOCK) {
       if (lane == 0) kv8_report(a.status);
     } else {
-      const float ks = kv8_append_one<T, D, CODE, false>(a, row0, slot, kvh, s_cs);
-      const float vs = kv8_append_one<T, D, CODE, true>(a, row0, slot, kvh, s_cs);
+      float ks, vs;
+      kv8_append_one<T, D, CODE>(a, row0, slot, kvh, s_cs, ks, vs);
       __syncwarp();
       if (lane == cnt - 1 && page == slot / KV8_BLOCK) kf = ks, vf = vs;
     }
-    if (early < ST - 1) {
-#pragma unroll
-      for (int s = 0; s < ST - 1; ++s)
-        if (s == early) load(s, __shfl_sync(0xffffffffu, page, s));
+    for (int s = early; s < ST - 1; ++s) {
+      if (s == early) load(s, __shfl_sync(0xffffffffu, page, s));
+      commit();
     }
   }
   if (vf != vf) kf = vf, vf = 0.f;              // seeing the block's keys is seeing its values: NaN through the scores
@@ -269,9 +310,9 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     qs[t] = s_qs[g + 8 * t];
-    lim[t] = g + 8 * t < live ? (a.causal ? len - (n - 1 - (r0 + g + 8 * t) / group) : len) : 0;
+    lim[t] = g + 8 * t < live ? (a.causal ? len - (n - 1 - query_of(r0 + g + 8 * t)) : len) : 0;
   }
-  const int first_lim = a.causal ? len - (n - 1 - r0 / group) : len;        // the fewest keys of a live row
+  const int first_lim = a.causal ? len - (n - 1 - query_of(r0)) : len;        // the fewest keys of a live row
 
   float o[MT][NT][4], m[NT], l[NT];
 #pragma unroll
@@ -283,14 +324,23 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
       for (int k = 0; k < 4; ++k) o[i][t][k] = 0.f;
   }
   float vref = 0.f;                            // o is in units of vref * 2^-15
-  for (int bs = 0; bs < cnt; bs += ST) {
+  uint32_t gone_of = __ballot_sync(0xffffffffu, page < 0);        // of the 32 blocks at hand
+  // where this lane reads: keys of tokens token(g) and 8 further, values of c's tokens
+  uint32_t k_at[KW], v_at[2];
 #pragma unroll
-    for (int s = 0; s < ST; ++s) {
-      const int b = bs + s;
-      if (b >= cnt) break;
+  for (int i = 0; i < KW; ++i) k_at[i] = ring_at + Ring::at(Ring::token(g), i * 4 + c);
+  int tok_of[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    tok_of[k] = Ring::token(2 * c + k);
+    v_at[k] = ring_at + KV8_BLOCK * D + Ring::at(tok_of[k], g * VB / 16) + (g * VB) % 16;
+  }
+  for (int b = 0, into = ST - 1, from = 0; b < cnt; ++b) {
+    {
       if ((b & 31) == 0) {
         if (b > 0) {
           page = page1, page1 = page2, kf = kf1, vf = vf1;
+          gone_of = __ballot_sync(0xffffffffu, page < 0);
           if (vf != vf) kf = vf, vf = 0.f;
         }
         kf1 = scale_of(a.kscale, page1), vf1 = scale_of(a.vscale, page1);
@@ -308,16 +358,22 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
         }
         vf *= kv8_inverse(vref) * 32768.f;
       }
+      asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+      __syncwarp();                           // block b has landed, and every lane is done with block b - 1
       const int nb = b + ST - 1;
-      if (nb < cnt) load((s + ST - 1) % ST, __shfl_sync(0xffffffffu, ((nb ^ b) & 32) ? page1 : page, nb & 31));
+      if (nb < cnt) load(into, __shfl_sync(0xffffffffu, ((nb ^ b) & 32) ? page1 : page, nb & 31));
+      commit();
+      const int place = from * STAGE;
+      into = from, from = from + 1 == ST ? 0 : from + 1;
       // ---- scores
       float sc[2][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
+        uint4 w4;
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-          const uint4& w4 = kb[s][2 * (j / 4) + h];
+          if (j % 4 == 0) w4 = kv8_shared16(k_at[j / 4] + place + 8 * h * D);
           const uint32_t w = (j % 4) == 0 ? w4.x : (j % 4) == 1 ? w4.y : (j % 4) == 2 ? w4.z : w4.w;
           uint32_t b0, b1;
           kv8_halves<CODE>(w, b0, b1);
@@ -325,10 +381,22 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
         }
       }
       const float kfac = __shfl_sync(0xffffffffu, kf, b & 31), vfac = __shfl_sync(0xffffffffu, vf, b & 31);
-      const bool gone = __shfl_sync(0xffffffffu, page, b & 31) < 0;
+      const bool gone = (gone_of >> (b & 31)) & 1;
       const int t0 = (w_lo + b) * KV8_BLOCK;
       const bool edge = gone || t0 + KV8_BLOCK > first_lim;
-      float x[NT][4];                         // (row g + 8 t; tokens 2c, 2c + 1, 2c + 8, 2c + 9)
+      uint32_t vb[4][VW];                     // c's tokens tok_of[0], tok_of[1], and 8 further
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t src = v_at[k & 1] + place + 8 * (k >> 1) * D;
+        if constexpr (VW == 2) {
+          const uint2 w = kv8_shared8(src);
+          vb[k][0] = w.x, vb[k][1] = w.y;
+        } else {
+          const uint4 w = kv8_shared16(src);
+          vb[k][0] = w.x, vb[k][1] = w.y, vb[k][2] = w.z, vb[k][3] = w.w;
+        }
+      }
+      float x[NT][4];                         // (row g + 8 t; the same tokens)
       bool rise = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -338,13 +406,13 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
       if (edge) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int tok = t0 + 2 * c + (k & 1) + 8 * (k >> 1);
+          const int tok = t0 + tok_of[k & 1] + 8 * (k >> 1);
 #pragma unroll
           for (int t = 0; t < NT; ++t)
             if (gone || tok >= lim[t]) x[t][k] = -INFINITY;
           if (gone || tok >= len) {           // bytes behind the context are no codes
 #pragma unroll
-            for (int i = 0; i < VW; ++i) vb[s][k][i] = 0u;
+            for (int i = 0; i < VW; ++i) vb[k][i] = 0u;
           }
         }
       }
@@ -387,8 +455,8 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
         const int w = i / 2;
         const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
         uint32_t a0, a1, a2, a3;
-        kv8_halves<CODE>(__byte_perm(vb[s][0][w], vb[s][1][w], sel), a0, a1);
-        kv8_halves<CODE>(__byte_perm(vb[s][2][w], vb[s][3][w], sel), a2, a3);
+        kv8_halves<CODE>(__byte_perm(vb[0][w], vb[1][w], sel), a0, a1);
+        kv8_halves<CODE>(__byte_perm(vb[2][w], vb[3][w], sel), a2, a3);
 #pragma unroll
         for (int t = 0; t < NT; ++t) kv8_mma(o[i][t], a0, a1, a2, a3, p[t][0], p[t][1]);
       }
@@ -403,6 +471,8 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
     if (c == 0) s_m[iw][g + 8 * t] = m[t], s_l[iw][g + 8 * t] = l[t];
   }
   const float unit = vref * (1.f / 32768.f);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();                               // the ring is done with
   // o[i][t][k]: channel g * VB + 2 i + (k >> 1), row 2c + (k & 1) + 8 t
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -410,7 +480,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
     for (int k = 0; k < 2; ++k) {
       const int r = 2 * c + k + 8 * t;
       if (r < live) {
-        float* dst = s_o + (iw * R + r) * D + g * VB;
+        float* dst = s_o(iw, r) + g * VB;
 #pragma unroll
         for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[i][t][k] * unit, o[i][t][k + 2] * unit);
       }
@@ -426,7 +496,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
 #pragma unroll
     for (int w = 0; w < WPI; ++w) {
       const float f = kv8_weight(s_m[w][r], s_l[w][r], mx);
-      const float2 v = *reinterpret_cast<const float2*>(s_o + (w * R + r) * D + ch);
+      const float2 v = *reinterpret_cast<const float2*>(s_o(w, r) + ch);
       if (f != 0.f) s0 += f * v.x, s1 += f * v.y, sum += f * s_l[w][r];
     }
     if (a.splits > 1) {
@@ -434,7 +504,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, NT == 2 && D == 128 ? 2 : D == 64
       *reinterpret_cast<float2*>(dst + ch) = make_float2(s0, s1);
       if (ch == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mx, sum);
     } else {
-      const int t = (r0 + r) / group, h = kvh * group + (r0 + r) % group;
+      const int t = query_of(r0 + r), h = kvh * group + r0 + r - t * group;
       const float inv = sum != 0.f ? 1.f / sum : 0.f;
       T* dst = static_cast<T*>(a.out) + (row0 + t) * a.ld_o + long(h) * D + ch;
       *reinterpret_cast<uint32_t*>(dst) = Pair16<T>::pack(s0 * inv, s1 * inv);
@@ -460,19 +530,33 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8AttnArgs a, long ti
   if (row0 < 0 || row0 + n > a.rows) return;
   const float* src = a.part + (tile * a.splits * a.part_rows + r) * (D + 2);
   const long step = long(a.part_rows) * (D + 2);
-  float mx = -INFINITY;
-  for (int z = 0; z < a.splits; ++z) mx = fmaxf(mx, src[z * step + D]);
   constexpr int PER = D / 32;
-  float acc[PER], sum = 0.f;
+  float acc[PER], sum = 0.f, mx = -INFINITY;
 #pragma unroll
   for (int k = 0; k < PER; ++k) acc[k] = 0.f;
-  for (int z = 0; z < a.splits; ++z) {
-    const float l = src[z * step + D + 1], mz = src[z * step + D];
-    const float f = kv8_weight(mz, l, mx);
-    if (f != 0.f) {
-      sum += f * l;
+  for (int z0 = 0; z0 < a.splits; z0 += 32) {             // a share's maximum and sum to a lane, 32 shares at a time
+    const int z = z0 + lane;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (z < a.splits) ml = *reinterpret_cast<const float2*>(src + z * step + D);
+    const float top = fmaxf(mx, warp_max(ml.x)), down = sum == 0.f ? 0.f : kv8_weight(mx, sum, top);
+    const float w = kv8_weight(ml.x, ml.y, top);
+    sum = (down != 0.f ? sum * down : 0.f) + warp_sum(w != 0.f ? w * ml.y : 0.f);
 #pragma unroll
-      for (int k = 0; k < PER; ++k) acc[k] += f * src[z * step + lane * PER + k];
+    for (int k = 0; k < PER; ++k) acc[k] = down != 0.f ? acc[k] * down : 0.f;
+    mx = top;
+    const int n_here = min(32, a.splits - z0);
+#pragma unroll 8
+    for (int i = 0; i < n_here; ++i) {
+      const float f = __shfl_sync(0xffffffffu, w, i);
+      const float* v = src + (z0 + i) * step + lane * PER;
+      float part[PER];
+#pragma unroll
+      for (int k = 0; k < PER; k += 2) {
+        const float2 t = *reinterpret_cast<const float2*>(v + k);
+        part[k] = t.x, part[k + 1] = t.y;
+      }
+#pragma unroll
+      for (int k = 0; k < PER; ++k) acc[k] += f != 0.f ? f * part[k] : 0.f;
     }
   }
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
@@ -534,7 +618,7 @@ extern "C" int ronn_kv8_attention(const Kv8AttnCall* call, cudaStream_t stream) 
   if (positions)
     for (int j = 0; j < head_dim / 2; ++j) tn.t[j] = turns[j];
   Kv8AttnArgs a{q, out, (uint8_t*)kcodes, (uint8_t*)vcodes, kscale, vscale, tables, kv_len, bt_row, seq_start, q_len, slots, positions,
-                (float*)scratch, status, ld_q, ld_o, num_blocks, rows, table_ld, int(xs), table_rows, max_blocks, heads, kv_heads, causal,
+                (float*)scratch, status, ld_q, ld_o, num_blocks, rows, table_ld, heads / kv_heads, int(xs), table_rows, max_blocks, heads, kv_heads, causal,
                 plan.splits, plan.share, part_rows, max_q_len, k_off, v_off, scale * 1.4426950408889634f};
   const long per_cta = KV8_NW / wpi;
   const dim3 grid{unsigned((xs + per_cta - 1) / per_cta), unsigned(mtiles), unsigned(splits)};
@@ -547,11 +631,12 @@ extern "C" int ronn_kv8_attention(const Kv8AttnCall* call, cudaStream_t stream) 
   } while (0)
 #define RONN_KV8W(T, D, C, NT, W) \
   do { \
-    constexpr int smem = KV8_NW * 8 * NT * D * 4; \
-    auto* kern = kv8_attention_kernel<T, D, C, NT, W, (D == 64 ? 3 : 2)>; \
+    constexpr int st = D == 64 ? 4 : 3, smem = KV8_NW * st * 32 * D; \
+    auto* kern = kv8_attention_kernel<T, D, C, NT, W, st>; \
     static bool seen[MAX_DEVICES] = {false}; \
     if (first_use_on_device(seen) && \
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3; \
+        (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess || \
+         cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)) return -3; \
     launch(kern, grid, dim3(KV8_NW * 32), smem, stream, a, tn); \
   } while (0)
 #define RONN_KV8T_(T, D) \
