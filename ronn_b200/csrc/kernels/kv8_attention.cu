@@ -8,12 +8,13 @@
 // Bound by memory: every code is read once for all the queries that share it.  A warp takes cache blocks of 16 tokens one
 // after the other, by asynchronous 16-byte copies into a ring of its own in shared memory and from there into the fragments
 // of mma.sync m16n8k16:
-//   S = Q K^T     A = up to 16 query rows (heads of the group, queries of a chunk), B = 8 tokens; the head dimension is the
-//                 sum's index, so its order is free: lane (g, c) of the fragment takes 16 consecutive bytes of one token, and
-//                 Q is laid out to match.
-//   O^T = V^T P^T A = 16 channels, B = 8 query rows.  The accumulator of S, (row g, two tokens of c), is the B fragment of P^T
-//                 as it stands; V's channels are in free order too: lane (g, c) takes 8 or 16 consecutive bytes of c's four
-//                 tokens and interleaves the bytes of two.
+//   S^T = K Q^T   A = 16 tokens, B = 8 query rows (heads of the group, queries of a chunk); the head dimension is the sum's
+//                 index, so its order is free: lane (g, c) of the fragment takes 16 consecutive bytes of a token, and Q is laid
+//                 out to match.
+//   O^T = V^T P^T A = 16 channels, B = P^T: the accumulator of S^T, (token g, two rows), turned around by movmatrix.  V's
+//                 channels are in free order too: lane (g, c) takes 8 or 16 consecutive bytes of c's four tokens and
+//                 interleaves the bytes of two.
+// Queries as B waste nothing on a decode step's missing rows: 8 products a block of 64 channels, not 12.
 // The 16-byte pieces of a row stand in the ring in an order that depends on the row (Kv8Ring), so that neither read meets a
 // bank twice.  Blocks held in registers instead cost 48 of them and with them a third of the warps an SM can hold.
 // Codes become f16 exactly.  Q in bf16 is scaled by a power of two for each row, so that it fits f16 (its 8 significant bits
@@ -67,6 +68,12 @@ __device__ __forceinline__ uint32_t kv8_half2(float lo, float hi) {
 
 // Weight of a partial result with maximum m and sum l beside others whose maximum is mx: none without keys, NaN for NaN.
 __device__ __forceinline__ float kv8_weight(float m, float l, float mx) { return l == 0.f ? 0.f : l != l ? l : kv8_exp2(m - mx); }
+
+__device__ __forceinline__ uint32_t kv8_turn(uint32_t a) {      // an 8 x 8 matrix of 16-bit values, transposed
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
 
 // Four codes in a word -> two f16 pairs.  int8: x + 128 as the low byte of a half with exponent 2^10 is 1024 + 128 + x.
 template <int CODE>
@@ -305,19 +312,22 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT
       qa[j][NT + t] = w.y;
     }
   }
-  float qs[NT];
-  int lim[NT];
+  float qs[NT][2];                             // of rows 2c and 2c + 1, and 8 t further
+  int lim[NT][2];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    qs[t] = s_qs[g + 8 * t];
-    lim[t] = g + 8 * t < live ? (a.causal ? len - (n - 1 - query_of(r0 + g + 8 * t)) : len) : 0;
-  }
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = 2 * c + k + 8 * t;
+      qs[t][k] = s_qs[r];
+      lim[t][k] = r < live ? (a.causal ? len - (n - 1 - query_of(r0 + r)) : len) : 0;
+    }
   const int first_lim = a.causal ? len - (n - 1 - query_of(r0)) : len;        // the fewest keys of a live row
 
-  float o[MT][NT][4], m[NT], l[NT];
+  float o[MT][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    m[t] = -INFINITY, l[t] = 0.f;
+    m[t][0] = m[t][1] = -INFINITY, l[t][0] = l[t][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -365,19 +375,21 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT
       commit();
       const int place = from * STAGE;
       into = from, from = from + 1 == ST ? 0 : from + 1;
-      // ---- scores
-      float sc[2][4];
+      // ---- scores: (tokens token(g) and 8 further; rows 2c and 2c + 1)
+      float sc[NT][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.f;
-        uint4 w4;
+      for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          if (j % 4 == 0) w4 = kv8_shared16(k_at[j / 4] + place + 8 * h * D);
-          const uint32_t w = (j % 4) == 0 ? w4.x : (j % 4) == 1 ? w4.y : (j % 4) == 2 ? w4.z : w4.w;
-          uint32_t b0, b1;
-          kv8_halves<CODE>(w, b0, b1);
-          kv8_mma(sc[h], qa[j][0], NT == 2 ? qa[j][1] : 0u, qa[j][NT], NT == 2 ? qa[j][NT + 1] : 0u, b0, b1);
+      for (int i = 0; i < KW; ++i) {
+        const uint4 w0 = kv8_shared16(k_at[i] + place), w1 = kv8_shared16(k_at[i] + place + 8 * D);
+        const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a0, a1, a2, a3;
+          kv8_halves<CODE>(u0[j], a0, a2);
+          kv8_halves<CODE>(u1[j], a1, a3);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) kv8_mma(sc[t], a0, a1, a2, a3, qa[4 * i + j][t], qa[4 * i + j][NT + t]);
         }
       }
       const float kfac = __shfl_sync(0xffffffffu, kf, b & 31), vfac = __shfl_sync(0xffffffffu, vf, b & 31);
@@ -396,58 +408,55 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT
           vb[k][0] = w.x, vb[k][1] = w.y, vb[k][2] = w.z, vb[k][3] = w.w;
         }
       }
-      float x[NT][4];                         // (row g + 8 t; the same tokens)
+      float x[NT][4];
       bool rise = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float f = kfac * qs[t];
-        x[t][0] = sc[0][2 * t] * f, x[t][1] = sc[0][2 * t + 1] * f, x[t][2] = sc[1][2 * t] * f, x[t][3] = sc[1][2 * t + 1] * f;
+        const float f0 = kfac * qs[t][0], f1 = kfac * qs[t][1];
+        x[t][0] = sc[t][0] * f0, x[t][1] = sc[t][1] * f1, x[t][2] = sc[t][2] * f0, x[t][3] = sc[t][3] * f1;
       }
       if (edge) {
+        const int mine = t0 + Ring::token(g);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int tok = t0 + tok_of[k & 1] + 8 * (k >> 1);
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-            if (gone || tok >= lim[t]) x[t][k] = -INFINITY;
-          if (gone || tok >= len) {           // bytes behind the context are no codes
+          for (int k = 0; k < 4; ++k)
+            if (gone || mine + 8 * (k >> 1) >= lim[t][k & 1]) x[t][k] = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (gone || t0 + tok_of[k & 1] + 8 * (k >> 1) >= len) {        // bytes behind the context are no codes
 #pragma unroll
             for (int i = 0; i < VW; ++i) vb[k][i] = 0u;
           }
-        }
       }
 #pragma unroll
-      for (int t = 0; t < NT; ++t) rise |= fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])) > m[t];
+      for (int t = 0; t < NT; ++t) rise |= fmaxf(x[t][0], x[t][2]) > m[t][0] || fmaxf(x[t][1], x[t][3]) > m[t][1];
       if (__any_sync(0xffffffffu, rise)) {
-        float alpha[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          float mx = fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          mx = fmaxf(mx, m[t]);
-          alpha[t] = mx == -INFINITY ? 1.f : kv8_exp2(m[t] - mx);
-          l[t] *= alpha[t];
-          m[t] = mx;
-        }
-        // o's rows run along c: rows 2c and 2c + 1 of the tile, held for scores by lanes g = 2c and 2c + 1
+          float alpha[2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float a0 = __shfl_sync(0xffffffffu, alpha[t], 8 * c), a1 = __shfl_sync(0xffffffffu, alpha[t], 8 * c + 4);
+          for (int k = 0; k < 2; ++k) {
+            float mx = fmaxf(x[t][k], x[t][k + 2]);
 #pragma unroll
-          for (int i = 0; i < MT; ++i) o[i][t][0] *= a0, o[i][t][1] *= a1, o[i][t][2] *= a0, o[i][t][3] *= a1;
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            mx = fmaxf(mx, m[t][k]);
+            alpha[k] = mx == -INFINITY ? 1.f : kv8_exp2(m[t][k] - mx);
+            l[t][k] *= alpha[k];
+            m[t][k] = mx;
+          }
+#pragma unroll
+          for (int i = 0; i < MT; ++i) o[i][t][0] *= alpha[0], o[i][t][1] *= alpha[1], o[i][t][2] *= alpha[0], o[i][t][3] *= alpha[1];
         }
       }
       uint32_t p[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float mm = m[t] == -INFINITY ? 0.f : m[t];
-        float e[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = kv8_exp2(x[t][k] - mm);
-        l[t] += (e[0] + e[1]) + (e[2] + e[3]);
-        p[t][0] = kv8_half2(e[0] * vfac, e[1] * vfac);
-        p[t][1] = kv8_half2(e[2] * vfac, e[3] * vfac);
+        const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
+        const float e0 = kv8_exp2(x[t][0] - m0), e1 = kv8_exp2(x[t][1] - m1), e2 = kv8_exp2(x[t][2] - m0), e3 = kv8_exp2(x[t][3] - m1);
+        l[t][0] += e0 + e2, l[t][1] += e1 + e3;
+        p[t][0] = kv8_turn(kv8_half2(e0 * vfac, e1 * vfac));
+        p[t][1] = kv8_turn(kv8_half2(e2 * vfac, e3 * vfac));
       }
       // ---- values: channel tile i has channels 2 i and 2 i + 1 of the lane's
 #pragma unroll
@@ -465,11 +474,13 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT
 
   // ---- the warps' results together
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
-    l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
-    if (c == 0) s_m[iw][g + 8 * t] = m[t], s_l[iw][g + 8 * t] = l[t];
-  }
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) l[t][k] += __shfl_xor_sync(0xffffffffu, l[t][k], d);
+      if (g == 0) s_m[iw][2 * c + k + 8 * t] = m[t][k], s_l[iw][2 * c + k + 8 * t] = l[t][k];
+    }
   const float unit = vref * (1.f / 32768.f);
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncwarp();                               // the ring is done with
