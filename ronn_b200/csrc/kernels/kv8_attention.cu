@@ -108,8 +108,9 @@ __device__ __forceinline__ uint2 kv8_shared8(uint32_t at) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
   return v;
 }
+template <int TO, int FROM>
 __device__ __forceinline__ void kv8_copy16(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(to), "l"(from), "n"(TO), "n"(FROM) : "memory");
 }
 
 // The new K and V of one row into its slot, by one warp: kv8_append for a run of one token, K in lanes 0 to 15 and V in the
@@ -158,7 +159,7 @@ __device__ __forceinline__ void kv8_item_sync(int item) {
 // CTA's warps work on it.  NT = 1: at most 8 rows.  ST: blocks in a warp's ring, one at work and the others on their way.
 // A warp's first loads start before q is fetched: the chain length -> page -> codes is the longer one.
 template <class T, int D, int CODE, int NT, int WPI, int ST>
-__global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT == 1 ? 4 : 3)) kv8_attention_kernel(Kv8AttnArgs a, Kv8Turns turns) {
+__global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 4 : 2)) kv8_attention_kernel(Kv8AttnArgs a, Kv8Turns turns) {
   constexpr int KW = D / 64;                  // 16-byte loads of K a lane and 8 tokens
   constexpr int VB = D / 8;                   // bytes of V a lane and token
   constexpr int VW = VB / 4;
@@ -218,22 +219,31 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT
   const bool appends = slot >= 0 && cnt > 0 && w_hi == nblk;    // the warp that reads the last block writes the new token
 
   using Ring = Kv8Ring<D>;
-  // this lane's pieces of a block: piece lane + 32 i, for keys and for values
-  auto load = [&](int into, int p) {
-    const long base = (long(max(p, 0)) * a.kv_heads + kvh) * (KV8_BLOCK * D) + lane * 16;
-    const uint8_t* kp = a.kcodes + base;
-    const uint8_t* vp = a.vcodes + base;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      const int piece = lane + 32 * i;
-      const uint32_t to = ring_at + into * STAGE + Ring::at(piece / Ring::PIECES, piece % Ring::PIECES);
-      kv8_copy16(to, kp + i * 512);
-      kv8_copy16(to + KV8_BLOCK * D, vp + i * 512);
+  // this lane's pieces of a block: piece lane + 32 i, for keys and for values; for 128 channels the pieces of odd i, four rows
+  // further, are turned differently
+  constexpr int BYTES = KV8_BLOCK * D;
+  const uint8_t* const k_from = a.kcodes + long(kvh) * BYTES + lane * 16;
+  const uint8_t* const v_from = a.vcodes + long(kvh) * BYTES + lane * 16;
+  const uint32_t to_even = ring_at + Ring::at(lane / Ring::PIECES, lane % Ring::PIECES);
+  const uint32_t to_odd = ring_at + Ring::at(lane / Ring::PIECES + 32 / Ring::PIECES, lane % Ring::PIECES) - 512;
+  const uint32_t page_bytes = uint32_t(a.kv_heads) * BYTES;
+  auto load = [&](int at, int p) {              // the block of page p to byte `at` of the ring
+    const unsigned long long off = static_cast<unsigned long long>(uint32_t(p)) * page_bytes;
+    const uint8_t *kp = k_from + off, *vp = v_from + off;
+    kv8_copy16<0, 0>(to_even + at, kp);
+    kv8_copy16<BYTES, 0>(to_even + at, vp);
+    kv8_copy16<512, 512>(to_odd + at, kp);
+    kv8_copy16<BYTES + 512, 512>(to_odd + at, vp);
+    if constexpr (D == 128) {
+      kv8_copy16<1024, 1024>(to_even + at, kp);
+      kv8_copy16<BYTES + 1024, 1024>(to_even + at, vp);
+      kv8_copy16<1536, 1536>(to_odd + at, kp);
+      kv8_copy16<BYTES + 1536, 1536>(to_odd + at, vp);
     }
   };
   auto commit = [&] { asm volatile("cp.async.commit_group;" ::: "memory"); };
   // pages and scales are looked up for 32 blocks at a time, one a lane: pages two such groups ahead, scales one
-  auto page_of = [&](int b) {
+  auto page_of = [&](int b) {                   // -1: none
     int p = b < cnt ? bt[b] : -1;
     if (b < cnt && (p < 0 || p >= a.num_blocks)) kv8_report(a.status), p = -1;
     return p;
@@ -241,10 +251,12 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT
   auto scale_of = [&](const float* s, int p) { return p >= 0 ? s[long(p) * a.kv_heads + kvh] : 0.f; };
   int page = page_of(lane), page1 = page_of(32 + lane), page2 = -1;
   float kf = scale_of(a.kscale, page), vf = scale_of(a.vscale, page), kf1 = 0.f, vf1 = 0.f;
+  uint32_t gone_of = __ballot_sync(0xffffffffu, page < 0);        // of the 32 blocks at hand
+  page = max(page, 0);                          // what is loaded for a block without a page is not used
   const int early = appends ? min(cnt - 1, ST - 1) : min(cnt, ST - 1);        // the last block waits for its new token
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) {                                          // one group a block, empty ones among them
-    if (s < early) load(s, __shfl_sync(0xffffffffu, page, s));
+    if (s < early) load(s * STAGE, __shfl_sync(0xffffffffu, page, s));
     if (!appends || s < early) commit();
   }
 
@@ -294,7 +306,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT
       if (lane == cnt - 1 && page == slot / KV8_BLOCK) kf = ks, vf = vs;
     }
     for (int s = early; s < ST - 1; ++s) {
-      if (s == early) load(s, __shfl_sync(0xffffffffu, page, s));
+      if (s == early) load(s * STAGE, __shfl_sync(0xffffffffu, page, s));
       commit();
     }
   }
@@ -334,7 +346,6 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT
       for (int k = 0; k < 4; ++k) o[i][t][k] = 0.f;
   }
   float vref = 0.f;                            // o is in units of vref * 2^-15
-  uint32_t gone_of = __ballot_sync(0xffffffffu, page < 0);        // of the 32 blocks at hand
   // where this lane reads: keys of tokens token(g) and 8 further, values of c's tokens
   uint32_t k_at[KW], v_at[2];
 #pragma unroll
@@ -345,12 +356,12 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT
     tok_of[k] = Ring::token(2 * c + k);
     v_at[k] = ring_at + KV8_BLOCK * D + Ring::at(tok_of[k], g * VB / 16) + (g * VB) % 16;
   }
-  for (int b = 0, into = ST - 1, from = 0; b < cnt; ++b) {
+  for (int b = 0, into = (ST - 1) * STAGE, from = 0; b < cnt; ++b) {
     {
       if ((b & 31) == 0) {
         if (b > 0) {
-          page = page1, page1 = page2, kf = kf1, vf = vf1;
-          gone_of = __ballot_sync(0xffffffffu, page < 0);
+          gone_of = __ballot_sync(0xffffffffu, page1 < 0);
+          page = max(page1, 0), page1 = page2, kf = kf1, vf = vf1;
           if (vf != vf) kf = vf, vf = 0.f;
         }
         kf1 = scale_of(a.kscale, page1), vf1 = scale_of(a.vscale, page1);
@@ -371,10 +382,10 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 6 : 4) : (NT
       asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
       __syncwarp();                           // block b has landed, and every lane is done with block b - 1
       const int nb = b + ST - 1;
-      if (nb < cnt) load(into, __shfl_sync(0xffffffffu, ((nb ^ b) & 32) ? page1 : page, nb & 31));
+      if (nb < cnt) load(into, max(__shfl_sync(0xffffffffu, ((nb ^ b) & 32) ? page1 : page, nb & 31), 0));
       commit();
-      const int place = from * STAGE;
-      into = from, from = from + 1 == ST ? 0 : from + 1;
+      const int place = from;
+      into = from, from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
       // ---- scores: (tokens token(g) and 8 further; rows 2c and 2c + 1)
       float sc[NT][4];
 #pragma unroll
