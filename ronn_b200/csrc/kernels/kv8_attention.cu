@@ -16,10 +16,13 @@
 //                 interleaves the bytes of two.
 // Queries as B waste nothing on a decode step's missing rows: 8 products a block of 64 channels, not 12.
 // The 16-byte pieces of a row stand in the ring in an order that depends on the row (Kv8Ring), so that neither read meets a
-// bank twice.  Blocks held in registers instead cost 48 of them and with them a third of the warps an SM can hold.
+// bank twice.  256 rows of 64 to 768 keys, 16 heads of 64 in int8, took 76 us with the blocks in registers (48 of them, and not
+// enough left), 76 with the ring and 80 registers a thread, 61 with the ring and 128: 16 warps an SM without spills beat 24
+// with.  What bounds it there is the instructions of a block, 226, a third of which turn int8 into f16; e4m3 has one for each
+// two codes and reaches 5 TB/s on long contexts.
 // Codes become f16 exactly.  Q in bf16 is scaled by a power of two for each row, so that it fits f16 (its 8 significant bits
 // do; what is 2^-34 of the row's largest is lost).  Softmax statistics, sums and O are in 32 bits; P is rounded to f16 as
-// 2^15 p, 2^-12 of it and never more than 2^-40.  The scale of a K block multiplies its scores, that of a V block its P,
+// 2^15 p, by at most 2^-11 of it or 2^-40.  The scale of a K block multiplies its scores, that of a V block its P,
 // relative to the largest V scale of the 32 blocks that the warp looks up together.
 #include "kv8.cuh"
 
@@ -534,41 +537,39 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
   }
 }
 
-// The shares of a row together: one warp for each row of each tile.
-template <class T, int D>
-__global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8AttnArgs a, long tiles) {
+// The shares of a row together: one CTA of CW warps for each row of each tile.  A warp weighs 32 shares at a time, one a lane,
+// and adds those of its own number; the warps' sums meet in shared memory, in order.  37 shares of 96 rows take 6 us with four
+// warps and 11 with one, 3 shares of 3456 rows are faster with one (chunks of 1 to 24 queries: 24.6 against 26.4 us in all).
+template <class T, int D, int KV8_CW>
+__global__ void __launch_bounds__(KV8_CW * 32) kv8_combine_kernel(Kv8AttnArgs a) {
+  constexpr int PER = D / 32;
+  __shared__ float s_acc[KV8_CW][D];
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const long unit = long(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const long tile = unit / a.part_rows;
-  const int r = int(unit - tile * a.part_rows);
-  if (tile >= tiles) return;
-  const int x = int(tile % a.items_x), r0 = int(tile / a.items_x) * 16;
-  const int seq = x / a.kv_heads, kvh = x - seq * a.kv_heads, group = a.heads / a.kv_heads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tile = int(blockIdx.x / a.part_rows), r = int(blockIdx.x) - tile * a.part_rows;
+  const int x = tile % a.items_x, r0 = tile / a.items_x * 16;
+  const int seq = x / a.kv_heads, kvh = x - seq * a.kv_heads, group = a.group;
   const int n = a.q_len ? a.q_len[seq] : 1;
   if (r0 + r >= n * group || r >= 16) return;
   const long row0 = a.seq_start ? long(a.seq_start[seq]) : seq;
   if (row0 < 0 || row0 + n > a.rows) return;
-  const float* src = a.part + (tile * a.splits * a.part_rows + r) * (D + 2);
+  const float* src = a.part + (long(tile) * a.splits * a.part_rows + r) * (D + 2);
   const long step = long(a.part_rows) * (D + 2);
-  constexpr int PER = D / 32;
-  float acc[PER], sum = 0.f, mx = -INFINITY;
+  auto share = [&](int z) { return z < a.splits ? *reinterpret_cast<const float2*>(src + z * step + D) : make_float2(-INFINITY, 0.f); };
+  float mx = -INFINITY;                                      // the row's maximum and sum, the same in every warp
+  for (int z0 = 0; z0 < a.splits; z0 += 32) mx = fmaxf(mx, share(z0 + lane).x);
+  mx = warp_max(mx);
+  float acc[PER], sum = 0.f;
 #pragma unroll
   for (int k = 0; k < PER; ++k) acc[k] = 0.f;
-  for (int z0 = 0; z0 < a.splits; z0 += 32) {             // a share's maximum and sum to a lane, 32 shares at a time
-    const int z = z0 + lane;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (z < a.splits) ml = *reinterpret_cast<const float2*>(src + z * step + D);
-    const float top = fmaxf(mx, warp_max(ml.x)), down = sum == 0.f ? 0.f : kv8_weight(mx, sum, top);
-    const float w = kv8_weight(ml.x, ml.y, top);
-    sum = (down != 0.f ? sum * down : 0.f) + warp_sum(w != 0.f ? w * ml.y : 0.f);
-#pragma unroll
-    for (int k = 0; k < PER; ++k) acc[k] = down != 0.f ? acc[k] * down : 0.f;
-    mx = top;
-    const int n_here = min(32, a.splits - z0);
-#pragma unroll 8
-    for (int i = 0; i < n_here; ++i) {
+  for (int z0 = 0; z0 < a.splits; z0 += 32) {
+    const float2 ml = share(z0 + lane);
+    const float w = kv8_weight(ml.x, ml.y, mx);
+    sum += w != 0.f ? w * ml.y : 0.f;
+    const int here = min(32, a.splits - z0);
+#pragma unroll 4
+    for (int i = warp; i < here; i += KV8_CW) {
       const float f = __shfl_sync(0xffffffffu, w, i);
       const float* v = src + (z0 + i) * step + lane * PER;
       float part[PER];
@@ -581,30 +582,42 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(Kv8AttnArgs a, long ti
       for (int k = 0; k < PER; ++k) acc[k] += f != 0.f ? f * part[k] : 0.f;
     }
   }
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  T* dst = static_cast<T*>(a.out) + (row0 + (r0 + r) / group) * a.ld_o + long(kvh * group + (r0 + r) % group) * D + lane * PER;
+  sum = warp_sum(sum);
 #pragma unroll
-  for (int k = 0; k < PER; k += 2) *reinterpret_cast<uint32_t*>(dst + k) = Pair16<T>::pack(acc[k] * inv, acc[k + 1] * inv);
+  for (int k = 0; k < PER; ++k) s_acc[warp][lane * PER + k] = acc[k];
+  __syncthreads();
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  for (int i = threadIdx.x; i < D / 2; i += KV8_CW * 32) {
+    float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < KV8_CW; ++w) v0 += s_acc[w][2 * i], v1 += s_acc[w][2 * i + 1];
+    T* dst = static_cast<T*>(a.out) + (row0 + (n == 1 ? 0 : (r0 + r) / group)) * a.ld_o;
+    dst += long(kvh * group + (n == 1 ? r0 + r : (r0 + r) % group)) * D + 2 * i;
+    *reinterpret_cast<uint32_t*>(dst) = Pair16<T>::pack(v0 * inv, v1 * inv);
+  }
 }
 
 }  // namespace ronn
 
 using namespace ronn;
 
+constexpr int KV8_SHARE = 32;
 struct Kv8Plan {
   int wpi, splits, share;      // warps of an item, CTAs along a context, cache blocks each of them takes
 };
 
-// Warps of an item: two where that gives every SM's schedulers at least two rounds of warps, else four.  A context is cut
-// into equal shares, whatever its row's length, so that long rows give more CTAs and not longer ones; shares are taken for
-// about six CTAs an SM at the longest context, of 64 blocks at least.
+// Warps of an item: two where that gives every SM's schedulers at least two rounds of warps, else four.  256 rows of 64 to 768
+// keys, 16 heads of 64, took 72, 65.5 and 72 us with one, two and four; 128 rows of 41 to 577 keys, 20 heads of 128: 72, 65.5 and
+// 65.5.  A context is cut into equal shares, whatever its row's length, so that long rows give more CTAs and not longer ones;
+// shares are taken for about six CTAs an SM at the longest context, of KV8_SHARE blocks at least (chunks of 1 to 24 queries over
+// 200 to 1500 keys: 28.7, 26.4 and 28.6 us with at least 16, 32 and 64).
 static Kv8Plan kv8_plan(long tiles, int max_ctx) {
   const int sms = device_sm_count(), nblk = (max_ctx + KV8_BLOCK - 1) / KV8_BLOCK;
   Kv8Plan p{tiles >= 8L * sms ? 2 : 4, 1, nblk > 0 ? nblk : 1};
   const long want = tiles > 0 ? 6L * sms / tiles : 1;
-  if (want > 1 && nblk > 64) {
+  if (want > 1 && nblk > KV8_SHARE) {
     const long share = (nblk + want - 1) / want;
-    p.share = int(share < 64 ? 64 : share);
+    p.share = int(share < KV8_SHARE ? KV8_SHARE : share);
     p.splits = (nblk + p.share - 1) / p.share;
     if (p.splits > 1) p.wpi = 4;
   }
@@ -630,7 +643,7 @@ extern "C" int ronn_kv8_attention(const Kv8AttnCall* call, cudaStream_t stream) 
   if (positions && (!turns || !slots)) return -2;
   if (head_dim != 64 && head_dim != 128) return -1;
   const long group_rows = long(max_q_len) * (heads / kv_heads), mtiles = (group_rows + 15) / 16, xs = long(n_seq) * kv_heads;
-  if (xs > 2147483647L || mtiles > 65535) return -2;
+  if (xs > 2147483647L || mtiles > 65535 || xs * mtiles * 16 > 2147483647L) return -2;
   const Kv8Plan plan = kv8_plan(xs * mtiles, max_ctx);
   const int splits = plan.splits, wpi = plan.wpi;
   const int part_rows = int(group_rows < 16 ? group_rows : 16);
@@ -670,7 +683,8 @@ extern "C" int ronn_kv8_attention(const Kv8AttnCall* call, cudaStream_t stream) 
     else return -1; \
     if (splits > 1) { \
       const long units = xs * mtiles * part_rows; \
-      launch(kv8_combine_kernel<T, D>, dim3(unsigned((units + 3) / 4)), dim3(128), 0, stream, a, xs * mtiles); \
+      if (splits > 8) launch(kv8_combine_kernel<T, D, 4>, dim3(unsigned(units)), dim3(128), 0, stream, a); \
+      else launch(kv8_combine_kernel<T, D, 1>, dim3(unsigned(units)), dim3(32), 0, stream, a); \
     } \
   } while (0)
   if (dtype == 0 && head_dim == 64) RONN_KV8T_(__nv_bfloat16, 64);

@@ -348,19 +348,19 @@ extern "C" long ronn_kv8_chunk_scratch(int n_seq, int max_kv, int kv_heads, int 
 }
 
 // Whether chunks of these sizes are faster that way (1) or straight from the codes (0), by what both cost in microseconds.
-// Expanded: a chain of 128-key tiles for each 128 queries and head, 2.2 us a tile (2.3 for heads of 128) while the SMs have
-// one such CTA each, and the values written and read.  Direct: 0.6 ns (1.0) for each 16 query rows and 16 keys.  Over 252 sizes
-// (1 to 16 sequences, contexts of 300 to 4000, 16 to 256 queries, four head layouts) the rule costs 0.5 % against the faster
-// form of each on average and 23 % at worst; 16 x 128 queries over 4000 keys, 32 / 8 heads of 128: 401 against 802 us; 4 x 32
-// queries over 4000 keys, 16 heads of 64: 86 against 33.
+// Expanded: a chain of 128-key tiles for each 128 queries and head, 2.4 us a tile (2.2 for heads of 128) while the SMs have
+// one such CTA each, and the values.  Direct: 0.4 ns (0.55) for each 16 query rows and 16 keys.  Over 252 sizes (1 to 16
+// sequences, contexts of 300 to 4000, 16 to 256 queries, four head layouts) the rule costs 0.3 % (1.0 %) against the faster
+// form of each on average and 12 % (27 %) at worst; 16 x 128 queries over 4000 keys, 32 / 8 heads of 128: 404 us against 670
+// direct; 4 x 32 queries over 4000 keys, 16 heads of 64: 86 against 37.
 extern "C" int ronn_kv8_chunk_form(int n_seq, int max_q, int max_ctx, int heads, int kv_heads, int head_dim) {
   if (n_seq <= 0 || max_q <= 0 || max_ctx <= 0 || kv_heads <= 0) return 0;
   const bool wide = head_dim > 64;
-  const double ctas = double(n_seq) * heads * ((max_q + 127) / 128) / device_sm_count() * (wide ? 1.0 : 0.8);
-  const double expanded = 11 + (max_ctx + 127) / 128 * (wide ? 2.3 : 2.2) * (ctas > 1 ? ctas : 1) +
-                          double(n_seq) * max_ctx * kv_heads * head_dim * 4 / 6.5e6;
+  const double ctas = double(n_seq) * heads * ((max_q + 127) / 128) / device_sm_count() * (wide ? 0.9 : 0.7);
+  const double expanded = 11 + (max_ctx + 127) / 128 * (wide ? 2.2 : 2.4) * (ctas > 1 ? ctas : 1) +
+                          double(n_seq) * max_ctx * kv_heads * head_dim * 2 / 6.5e6;
   const double tiles = double(n_seq) * kv_heads * ((long(max_q) * (heads / kv_heads) + 15) / 16);
-  return expanded < 12 + tiles * ((max_ctx + 15) / 16) * (wide ? 1e-3 : 0.6e-3);
+  return expanded < 15 + tiles * ((max_ctx + 15) / 16) * (wide ? 0.55e-3 : 0.4e-3);
 }
 
 // The same call as ronn_kv8_attention with queries grouped by sequence, no append, and scale > 0.

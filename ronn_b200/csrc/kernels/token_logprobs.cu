@@ -524,11 +524,18 @@ static int launch_token_logprobs(const TlArgs& a, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a) == cudaSuccess ? 0 : -100;
 }
 
-// logits: [rows, ld], dtype 0 bf16, 1 fp16, 2 fp32; tokens: int32 (wide_tokens: int64) every token_stride values, or null (a
-// token outside [0, vocab) is not given: log probability 0, rank 0); top_ids, top_logprobs: [rows, top], top <= min(vocab, 32).
-extern "C" int ronn_token_logprobs(const void* logits, long ld, int vocab, long rows, const void* tokens, long token_stride,
-                                   int wide_tokens, float* logprob, int* rank, float* entropy, int* top_ids, float* top_logprobs,
-                                   int top, int dtype, cudaStream_t stream) {
+// One call.  logits: [rows, ld], dtype 0 bf16, 1 fp16, 2 fp32; tokens: int32 (wide_tokens: int64) every token_stride values, or
+// null (a token outside [0, vocab) is not given: log probability 0, rank 0); top_ids, top_logprobs: [rows, top], top <= min(vocab, 32).
+struct TokenLogprobsCall {
+  const void *logits, *tokens;
+  float *logprob, *entropy, *top_logprobs;
+  int *rank, *top_ids;
+  long ld, rows, token_stride;
+  int vocab, wide_tokens, top, dtype;
+};
+
+extern "C" int ronn_token_logprobs(const TokenLogprobsCall* call, cudaStream_t stream) {
+  const auto& [logits, tokens, logprob, entropy, top_logprobs, rank, top_ids, ld, rows, token_stride, vocab, wide_tokens, top, dtype] = *call;
   if (rows <= 0) return 0;
   if (vocab <= 0 || vocab > (1 << 30) || top < 0 || top > TL_TOP || top > vocab || rows > 2147483647L / TL_CLUSTER) return -2;
   if (dtype < 0 || dtype > 2) return -1;

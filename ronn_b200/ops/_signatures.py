@@ -54,7 +54,7 @@ def declare(lib):
     sig("ronn_kv8_chunk_scratch", [I, I, I, I], restype=L)
     sig("ronn_kv8_chunk_form", [I, I, I, I, I, I])
     sig("ronn_kv8_attention_scratch", [I, I, I, I, I, I], restype=L)
-    sig("ronn_token_logprobs", [V, L, I, L, V, L, I, V, V, V, V, V, I, I, V])
+    sig("ronn_token_logprobs", [C.c_char_p, V])
     sig("ronn_fmha", [V, L, L, I, I, I, V, V, V, V, L, I, I, I, I, I, I, F, I, V, V])
     sig("ronn_fmha_paged", [V, L, L, I, V, V, L, V, I, V, V, V, V, V, L, I, I, I, I, I, I, F, I, V, V])
     sig("ronn_conv2d", [V, V, V, V, V, I, I, I, I, I, I, I, I, I, I, I, I, I, I, V, L, V, V], optional=True)

@@ -1,14 +1,16 @@
 """Log probabilities of tokens from logits: what a served request that asks for them is answered with, and how texts are scored."""
 from __future__ import annotations
 
+import struct
 from typing import NamedTuple, Optional
 
 import torch
 
 from .. import _native
-from .kernels import OperandError, _DT, _check, _ptr
+from .kernels import OperandError, _DT, _check
 
 MAX_TOP = 32
+_CALL = struct.Struct("=7Q3q4i")            # the launcher's call record (token_logprobs.cu)
 
 
 class TokenLogprobs(NamedTuple):
@@ -43,13 +45,16 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         with torch.cuda.device(index):
             return token_logprobs(logits, tokens, top)
     top = int(top)
-    f = torch.empty((2 + top, rows) if rows else (2, 0), dtype=torch.float32, device=dev)
-    i = torch.empty(((1 + top) * rows,), dtype=torch.int32, device=dev)
-    rank, ids, tops = i[:rows], i[rows:].view(rows, top), f[2:].view(rows, top)
-    wide = tokens is not None and tokens.dtype is torch.int64
-    rc = _native.cuda().ronn_token_logprobs(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, vocab, rows, _ptr(tokens),
-                                            (tokens.stride(0) if rows > 1 else 1) if tokens is not None else 0, 1 if wide else 0,
-                                            f.data_ptr(), rank.data_ptr(), f.data_ptr() + 4 * rows, ids.data_ptr(), tops.data_ptr(), top,
-                                            _DT[logits.dtype], torch._C._cuda_getCurrentRawStream(index))
+    f = torch.empty((2 + top) * rows, dtype=torch.float32, device=dev)
+    i = torch.empty((1 + top) * rows, dtype=torch.int32, device=dev)
+    logprob, entropy, tops = f.split((rows, rows, top * rows))
+    rank, ids = i.split((rows, top * rows))
+    at, ints = f.data_ptr(), i.data_ptr()
+    token_ptr, stride, wide = 0, 0, 0
+    if tokens is not None:
+        token_ptr, stride, wide = tokens.data_ptr(), tokens.stride(0) if rows > 1 else 1, int(tokens.dtype is torch.int64)
+    rc = _native.cuda().ronn_token_logprobs(_CALL.pack(logits.data_ptr(), token_ptr, at, at + 4 * rows, at + 8 * rows, ints, ints + 4 * rows,
+                                                       logits.stride(0) if rows > 1 else vocab, rows, stride, vocab, wide, top,
+                                                       _DT[logits.dtype]), torch._C._cuda_getCurrentRawStream(index))
     _check(rc, "token_logprobs")
-    return TokenLogprobs(f[0], rank, f[1], ids, tops)
+    return TokenLogprobs(logprob, rank, entropy, ids.view(rows, top), tops.view(rows, top))
