@@ -18,8 +18,9 @@
 // The 16-byte pieces of a row stand in the ring in an order that depends on the row (Kv8Ring), so that neither read meets a
 // bank twice.  256 rows of 64 to 768 keys, 16 heads of 64 in int8, took 76 us with the blocks in registers (48 of them, and not
 // enough left), 76 with the ring and 80 registers a thread, 61 with the ring and 128: 16 warps an SM without spills beat 24
-// with.  What bounds it there is the instructions of a block, 226, a third of which turn int8 into f16; e4m3 has one for each
-// two codes and reaches 5 TB/s on long contexts.
+// with.  54 us of the 61 are this kernel: it issues in 59 % of its cycles, about 180 instructions a block (a third of them turn
+// int8 into f16; e4m3 takes one for two codes) and 1100 a warp around them, and the longest rows are alone at the end.  Long
+// contexts of e4m3 go by at 5 TB/s.
 // Codes become f16 exactly.  Q in bf16 is scaled by a power of two for each row, so that it fits f16 (its 8 significant bits
 // do; what is 2^-34 of the row's largest is lost).  Softmax statistics, sums and O are in 32 bits; P is rounded to f16 as
 // 2^15 p, by at most 2^-11 of it or 2^-40.  The scale of a K block multiplies its scores, that of a V block its P,
@@ -101,14 +102,16 @@ template <int D> struct Kv8Ring {
   static __device__ __forceinline__ int token(int n) { return D == 64 ? n ^ ((n >> 1) & 1) : n; }
   static __device__ __forceinline__ int at(int t, int piece) { return t * D + ((piece ^ turn(t)) << 4); }
 };
+template <int OFF>
 __device__ __forceinline__ uint4 kv8_shared16(uint32_t at) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at), "n"(OFF) : "memory");
   return v;
 }
+template <int OFF>
 __device__ __forceinline__ uint2 kv8_shared8(uint32_t at) {
   uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(v.x), "=r"(v.y) : "r"(at), "n"(OFF) : "memory");
   return v;
 }
 template <int TO, int FROM>
@@ -159,9 +162,9 @@ __device__ __forceinline__ void kv8_item_sync(int item) {
 }
 
 // An item is a tile of up to 16 query rows of one (sequence, KV head), and one of `splits` shares of its blocks; WPI of the
-// CTA's warps work on it.  NT = 1: at most 8 rows.  ST: blocks in a warp's ring, one at work and the others on their way.
+// CTA's warps work on it.  NT = 1: at most 8 rows.  U: blocks a warp works on at a time; ST: blocks in its ring, U at work and the others on their way.
 // A warp's first loads start before q is fetched: the chain length -> page -> codes is the longer one.
-template <class T, int D, int CODE, int NT, int WPI, int ST>
+template <class T, int D, int CODE, int NT, int WPI, int U, int ST>
 __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 4 : 2)) kv8_attention_kernel(Kv8AttnArgs a, Kv8Turns turns) {
   constexpr int KW = D / 64;                  // 16-byte loads of K a lane and 8 tokens
   constexpr int VB = D / 8;                   // bytes of V a lane and token
@@ -256,11 +259,14 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
   float kf = scale_of(a.kscale, page), vf = scale_of(a.vscale, page), kf1 = 0.f, vf1 = 0.f;
   uint32_t gone_of = __ballot_sync(0xffffffffu, page < 0);        // of the 32 blocks at hand
   page = max(page, 0);                          // what is loaded for a block without a page is not used
-  const int early = appends ? min(cnt - 1, ST - 1) : min(cnt, ST - 1);        // the last block waits for its new token
+  constexpr int AHEAD = ST - U;                // blocks on their way, a group of U at a time
+  static_assert(ST % U == 0 && AHEAD > 0, "whole groups");
+  const int early = appends ? min(cnt - 1, AHEAD) : min(cnt, AHEAD);          // the last block waits for its new token
+  const int held = appends && early < AHEAD ? early / U : AHEAD;             // and with it its group
 #pragma unroll
-  for (int s = 0; s < ST - 1; ++s) {                                          // one group a block, empty ones among them
+  for (int s = 0; s < AHEAD; ++s) {
     if (s < early) load(s * STAGE, __shfl_sync(0xffffffffu, page, s));
-    if (!appends || s < early) commit();
+    if (s % U == U - 1 && s / U < held) commit();
   }
 
   // ---- q to shared memory: rotated, scaled to f16
@@ -268,11 +274,11 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
     for (int j = it; j < D / 2; j += WPI * 32) s_cs[kv8_angle_at<D>(j)] = kv8_cos_sin(turns.t[j], pos);
     kv8_item_sync<WPI>(in_cta);
   }
-  for (int r = iw; r < R; r += WPI) {
+  for (int r = iw; r < live; r += WPI) {
     const int chunk = lane % CH;
-    uint4 h = make_uint4(0u, 0u, 0u, 0u);
-    float down = 0.f;
-    if (r < live) {
+    uint4 h;
+    float down;
+    {
       const int t = query_of(r0 + r), head = kvh * group + r0 + r - t * group;
       Vec8 x = *reinterpret_cast<const Vec8*>(static_cast<const T*>(a.q) + (row0 + t) * a.ld_q + long(head) * D + chunk * 8);
       if (a.positions) {
@@ -308,9 +314,9 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
       __syncwarp();
       if (lane == cnt - 1 && page == slot / KV8_BLOCK) kf = ks, vf = vs;
     }
-    for (int s = early; s < ST - 1; ++s) {
-      if (s == early) load(s * STAGE, __shfl_sync(0xffffffffu, page, s));
-      commit();
+    if (early < AHEAD) {
+      load(early * STAGE, __shfl_sync(0xffffffffu, page, early));
+      for (int s = held; s < AHEAD / U; ++s) commit();
     }
   }
   if (vf != vf) kf = vf, vf = 0.f;              // seeing the block's keys is seeing its values: NaN through the scores
@@ -322,7 +328,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
     const int ch = (j / 4) * 64 + c * 16 + (j % 4) * 4;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const uint2 w = *reinterpret_cast<const uint2*>(&s_q[g + 8 * t][ch]);
+      const uint2 w = g + 8 * t < live ? *reinterpret_cast<const uint2*>(&s_q[g + 8 * t][ch]) : make_uint2(0u, 0u);
       qa[j][t] = w.x;
       qa[j][NT + t] = w.y;
     }
@@ -334,7 +340,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int r = 2 * c + k + 8 * t;
-      qs[t][k] = s_qs[r];
+      qs[t][k] = r < live ? s_qs[r] : 0.f;
       lim[t][k] = r < live ? (a.causal ? len - (n - 1 - query_of(r0 + r)) : len) : 0;
     }
   const int first_lim = a.causal ? len - (n - 1 - query_of(r0)) : len;        // the fewest keys of a live row
@@ -359,43 +365,50 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
     tok_of[k] = Ring::token(2 * c + k);
     v_at[k] = ring_at + KV8_BLOCK * D + Ring::at(tok_of[k], g * VB / 16) + (g * VB) % 16;
   }
-  for (int b = 0, into = (ST - 1) * STAGE, from = 0; b < cnt; ++b) {
-    {
-      if ((b & 31) == 0) {
-        if (b > 0) {
-          gone_of = __ballot_sync(0xffffffffu, page1 < 0);
-          page = max(page1, 0), page1 = page2, kf = kf1, vf = vf1;
-          if (vf != vf) kf = vf, vf = 0.f;
-        }
-        kf1 = scale_of(a.kscale, page1), vf1 = scale_of(a.vscale, page1);
-        page2 = page_of(b + 64 + lane);
-        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vf)));
-        if (top > vref) {
-          const float down = vref * kv8_inverse(top);          // 0 the first time
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) o[i][t][k] *= down;
-          vref = top;
-        }
-        vf *= kv8_inverse(vref) * 32768.f;
+  for (int b = 0, into = AHEAD * STAGE, from = 0; b < cnt; b += U) {
+    if ((b & 31) == 0) {
+      if (b > 0) {
+        gone_of = __ballot_sync(0xffffffffu, page1 < 0);
+        page = max(page1, 0), page1 = page2, kf = kf1, vf = vf1;
+        if (vf != vf) kf = vf, vf = 0.f;
       }
-      asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
-      __syncwarp();                           // block b has landed, and every lane is done with block b - 1
-      const int nb = b + ST - 1;
-      if (nb < cnt) load(into, max(__shfl_sync(0xffffffffu, ((nb ^ b) & 32) ? page1 : page, nb & 31), 0));
-      commit();
-      const int place = from;
-      into = from, from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
-      // ---- scores: (tokens token(g) and 8 further; rows 2c and 2c + 1)
-      float sc[NT][4];
+      kf1 = scale_of(a.kscale, page1), vf1 = scale_of(a.vscale, page1);
+      page2 = page_of(b + 64 + lane);
+      const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vf)));
+      if (top > vref) {
+        const float down = vref * kv8_inverse(top);          // 0 the first time
 #pragma unroll
-      for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[i][t][k] *= down;
+        vref = top;
+      }
+      vf *= kv8_inverse(vref) * 32768.f;
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD / U - 1) : "memory");
+    __syncwarp();                             // blocks b .. have landed, and every lane is done with those before
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int nb = b + AHEAD + u;
+      if (nb < cnt) load(into + u * STAGE, max(__shfl_sync(0xffffffffu, ((nb ^ b) & 32) ? page1 : page, nb & 31), 0));
+    }
+    commit();
+    const int place = from;
+    into = from, from = from + U * STAGE == ST * STAGE ? 0 : from + U * STAGE;
+    // ---- scores: (tokens token(g) and 8 further; rows 2c and 2c + 1)
+    float x[U][NT][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) x[u][t][0] = x[u][t][1] = x[u][t][2] = x[u][t][3] = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < KW; ++i) {
-        const uint4 w0 = kv8_shared16(k_at[i] + place), w1 = kv8_shared16(k_at[i] + place + 8 * D);
+        const uint32_t at = k_at[i] + place;
+        const uint4 w0 = kv8_shared16<0>(at + u * STAGE), w1 = kv8_shared16<8 * D>(at + u * STAGE);
         const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -403,76 +416,93 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
           kv8_halves<CODE>(u0[j], a0, a2);
           kv8_halves<CODE>(u1[j], a1, a3);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) kv8_mma(sc[t], a0, a1, a2, a3, qa[4 * i + j][t], qa[4 * i + j][NT + t]);
+          for (int t = 0; t < NT; ++t) kv8_mma(x[u][t], a0, a1, a2, a3, qa[4 * i + j][t], qa[4 * i + j][NT + t]);
         }
       }
-      const float kfac = __shfl_sync(0xffffffffu, kf, b & 31), vfac = __shfl_sync(0xffffffffu, vf, b & 31);
-      const bool gone = (gone_of >> (b & 31)) & 1;
-      const int t0 = (w_lo + b) * KV8_BLOCK;
-      const bool edge = gone || t0 + KV8_BLOCK > first_lim;
-      uint32_t vb[4][VW];                     // c's tokens tok_of[0], tok_of[1], and 8 further
+    float vfac[U];
+    bool rise = false;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t src = v_at[k & 1] + place + 8 * (k >> 1) * D;
-        if constexpr (VW == 2) {
-          const uint2 w = kv8_shared8(src);
-          vb[k][0] = w.x, vb[k][1] = w.y;
-        } else {
-          const uint4 w = kv8_shared16(src);
-          vb[k][0] = w.x, vb[k][1] = w.y, vb[k][2] = w.z, vb[k][3] = w.w;
-        }
-      }
-      float x[NT][4];
-      bool rise = false;
+    for (int u = 0; u < U; ++u) {
+      const float kfac = __shfl_sync(0xffffffffu, kf, (b + u) & 31);
+      vfac[u] = __shfl_sync(0xffffffffu, vf, (b + u) & 31);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const float f0 = kfac * qs[t][0], f1 = kfac * qs[t][1];
-        x[t][0] = sc[t][0] * f0, x[t][1] = sc[t][1] * f1, x[t][2] = sc[t][2] * f0, x[t][3] = sc[t][3] * f1;
+        x[u][t][0] *= f0, x[u][t][1] *= f1, x[u][t][2] *= f0, x[u][t][3] *= f1;
       }
-      if (edge) {
-        const int mine = t0 + Ring::token(g);
+    }
+    const uint32_t gone = (gone_of >> (b & 31)) & ((1u << U) - 1u);          // blocks without a page, or behind the warp's last
+    const int t0 = (w_lo + b) * KV8_BLOCK;
+    const bool edge = gone || t0 + U * KV8_BLOCK > first_lim;
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int mine = (gone >> u) & 1 ? 0x7fffffff - 8 : t0 + u * KV8_BLOCK + Ring::token(g);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (gone || mine + 8 * (k >> 1) >= lim[t][k & 1]) x[t][k] = -INFINITY;
+            if (mine + 8 * (k >> 1) >= lim[t][k & 1]) x[u][t][k] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) rise |= fmaxf(x[u][t][0], x[u][t][2]) > m[t][0] || fmaxf(x[u][t][1], x[u][t][3]) > m[t][1];
+    if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float alpha[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float mx = m[t][k];
+#pragma unroll
+          for (int u = 0; u < U; ++u) mx = fmaxf(mx, fmaxf(x[u][t][k], x[u][t][k + 2]));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          alpha[k] = mx == -INFINITY ? 1.f : kv8_exp2(m[t][k] - mx);
+          l[t][k] *= alpha[k];
+          m[t][k] = mx;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) o[i][t][0] *= alpha[0], o[i][t][1] *= alpha[1], o[i][t][2] *= alpha[0], o[i][t][3] *= alpha[1];
+      }
+    }
+    uint32_t p[U][NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float e0 = kv8_exp2(x[u][t][0] - m0), e1 = kv8_exp2(x[u][t][1] - m1), e2 = kv8_exp2(x[u][t][2] - m0), e3 = kv8_exp2(x[u][t][3] - m1);
+        l[t][0] += e0 + e2, l[t][1] += e1 + e3;
+        p[u][t][0] = kv8_turn(kv8_half2(e0 * vfac[u], e1 * vfac[u]));
+        p[u][t][1] = kv8_turn(kv8_half2(e2 * vfac[u], e3 * vfac[u]));
+      }
+    }
+    // ---- values: channel tile i has channels 2 i and 2 i + 1 of the lane's
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t vb[4][VW];                     // c's tokens tok_of[0], tok_of[1], and 8 further
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t src = v_at[k & 1] + place + u * STAGE;
+        if constexpr (VW == 2) {
+          const uint2 w = k < 2 ? kv8_shared8<0>(src) : kv8_shared8<8 * D>(src);
+          vb[k][0] = w.x, vb[k][1] = w.y;
+        } else {
+          const uint4 w = k < 2 ? kv8_shared16<0>(src) : kv8_shared16<8 * D>(src);
+          vb[k][0] = w.x, vb[k][1] = w.y, vb[k][2] = w.z, vb[k][3] = w.w;
+        }
+      }
+      if (edge) {                             // bytes behind the context are no codes
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (gone || t0 + tok_of[k & 1] + 8 * (k >> 1) >= len) {        // bytes behind the context are no codes
+          if (((gone >> u) & 1) || t0 + u * KV8_BLOCK + tok_of[k & 1] + 8 * (k >> 1) >= len) {
 #pragma unroll
             for (int i = 0; i < VW; ++i) vb[k][i] = 0u;
           }
       }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) rise |= fmaxf(x[t][0], x[t][2]) > m[t][0] || fmaxf(x[t][1], x[t][3]) > m[t][1];
-      if (__any_sync(0xffffffffu, rise)) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          float alpha[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float mx = fmaxf(x[t][k], x[t][k + 2]);
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            mx = fmaxf(mx, m[t][k]);
-            alpha[k] = mx == -INFINITY ? 1.f : kv8_exp2(m[t][k] - mx);
-            l[t][k] *= alpha[k];
-            m[t][k] = mx;
-          }
-#pragma unroll
-          for (int i = 0; i < MT; ++i) o[i][t][0] *= alpha[0], o[i][t][1] *= alpha[1], o[i][t][2] *= alpha[0], o[i][t][3] *= alpha[1];
-        }
-      }
-      uint32_t p[NT][2];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float m0 = m[t][0] == -INFINITY ? 0.f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
-        const float e0 = kv8_exp2(x[t][0] - m0), e1 = kv8_exp2(x[t][1] - m1), e2 = kv8_exp2(x[t][2] - m0), e3 = kv8_exp2(x[t][3] - m1);
-        l[t][0] += e0 + e2, l[t][1] += e1 + e3;
-        p[t][0] = kv8_turn(kv8_half2(e0 * vfac, e1 * vfac));
-        p[t][1] = kv8_turn(kv8_half2(e2 * vfac, e3 * vfac));
-      }
-      // ---- values: channel tile i has channels 2 i and 2 i + 1 of the lane's
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int w = i / 2;
@@ -481,7 +511,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
         kv8_halves<CODE>(__byte_perm(vb[0][w], vb[1][w], sel), a0, a1);
         kv8_halves<CODE>(__byte_perm(vb[2][w], vb[3][w], sel), a2, a3);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) kv8_mma(o[i][t], a0, a1, a2, a3, p[t][0], p[t][1]);
+        for (int t = 0; t < NT; ++t) kv8_mma(o[i][t], a0, a1, a2, a3, p[u][t][0], p[u][t][1]);
       }
     }
   }
@@ -666,8 +696,8 @@ extern "C" int ronn_kv8_attention(const Kv8AttnCall* call, cudaStream_t stream) 
   } while (0)
 #define RONN_KV8W(T, D, C, NT, W) \
   do { \
-    constexpr int st = D == 64 ? 4 : 3, smem = KV8_NW * st * 32 * D; \
-    auto* kern = kv8_attention_kernel<T, D, C, NT, W, st>; \
+    constexpr int u = D == 64 ? 2 : 1, st = D == 64 ? 6 : 3, smem = KV8_NW * st * 32 * D; \
+    auto* kern = kv8_attention_kernel<T, D, C, NT, W, u, st>; \
     static bool seen[MAX_DEVICES] = {false}; \
     if (first_use_on_device(seen) && \
         (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess || \
