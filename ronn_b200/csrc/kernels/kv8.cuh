@@ -36,11 +36,9 @@ __device__ __forceinline__ float kv8_least_scale(uint32_t amax) {
   return __uint_as_float(uint32_t(e + 127) << 23);
 }
 
-// 1 / s for a scale made above (a power of two between 2^-100 and 2^122); 0 for 0 (a block never written) and for NaN.
-__device__ __forceinline__ float kv8_inverse(float s) {
-  const uint32_t ex = __float_as_uint(s) >> 23;
-  return ex == 0 || ex >= 254 ? 0.f : __uint_as_float((254u - ex) << 23);
-}
+// 1 / s, exact for a scale made above; 0 for 0 (a block never written) and for NaN.  Scales that another quantiser left in a
+// cache need not be powers of two.
+__device__ __forceinline__ float kv8_inverse(float s) { return s > 0.f && s < 8.5e37f ? __frcp_rn(s) : 0.f; }
 
 // Four values (already divided by the scale) to four codes, round to nearest even.
 template <int CODE>

@@ -159,10 +159,12 @@ kv8_read_kernel(const uint8_t* __restrict__ kcodes, const uint8_t* __restrict__ 
   }
 }
 
-// The pages of n_seq contexts as values in order, for the tensor-core attention: [seq][nb][kv_heads][16][D] of K and of V, the
-// table that says so, and the sequences' lengths, checked.  One warp for each (block, head, K or V).  A value is exact in
-// bf16; in fp16 it is kept within the type's range.  Slots behind the context are zeros.  A poisoned block has NaN keys and
-// zero values, so that only those who see it read NaN.  Sequences without keys get their zeros here.
+// The pages of n_seq contexts as values in order, for the tensor-core attention: [seq][nb][kv_heads][16][D] of K and of V and the
+// table that says so.  One warp for each (block, head, K or V).  A value is exact in bf16; in fp16 it is kept within the type's
+// range.  Slots behind the context are zeros.  A poisoned block has NaN keys and zero values, so that only those who see it
+// read NaN.  Sequences without keys get their zeros here.
+// The lengths it goes by were checked by the kernel before it: the attention that follows reads them before it waits for this
+// kernel, which therefore lets it start only once they are in memory.
 struct Kv8ExpandArgs {
   const uint8_t *kcodes, *vcodes;
   const float *kscale, *vscale;
@@ -171,25 +173,29 @@ struct Kv8ExpandArgs {
   int *table, *start_out, *q_out, *kv_out;
   uint32_t* status;
   long table_ld, num_blocks, rows, ld_o;
-  int table_rows, max_blocks, nb, kv_heads, heads, max_q;
+  int n_seq, table_rows, max_blocks, nb, kv_heads, heads, max_q;
 };
+
+// The sequences' places and lengths, checked: one that passes a bound has no queries and no keys, and is reported.
+__global__ void __launch_bounds__(256) kv8_lengths_kernel(Kv8ExpandArgs a) {
+  pdl_wait();
+  for (int seq = blockIdx.x * 256 + threadIdx.x; seq < a.n_seq; seq += gridDim.x * 256) {
+    const int n = a.q_len[seq], len = a.kv_len[seq], table = a.bt_row ? a.bt_row[seq] : seq;
+    const long row0 = a.seq_start[seq];
+    const bool ok = row0 >= 0 && n >= 0 && n <= a.max_q && row0 + n <= a.rows && len <= a.nb * KV8_BLOCK && len <= a.max_blocks * KV8_BLOCK &&
+                    table >= 0 && table < a.table_rows;
+    if (!ok) kv8_report(a.status);
+    a.start_out[seq] = ok ? int(row0) : 0, a.q_out[seq] = ok ? n : 0, a.kv_out[seq] = ok && len > 0 ? len : 0;
+  }
+}
 
 template <class T, int D, int CODE>
 __global__ void __launch_bounds__(256) kv8_expand_kernel(Kv8ExpandArgs a) {
   pdl_wait();
   pdl_trigger();
   const int seq = blockIdx.y, lane = threadIdx.x & 31, unit = blockIdx.x * 8 + (threadIdx.x >> 5);
-  int n = a.q_len[seq], len = a.kv_len[seq];
-  const long row0 = a.seq_start[seq];
-  const int table = a.bt_row ? a.bt_row[seq] : seq;
-  const bool ok = row0 >= 0 && n >= 0 && n <= a.max_q && row0 + n <= a.rows && len <= a.nb * KV8_BLOCK && len <= a.max_blocks * KV8_BLOCK &&
-                  table >= 0 && table < a.table_rows;
-  if (!ok) n = 0, len = 0;
-  if (len < 0) len = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    if (!ok) kv8_report(a.status);
-    a.start_out[seq] = ok ? int(row0) : 0, a.q_out[seq] = n, a.kv_out[seq] = len;
-  }
+  const int n = a.q_out[seq], len = a.kv_out[seq];
+  const long row0 = a.start_out[seq];
   if (len == 0) {
     const int width = a.heads * (D / 8);
     for (long i = long(blockIdx.x) * 256 + threadIdx.x; i < long(n) * width; i += long(gridDim.x) * 256)
@@ -202,7 +208,7 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(Kv8ExpandArgs a) {
   const int h = is_v ? rest - a.kv_heads : rest;
   const int to = seq * a.nb + b;
   if (rest == 0 && lane == 0) a.table[to] = to;
-  const int page = a.tables[long(table) * a.table_ld + b];
+  const int page = a.tables[long(a.bt_row ? a.bt_row[seq] : seq) * a.table_ld + b];
   const bool there = page >= 0 && page < a.num_blocks;
   if (!there && lane == 0) kv8_report(a.status);
   const long src = long(there ? page : 0) * a.kv_heads + h;
@@ -382,7 +388,8 @@ extern "C" int ronn_kv8_chunk_attention(const Kv8AttnCall* c, cudaStream_t strea
     Kv8ExpandArgs a{static_cast<const uint8_t*>(c->kcodes), static_cast<const uint8_t*>(c->vcodes), c->kscale, c->vscale,
                     c->bt_row ? c->tables : c->tables + s0 * c->table_ld, c->bt_row ? c->bt_row + s0 : nullptr, c->seq_start + s0, c->q_len + s0,
                     c->kv_len + s0, k, k + elems, c->out, table, start, ql, kl, c->status, c->table_ld, c->num_blocks, c->rows, c->ld_o,
-                    c->bt_row ? c->table_rows : c->table_rows - s0, c->max_blocks, nb, c->kv_heads, c->heads, c->max_q_len};
+                    n, c->bt_row ? c->table_rows : c->table_rows - s0, c->max_blocks, nb, c->kv_heads, c->heads, c->max_q_len};
+    launch(kv8_lengths_kernel, dim3(unsigned(n < 4096 ? (n + 255) / 256 : 16)), dim3(256), 0, stream, a);
     const long units = 2L * nb * c->kv_heads;
     const dim3 grid{unsigned((units + 7) / 8), unsigned(n), 1u};
 #define RONN_KV8X(T, D, C) launch(kv8_expand_kernel<T, D, C>, grid, dim3(256), 0, stream, a)

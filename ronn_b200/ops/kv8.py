@@ -59,7 +59,8 @@ class KV8Cache:
         self.code = _CODES[k.dtype]
         self._index = k.get_device()                        # -1 on the host
         self._pointers = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
-        self._status = None
+        # made here, not in a call: a call may be the first of a graph's capture, whose memory goes with the graph
+        self._status = status_word(k.device).data_ptr() if self._index >= 0 else 0
 
     @classmethod
     def alloc(cls, num_blocks: int, kv_heads: int, head_dim: int, precision: str = "int8", device="cuda") -> "KV8Cache":
@@ -87,8 +88,6 @@ def _launch(cache: KV8Cache, fn) -> None:
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return _launch(cache, fn)
-    if cache._status is None:
-        cache._status = status_word(cache.device).data_ptr()
     fn(_native.cuda(), cache._status, _raw_stream(index))
 
 
@@ -171,7 +170,8 @@ def kv8_append(qkv: torch.Tensor, k_off: int, v_off: int, slots: torch.Tensor, c
         ld_rot = _rows16("rotated", to, k_off + kvh * d, index, qkv.dtype)
         if to.shape[0] < tokens:
             raise OperandError(f"rotated has {to.shape[0]} rows for {tokens} tokens")
-        rot, pos, turns = to.data_ptr(), _ints("positions", positions, tokens, index), _turns(d, float(rope_base))[1]
+        angles = _turns(d, float(rope_base))                 # kept while the launcher copies it
+        rot, pos, turns = to.data_ptr(), _ints("positions", positions, tokens, index), angles[1]
 
     def go(lib, status, stream):
         if _checks.enabled():
@@ -273,7 +273,8 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, 
     if append is not None:
         more = dict(k_off=k_off, v_off=v_off, slots=_ints("slots", slots, rows, index))
         if rope is not None:
-            more.update(positions=_ints("positions", rope[0], rows, index), turns=_turns(d, float(rope[1]))[1])
+            angles = _turns(d, float(rope[1]))
+            more.update(positions=_ints("positions", rope[0], rows, index), turns=angles[1])
     if max_ctx < 0:
         raise OperandError(f"max_ctx is {max_ctx}")
 

@@ -79,15 +79,16 @@ def attend(q, kvals, vvals, pages, limit, scale):
     return torch.einsum("hk,hkd->hd", p, v), torch.einsum("hk,hkd->hd", p, v.abs()), size, limit * torch.nan_to_num(v).abs().amax((1, 2))
 
 
-def bound(ref, weight, size, most, dtype, d, p_round=2.0 ** -11, p_floor=2.0 ** -40):
+def bound(ref, weight, size, most, dtype, d, p_round=2.0 ** -11, p_floor=2.0 ** -40, kv_round=0.0):
     """How far a kernel's output may be from ``attend``'s.  Rounding of the result: eps / 2 of its type.  Rounding of the
     probabilities to 16 bits (``p_round``; the sum of them is kept in 32): that fraction of sum p |v|.  The scores are sums
     of d products in 32 bits, with the factors of the scale and of log2 e: (d + 8) * 2^-23 of sum |q k| at most (accumulation
     that truncates costs a whole step), which moves p, and their sum, by that much each; exponentials and the running
     rescaling: 2^-20 of p.  A probability kept as 2^15 p in fp16 has steps of 2^-24 at its smallest, so half of that over 2^15,
     2^-40, of each |v| can be lost (``p_floor``; kept as p itself: half a step, 2^-25).  32-bit arithmetic that takes subnormals for zero loses up to 2^-126 (for |v| up to 1; in proportion above) of each
-    product, and of the result."""
+    product, and of the result.  Keys and values that are rounded on the way (``kv_round`` of each) move a score by that fraction
+    of sum |q k|, p and the sum of p by as much each, and v by its own."""
     u = torch.finfo(dtype).eps / 2
-    rel = p_round + 2 * (d + 8) * 2.0 ** -23 * size[..., None] + 2.0 ** -20
+    rel = p_round + 2 * ((d + 8) * 2.0 ** -23 + kv_round) * size[..., None] + kv_round + 2.0 ** -20
     return (u * ref.abs() + (1 + u) * rel * weight + most[..., None] * p_floor + (most[..., None] + 2) * 2.0 ** -126
             + torch.finfo(dtype).smallest_normal * u * 2)

@@ -170,7 +170,7 @@ def _pages(lens, blocks, seed):
     return table
 
 
-def _compare(out, cache, q, tables, limits, heads, scale=None, p_round=2.0 ** -11, p_floor=2.0 ** -40):
+def _compare(out, cache, q, tables, limits, heads, scale=None, p_round=2.0 ** -11, p_floor=2.0 ** -40, kv_round=0.0):
     """q [rows, heads * d]; row r sees limits[r] keys of tables[r]."""
     d = cache.head_dim
     kv, vv = Cache(cache.k, cache.k_scale).values(), Cache(cache.v, cache.v_scale).values()
@@ -179,7 +179,7 @@ def _compare(out, cache, q, tables, limits, heads, scale=None, p_round=2.0 ** -1
         ref, *about = attend(q[r].cpu().reshape(heads, d), kv, vv, tables[r].tolist(), n, sc)
         got = out[r].cpu().double().reshape(heads, d)
         assert torch.equal(torch.isnan(got), torch.isnan(ref)), r
-        off = (got - ref).abs() - bound(ref, *about, q.dtype, d, p_round, p_floor)
+        off = (got - ref).abs() - bound(ref, *about, q.dtype, d, p_round, p_floor, kv_round)
         assert not (off > 0).any(), (r, n, float(off.max()))
 
 
@@ -359,6 +359,59 @@ def test_captured_decode_steps_replay_on_new_contents():
         torch.cuda.synchronize()
         for q, o in zip(qs, outs):
             _compare(o, cache, q, table, new, heads)
+
+
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+def test_scales_that_are_no_powers_of_two(code):
+    """A cache that something else filled: read, attended to, and appended to (its scale stays where it is large enough)."""
+    ops, heads, kvh, d = _ops(), 4, 2, 64
+    lens = [70, 33]
+    cache, table = _filled(8, kvh, d, code, 101), _pages(lens, 8, 102)
+    g = torch.Generator().manual_seed(103)
+    for s in (cache.k_scale, cache.v_scale):
+        s.mul_(1 + torch.rand(8, kvh, generator=g).cuda())
+    q = _activations(2, heads * d, "bf16", 104)
+    _compare(ops.kv8_attention(q, cache, table.cuda(), _i32(lens), heads, 70), cache, q, table, lens, heads)
+    for form in ("direct", "expanded"):
+        out = ops.kv8_prefill_attention(q, 0, cache, table.cuda(), _i32([0, 1]), _i32([1, 1]), _i32(lens), 1, 70, heads, form=form)
+        # expanded to bf16, values that are no code times a power of two are rounded
+        _compare(out, cache, q, table, lens, heads, p_round=2.0 ** -8, kv_round=2.0 ** -8 if form == "expanded" else 0.0)
+    at = int(table[0, 4]) * 16 + 6
+    old = [t.clone() for t in (cache.k, cache.k_scale)]
+    x = _activations(1, 3 * kvh * d, "bf16", 105) * 1e-3
+    ops.kv8_append(x, kvh * d, 2 * kvh * d, _i32([at]), cache, kvh)
+    assert torch.equal(cache.k_scale, old[1])
+    back = cache.k.float()[at // 16, :, 6] * cache.k_scale[at // 16][:, None]
+    step = cache.k_scale[at // 16][:, None] * (0.5 if code == "int8" else 0.0)
+    want = x[0, kvh * d:2 * kvh * d].float().view(kvh, d)
+    assert bool(((back - want).abs() <= step * (1 + 2.0 ** -10) + want.abs() * (0 if code == "int8" else 2.0 ** -4) + cache.k_scale[at // 16][:, None] * 2.0 ** -9).all())
+
+
+def test_lengths_written_just_before_the_call():
+    """An expanded chunk goes by what the stream holds when it runs, captured and replayed with new lengths too."""
+    ops, heads, kvh, d = _ops(), 4, 4, 64
+    cache, table = _filled(40, kvh, d, "int8", 111), _pages([300, 300], 40, 112)
+    q, tab = _activations(64, heads * d, "bf16", 113), table.cuda()
+    start, count, keys = _i32([0, 0]), _i32([0, 0]), _i32([0, 0])
+    out = torch.zeros(64, heads * d, dtype=torch.bfloat16, device="cuda")
+    call = lambda: ops.kv8_prefill_attention(q, 0, cache, tab, start, count, keys, 40, 300, heads, out=out, form="expanded")
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for run in (call, g.replay):
+        for s, n, k in (([0, 40], [40, 24], [300, 77]), ([5, 0], [7, 2], [16, 300]), ([0, 30], [30, 0], [0, 8])):
+            fresh = [_i32(v) for v in (s, n, k)]
+            out.fill_(3.0)
+            for dst, src in zip((start, count, keys), fresh):
+                dst.copy_(src)
+            run()
+            rows = [s[i] + j for i in range(2) for j in range(n[i])]
+            limits = [max(0, k[i] - (n[i] - 1 - j)) for i in range(2) for j in range(n[i])]
+            _compare(out[rows], cache, q[rows], [table[i] for i in range(2) for _ in range(n[i])], limits, heads, p_round=2.0 ** -8)
+            assert bool((out[[r for r in range(64) if r not in set(rows)]] == 3).all())
+    ops.check_status()
 
 
 def test_cache_of_more_than_2_31_codes():
