@@ -434,3 +434,69 @@ def test_cache_of_more_than_2_31_codes():
     k, v = ops.kv8_read(cache, _i32([blocks - 1]))
     assert float((k[0, :, 0].reshape(-1).double() - q[0].double()).abs().max()) <= float(q.abs().max()) * 2.0 ** -4
     assert torch.equal(k[:, :, 0], v[:, :, 0])
+
+
+def test_calls_on_several_streams_share_a_cache():
+    """Decode steps of different sequences on different streams, append included, each behind the kernels that made its inputs."""
+    ops, heads, kvh, d = _ops(), 8, 4, 64
+    lens = [900 + 37 * i for i in range(6)]
+    blocks = sum(-(-n // 16) for n in lens) + 1
+    cache, table = _filled(blocks, kvh, d, "fp8", 121), _pages(lens, blocks, 122)
+    tab = table.cuda()
+    rows = [_activations(1, (heads + 2 * kvh) * d, "bf16", 130 + i) for i in range(6)]
+    k_off, v_off = heads * d, (heads + kvh) * d
+    twin = ops.KV8Cache(*[t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)])
+    torch.cuda.synchronize()
+    outs, streams = [], [torch.cuda.Stream() for _ in range(3)]
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 3]):
+            qkv = rows[i] * 0.5
+            slot = _i32([int(table[i, (lens[i] - 1) // 16]) * 16 + (lens[i] - 1) % 16])
+            outs.append((qkv, slot, ops.kv8_attention(qkv, cache, tab[i:i + 1], _i32([lens[i]]), heads, lens[i], append=(k_off, v_off, slot))))
+    torch.cuda.synchronize()
+    for i, (qkv, slot, out) in enumerate(outs):
+        ops.kv8_append(qkv, k_off, v_off, slot, twin, heads)
+        _compare(out, cache, qkv[:, :heads * d], table[i:i + 1], [lens[i]], heads)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in ((cache.k, twin.k), (cache.v, twin.v), (cache.k_scale, twin.k_scale),
+                                                                                  (cache.v_scale, twin.v_scale)))
+
+
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+def test_a_step_run_twice_leaves_the_same_cache(code):
+    """A captured step is run once eagerly and again by its first replay."""
+    ops, heads, kvh, d = _ops(), 2, 2, 128
+    lens = [20, 48, 33]
+    blocks = 9
+    cache, table = _filled(blocks, kvh, d, code, 141), _pages(lens, blocks, 142)
+    slots = _i32([int(table[i, (n - 1) // 16]) * 16 + (n - 1) % 16 for i, n in enumerate(lens)])
+    qkv = _activations(3, 6 * d, "fp16", 143) * 8
+    call = lambda: ops.kv8_attention(qkv, cache, table.cuda(), _i32(lens), heads, 48, append=(2 * d, 4 * d, slots), rope=(_i32([n - 1 for n in lens]), 1e4))
+    one = call()
+    state = [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    assert torch.equal(call(), one)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(state, (cache.k, cache.v, cache.k_scale, cache.v_scale)))
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0])
+def test_scales_of_the_scores(scale):
+    ops, heads, kvh, d = _ops(), 4, 2, 64
+    lens = [50, 77]
+    cache, table = _filled(9, kvh, d, "int8", 151), _pages(lens, 9, 152)
+    q = _activations(2, heads * d, "bf16", 153) * 0.1
+    _compare(ops.kv8_attention(q, cache, table.cuda(), _i32(lens), heads, 77, scale=scale), cache, q, table, lens, heads, scale)
+    for form in (None, "direct", "expanded"):                          # a scale that is not positive goes by the codes
+        out = ops.kv8_prefill_attention(q, 0, cache, table.cuda(), _i32([0, 1]), _i32([1, 1]), _i32(lens), 1, 77, heads, scale=scale, form=form)
+        _compare(out, cache, q, table, lens, heads, scale, p_round=2.0 ** -8)
+
+
+def test_rows_of_extreme_queries():
+    """Queries with infinities and NaN, zeros and subnormals spoil no other row."""
+    ops, heads, kvh, d = _ops(), 2, 2, 64
+    lens = [40] * 6
+    cache, table = _filled(20, kvh, d, "fp8", 161), _pages(lens, 20, 162)
+    q = _activations(6, heads * d, "bf16", 163) * 0.2
+    q[0, 3], q[1, 5], q[2] = math.inf, math.nan, 0
+    q[3] = 1e-39
+    out = ops.kv8_attention(q, cache, table.cuda(), _i32(lens), heads, 40)
+    assert torch.isnan(out[0, :d]).all() and torch.isnan(out[1, :d]).all() and not torch.isnan(out[:2, d:]).any() and not torch.isnan(out[2:]).any()
+    _compare(out[2:], cache, q[2:].where(q[2:].abs() > 1e-38, torch.zeros_like(q[2:])), table[2:], lens[2:], heads)

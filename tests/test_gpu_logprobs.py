@@ -178,3 +178,34 @@ def test_rows_of_a_captured_graph_follow_their_inputs():
         g.replay()
         want = ops.token_logprobs(x, t, 5)
         assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,few", [(150, 4), (1, 3), (150, 0)])
+def test_the_best_tokens_in_few_threads(dtype, rows, few):
+    """Large logits in the vectors of a few threads only (every 256th 16-byte vector), more than there is room for as
+    candidates: the alternatives come one by one."""
+    vocab, e = 262144, 4 if dtype == "fp32" else 8
+    x = torch.randn(rows, vocab // e // 256, 256, e, generator=torch.Generator().manual_seed(rows))
+    x[:, :, 3:3 + few] += 40.0
+    if few == 0:
+        x = torch.round(x)                                            # eleven values: ties across all threads
+    _check(x.reshape(rows, vocab).to(DT[dtype]).cuda(), torch.randint(0, vocab, (rows,), generator=torch.Generator().manual_seed(2)), few + 2)
+
+
+def test_streams_and_many_calls_at_once():
+    """Calls on several streams, each on inputs its own stream has just made."""
+    ops = _ops()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    results = []
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 4]):
+            g = torch.Generator(device="cuda").manual_seed(i)
+            x = torch.randn(3 + i, 40001, generator=g, device="cuda") * 3
+            t = torch.randint(0, 40001, (3 + i,), generator=g, device="cuda")
+            results.append((x, t, ops.token_logprobs(x, t, 7)))
+    torch.cuda.synchronize()
+    for x, t, r in results:
+        again = ops.token_logprobs(x, t, 7)
+        assert all(torch.equal(a, b) for a, b in zip(r, again))
+    _check(results[5][0], results[5][1].cpu(), 7)
