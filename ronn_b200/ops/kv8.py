@@ -80,15 +80,22 @@ class KV8Cache:
         return self.k.dtype
 
 
-def _launch(cache: KV8Cache, fn) -> None:
-    """``fn(library, status word, raw stream)`` on the cache's device, current or not, and that device's current stream."""
-    index = cache._index
-    if index < 0:
-        raise OperandError(f"the 8-bit cache kernels run on a CUDA device, got a cache on {cache.device}")
-    if index != torch._C._cuda_getDevice():
-        with torch.cuda.device(index):
-            return _launch(cache, fn)
-    fn(_native.cuda(), cache._status, _raw_stream(index))
+class _On:
+    """The cache's device for a call made while another is current."""
+    __slots__ = ("_ctx",)
+
+    def __init__(self, index: int):
+        if index < 0:
+            raise OperandError("the 8-bit cache kernels run on a CUDA device, got a cache on the host")
+        self._ctx = torch.cuda.device(index) if index != torch._C._cuda_getDevice() else None
+
+    def __enter__(self):
+        if self._ctx is not None:
+            self._ctx.__enter__()
+
+    def __exit__(self, *error):
+        if self._ctx is not None:
+            self._ctx.__exit__(*error)
 
 
 def _rows16(what: str, t: torch.Tensor, cols: int, index: int, dtype: Optional[torch.dtype] = None) -> int:
@@ -173,32 +180,30 @@ def kv8_append(qkv: torch.Tensor, k_off: int, v_off: int, slots: torch.Tensor, c
         angles = _turns(d, float(rope_base))                 # kept while the launcher copies it
         rot, pos, turns = to.data_ptr(), _ints("positions", positions, tokens, index), angles[1]
 
-    def go(lib, status, stream):
+    with _On(index):
         if _checks.enabled():
             _run_check(_checks.kv8_append, qkv, slots, cache.k, positions)
-        _check(lib.ronn_kv8_append(_APPEND_CALL.pack(qkv.data_ptr(), rot, slot_ptr, pos, turns, *cache._pointers, status, ld, ld_rot,
-                                                     cache.num_blocks, tokens, k_off, v_off, heads, kvh, d, _DTYPES[qkv.dtype],
-                                                     cache.code, 0), stream), "kv8_append")
-    _launch(cache, go)
+        rc = _native.cuda().ronn_kv8_append(_APPEND_CALL.pack(qkv.data_ptr(), rot, slot_ptr, pos, turns, *cache._pointers, cache._status, ld,
+                                                              ld_rot, cache.num_blocks, tokens, k_off, v_off, heads, kvh, d,
+                                                              _DTYPES[qkv.dtype], cache.code, 0), _raw_stream(index))
+    _check(rc, "kv8_append")
 
 
 def kv8_read(cache: KV8Cache, blocks: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of whole cache blocks (int32 [n]) as two [n, kv_heads, 16, head_dim] tensors."""
     if dtype not in _DTYPES:
         raise OperandError(f"kv8_read gives bf16 or fp16, not {dtype}")
-    n = blocks.numel()
-    ptr = _ints("blocks", blocks, n, cache._index)
-    out = []
-
-    def go(lib, status, stream):
+    n, index = blocks.numel(), cache._index
+    ptr = _ints("blocks", blocks, n, index)
+    with _On(index):
         if _checks.enabled():
             _run_check(_checks._in_range, "blocks", blocks, 0, cache.num_blocks, "cache blocks")
-        both = torch.empty((2, n, cache.kv_heads, _BLOCK, cache.head_dim), dtype=dtype, device=blocks.device)
-        out.extend(both.unbind(0))
-        _check(lib.ronn_kv8_read(_READ_CALL.pack(*cache._pointers, ptr, out[0].data_ptr(), out[1].data_ptr(), status, n, cache.num_blocks,
-                                                 cache.kv_heads, cache.head_dim, _DTYPES[dtype], cache.code), stream), "kv8_read")
-    _launch(cache, go)
-    return out[0], out[1]
+        shape = (n, cache.kv_heads, _BLOCK, cache.head_dim)
+        k, v = blocks.new_empty(shape, dtype=dtype), blocks.new_empty(shape, dtype=dtype)
+        rc = _native.cuda().ronn_kv8_read(_READ_CALL.pack(*cache._pointers, ptr, k.data_ptr(), v.data_ptr(), cache._status, n, cache.num_blocks,
+                                                          cache.kv_heads, cache.head_dim, _DTYPES[dtype], cache.code), _raw_stream(index))
+    _check(rc, "kv8_read")
+    return k, v
 
 
 def _out(out: Optional[torch.Tensor], q: torch.Tensor, rows: int, cols: int, index: int) -> int:
@@ -222,27 +227,26 @@ def _scale(scale: Optional[float], d: int) -> float:
 def _attention(what, cache, q, q_off, ld, tables, table, bt_row, seq_start, q_len, kv_len, out, ld_o, n_seq, max_q, max_ctx, heads, causal,
                scale, check, k_off=0, v_off=0, slots=0, positions=0, turns=0, form=None) -> torch.Tensor:
     table_ld, table_rows, width = table
-    result = [out]
-
-    def go(lib, status, stream):
+    kvh, d, index, longest = cache.kv_heads, cache.head_dim, cache._index, min(max_ctx, width * _BLOCK)
+    with _On(index):
         if _checks.enabled():
             check()
-        kvh, d, longest = cache.kv_heads, cache.head_dim, min(max_ctx, width * _BLOCK)
+        lib = _native.cuda()
         if out is None:
-            result[0] = torch.empty((q.shape[0], heads * d), dtype=q.dtype, device=q.device)
+            out = q.new_empty((q.shape[0], heads * d))
         chunked = seq_start != 0 and scale > 0 and longest > 0 and (lib.ronn_kv8_chunk_form(n_seq, max_q, longest, heads, kvh, d) if form is None
                                                                     else form == "expanded")
         need = (lib.ronn_kv8_chunk_scratch(n_seq, longest, kvh, d) if chunked else
                 lib.ronn_kv8_attention_scratch(n_seq, max_q, longest, heads, kvh, d))
         # this call's own: captured graphs and other streams share none
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        scratch = q.new_empty((need,), dtype=torch.uint8) if need else None
         call = lib.ronn_kv8_chunk_attention if chunked else lib.ronn_kv8_attention
-        _check(call(_ATTENTION_CALL.pack(
-            q.data_ptr() + 2 * q_off, *cache._pointers, tables.data_ptr(), bt_row, seq_start, q_len, kv_len, result[0].data_ptr(), slots,
-            positions, turns, scratch.data_ptr() if need else 0, status, ld, q.shape[0], cache.num_blocks, table_ld, ld_o or heads * d, need,
-            table_rows, width, n_seq, max_q, longest, heads, kvh, d, causal, _DTYPES[q.dtype], cache.code, k_off, v_off, scale), stream), what)
-    _launch(cache, go)
-    return result[0]
+        rc = call(_ATTENTION_CALL.pack(
+            q.data_ptr() + 2 * q_off, *cache._pointers, tables.data_ptr(), bt_row, seq_start, q_len, kv_len, out.data_ptr(), slots, positions,
+            turns, scratch.data_ptr() if need else 0, cache._status, ld, q.shape[0], cache.num_blocks, table_ld, ld_o or heads * d, need,
+            table_rows, width, n_seq, max_q, longest, heads, kvh, d, causal, _DTYPES[q.dtype], cache.code, k_off, v_off, scale), _raw_stream(index))
+    _check(rc, what)
+    return out
 
 
 def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, ctx_len: torch.Tensor, heads: int, max_ctx: int,

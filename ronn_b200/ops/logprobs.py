@@ -36,17 +36,16 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         raise OperandError(f"logits must have a vocabulary and unit column stride, got {tuple(logits.shape)}, strides {logits.stride()}")
     if not 0 <= int(top) <= min(MAX_TOP, vocab):
         raise OperandError(f"top is {top}; up to {min(MAX_TOP, vocab)} alternatives of {vocab} tokens")
-    dev, index = logits.device, logits.get_device()
+    index = logits.get_device()
     if tokens is not None:
         if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 1 or tokens.numel() != rows or tokens.get_device() != index:
-            raise OperandError(f"tokens must be {rows} int32 or int64 values on {dev}, got {tokens.dtype} {tuple(tokens.shape)} on "
+            raise OperandError(f"tokens must be {rows} int32 or int64 values on {logits.device}, got {tokens.dtype} {tuple(tokens.shape)} on "
                                f"{tokens.device}")
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return token_logprobs(logits, tokens, top)
     top = int(top)
-    f = torch.empty((2 + top) * rows, dtype=torch.float32, device=dev)
-    i = torch.empty((1 + top) * rows, dtype=torch.int32, device=dev)
+    f, i = logits.new_empty(((2 + top) * rows,), dtype=torch.float32), logits.new_empty(((1 + top) * rows,), dtype=torch.int32)
     logprob, entropy, tops = f.split((rows, rows, top * rows))
     rank, ids = i.split((rows, top * rows))
     at, ints = f.data_ptr(), i.data_ptr()
