@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
     return p;
   };
   auto scale_of = [&](const float* s, int p) { return p >= 0 ? s[long(p) * a.kv_heads + kvh] : 0.f; };
-  int page = page_of(lane), page1 = page_of(32 + lane), page2 = -1;
+  int page = page_of(lane), page1 = cnt > 32 ? page_of(32 + lane) : -1, page2 = -1;
   float kf = scale_of(a.kscale, page), vf = scale_of(a.vscale, page), kf1 = 0.f, vf1 = 0.f;
   uint32_t gone_of = __ballot_sync(0xffffffffu, page < 0);        // of the 32 blocks at hand
   page = max(page, 0);                          // what is loaded for a block without a page is not used
@@ -372,8 +372,10 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
         page = max(page1, 0), page1 = page2, kf = kf1, vf = vf1;
         if (vf != vf) kf = vf, vf = 0.f;
       }
-      kf1 = scale_of(a.kscale, page1), vf1 = scale_of(a.vscale, page1);
-      page2 = page_of(b + 64 + lane);
+      if (cnt > b + 32) {
+        kf1 = scale_of(a.kscale, page1), vf1 = scale_of(a.vscale, page1);
+        page2 = cnt > b + 64 ? page_of(b + 64 + lane) : -1;
+      }
       const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vf)));
       if (top > vref) {
         const float down = vref * kv8_inverse(top);          // 0 the first time
