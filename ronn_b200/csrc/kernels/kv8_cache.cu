@@ -24,14 +24,14 @@ struct Kv8AppendArgs {
   float* vscale;
   uint32_t* status;
   long ld, ld_rot, tokens, num_slots;
-  int k_off, v_off, heads, kv_heads, per_cta;
+  int k_off, v_off, heads, kv_heads, per_cta, window;
 };
 
 // Tokens of one cache block stand in consecutive rows with rising slots; such a run (1 to 16 tokens) is one unit of work
 // for each head, and a warp holds the head's part of it in registers: 16 tokens x 64 or 128 values, 16 or 32 registers.
 // The block's largest magnitude, its scale, the codes and, where the scale grew, the older codes are the warp's own
-// affair, without shared memory.  A CTA looks at the 16 rows of its window for the first rows of runs (grid.x), and at a
-// share of the heads (grid.y).
+// affair, without shared memory.  A CTA looks at the rows of its window, 16 or 1, for the first rows of runs (grid.x), and at
+// a share of the heads (grid.y).
 constexpr int KV8_AP_WARPS = 8;
 
 template <class T, int D, int CODE, bool ROPE>
@@ -46,12 +46,12 @@ kv8_append_kernel(Kv8AppendArgs a, Kv8Turns turns) {
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane / CH, chunk = lane % CH;
-  // the window's 16 rows and the 15 behind them, one per lane
-  const long w0 = long(blockIdx.x) * KV8_BLOCK;
+  // the window's rows and at least 15 behind them, one per lane
+  const long w0 = long(blockIdx.x) * a.window;
   const long row = w0 + lane;
   int slot = row < a.tokens ? max(a.slots[row], -1) : -2;      // -2: past the end
   if (slot >= a.num_slots) {
-    if (lane < KV8_BLOCK) kv8_report(a.status);
+    if (lane < a.window) kv8_report(a.status);
     slot = -1;
   }
   int before = __shfl_up_sync(0xffffffffu, slot, 1);
@@ -70,7 +70,7 @@ kv8_append_kernel(Kv8AppendArgs a, Kv8Turns turns) {
   const int u0 = blockIdx.y * a.per_cta, u1 = min(units, u0 + a.per_cta);
   const T* qkv = static_cast<const T*>(a.qkv);
 
-  for (uint32_t todo = starts & live & 0xffffu; todo; todo &= todo - 1) {
+  for (uint32_t todo = starts & live & ((1u << a.window) - 1u); todo; todo &= todo - 1) {
     const int first = __ffs(todo) - 1;
     const uint32_t later = first < 31 ? starts >> (first + 1) : 0u;
     const int n = min(later ? __ffs(later) : 32 - first, KV8_BLOCK);     // rows of the run (a block's end ends it)
@@ -278,12 +278,17 @@ extern "C" int ronn_kv8_append(const Kv8AppendCall* call, cudaStream_t stream) {
   if (positions)
     for (int j = 0; j < head_dim / 2 && j < KV8_MAX_HALF; ++j) tn.t[j] = turns[j];
   const int units = (positions ? heads : 0) + 2 * kv_heads;
-  const int per_cta = positions ? 2 * KV8_AP_WARPS : KV8_AP_WARPS;
-  const long windows = (tokens + KV8_BLOCK - 1) / KV8_BLOCK;
+  // Windows of 16 rows and, with rotary embedding, two units a warp (its table of angles serves more heads) where that gives two
+  // CTAs an SM; else of one row and one unit a warp.  16 prompts of 64 to 512 tokens: 11.5 us either way; 5 single tokens with
+  // rotary, 40 / 20 heads of 128, which 16 rows put one after the other: 18 against 9 us.
+  const long coarse = (tokens + KV8_BLOCK - 1) / KV8_BLOCK * ((units + 2 * KV8_AP_WARPS - 1) / (2 * KV8_AP_WARPS));
+  const bool few = coarse < 2L * device_sm_count();
+  const int window = few ? 1 : KV8_BLOCK, per_cta = positions && !few ? 2 * KV8_AP_WARPS : KV8_AP_WARPS;
+  const long windows = (tokens + window - 1) / window;
   const int ys = (units + per_cta - 1) / per_cta;
   if (windows > 2147483647L || ys > 65535) return -2;
   Kv8AppendArgs a{qkv, rotated, slots, positions, (uint8_t*)kcodes, (uint8_t*)vcodes, kscale, vscale, status, ld, ld_rot, tokens,
-                  num_blocks * KV8_BLOCK, k_off, v_off, heads, kv_heads, per_cta};
+                  num_blocks * KV8_BLOCK, k_off, v_off, heads, kv_heads, per_cta, window};
   const dim3 grid{unsigned(windows), unsigned(ys), 1u};
   const size_t smem = positions ? size_t(KV8_BLOCK) * (head_dim / 2) * sizeof(float4) : 0;
 #define RONN_KV8A(T, D, C) \

@@ -23,8 +23,6 @@
 
 namespace ronn {
 
-constexpr int TL_THREADS = 256;
-constexpr int TL_WARPS = TL_THREADS / 32;
 constexpr int TL_TOP = 32;
 constexpr int TL_CLUSTER = 8;
 constexpr int TL_SLACK = 8;            // threads beyond `top` that may offer candidates
@@ -224,8 +222,9 @@ __device__ __forceinline__ uint4 tl_load(const T* base, int v, int skip, int end
   return *reinterpret_cast<const uint4*>(edge);
 }
 
-template <class T>
-__global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(TlArgs a) {
+template <class T, int TL_THREADS>
+__global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_kernel(TlArgs a) {
+  constexpr int TL_WARPS = TL_THREADS / 32;
   using V = TlVec<T>;
   constexpr int E = V::E;
   __shared__ TlShare s_share[TL_CLUSTER];                                // of the first CTA: one of each CTA
@@ -554,7 +553,7 @@ __global__ void __launch_bounds__(TL_THREADS, 4) token_logprobs_kernel(TlArgs a)
 
 using namespace ronn;
 
-template <class T>
+template <class T, int TL_THREADS>
 static int launch_token_logprobs(const TlArgs& a, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(a.rows * a.cluster));
@@ -568,7 +567,7 @@ static int launch_token_logprobs(const TlArgs& a, cudaStream_t stream) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a) == cudaSuccess ? 0 : -100;
+  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, TL_THREADS>, a) == cudaSuccess ? 0 : -100;
 }
 
 // One call.  logits: [rows, ld], dtype 0 bf16, 1 fp16, 2 fp32; tokens: int32 (wide_tokens: int64) every token_stride values, or
@@ -590,8 +589,14 @@ extern "C" int ronn_token_logprobs(const TokenLogprobsCall* call, cudaStream_t s
   // alternatives took 24.6 us with 1 or 2, 31 with 4, 49 with 8 (now 22.5 with 2); 1 x 50257 took 20, 15.8, 13.8 and 13.8.
   const long vectors = vocab / (dtype == 2 ? 4 : 8);
   int cl = 1;
-  while (cl < TL_CLUSTER && rows * cl < device_sm_count() && vectors >= 2L * cl * TL_THREADS * TL_BATCH) cl *= 2;
+  while (cl < TL_CLUSTER && rows * cl < device_sm_count() && vectors >= 2L * cl * 256 * TL_BATCH) cl *= 2;
   const TlArgs a{logits, tokens, logprob, entropy, top_logprobs, rank, top_ids, ld, token_stride, rows, vocab, top, cl, wide_tokens};
-  return dtype == 0 ? launch_token_logprobs<__nv_bfloat16>(a, stream) : dtype == 1 ? launch_token_logprobs<__half>(a, stream)
-                                                                                   : launch_token_logprobs<float>(a, stream);
+  // Many short rows: CTAs of 64 threads, 16 to an SM.  Microseconds with 256 and with 64 threads, five alternatives: 4800 x 1000
+  // bf16 66 and 41, 2400 x 4728 41 and 33, 600 x 12000 22.6 and 18.4; but 4800 x 32000 124 and 127, 300 x 12000 14.3 and 18.4.
+  const bool narrow = cl == 1 && rows >= 4L * device_sm_count() && vectors <= 1500;
+#define RONN_TL(T) return narrow ? launch_token_logprobs<T, 64>(a, stream) : launch_token_logprobs<T, 256>(a, stream)
+  if (dtype == 0) RONN_TL(__nv_bfloat16);
+  if (dtype == 1) RONN_TL(__half);
+  RONN_TL(float);
+#undef RONN_TL
 }

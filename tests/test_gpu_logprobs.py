@@ -209,3 +209,15 @@ def test_streams_and_many_calls_at_once():
         again = ops.token_logprobs(x, t, 7)
         assert all(torch.equal(a, b) for a, b in zip(r, again))
     _check(results[5][0], results[5][1].cpu(), 7)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,vocab,pad", [(700, 31, 0), (601, 1000, 3), (650, 5999, 1)])
+@pytest.mark.parametrize("top", [0, 5, 31])
+def test_many_short_rows(dtype, rows, vocab, pad, top):
+    x = _logits(rows, vocab + pad, dtype, rows)[:, :vocab]
+    x[5] = 2.0
+    x[6, 1:] = -math.inf
+    x[7] = -math.inf
+    tokens = torch.randint(0, vocab, (rows,), generator=torch.Generator().manual_seed(3))
+    _check(x, tokens, top)
