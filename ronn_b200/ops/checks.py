@@ -104,9 +104,10 @@ def embedding(ids, table, positions=None, pos_table=None) -> None:
         _in_range("positions", positions, 0, pos_table.shape[0], "rows of the position table")
 
 
-def sequences(tokens: int, seq_start, q_len, kv_len, contiguous_kv: bool, table_keys: Optional[int] = None) -> None:
+def sequences(tokens: int, seq_start, q_len, kv_len, contiguous_kv: bool, table_keys: Optional[int] = None,
+              fewer_keys: bool = False) -> None:
     """Sequence index tensors of the tensor-core attention kernels: query rows inside the buffer; keys inside the
-    buffer (contiguous form) or inside a table row (paged form)."""
+    buffer (contiguous form) or inside a table row (paged form), no fewer than the queries unless ``fewer_keys``."""
     _in_range("seq_start", seq_start, 0, max(tokens, 1), "rows of the token buffer")
     _in_range("q_len", q_len, 0, tokens + 1, "rows of the token buffer")
     end = seq_start.long() + q_len.long()
@@ -121,6 +122,6 @@ def sequences(tokens: int, seq_start, q_len, kv_len, contiguous_kv: bool, table_
     else:
         _in_range("kv_len", kv_len, 0, int(table_keys) + 1, "keys a table row can list")
         short = kv_len.long() < q_len.long()
-        if bool(short.any()):
+        if bool(short.any()) and not fewer_keys:
             i, _ = _first_bad(kv_len, short)
             raise IndexCheckError(f"sequence {i}: {int(q_len[i])} queries but only {int(kv_len[i])} keys")

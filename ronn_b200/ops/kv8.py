@@ -38,7 +38,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 
 class KV8Cache:
     """Codes and scales of one layer's keys and values, or of one rank's share of them."""
-    __slots__ = ("k", "v", "k_scale", "v_scale", "num_blocks", "kv_heads", "head_dim", "code", "_index", "_pointers", "_status")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_blocks", "kv_heads", "head_dim", "code", "_index", "_status")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dtype not in _CODES or v.dtype != k.dtype:
@@ -58,7 +58,6 @@ class KV8Cache:
         self.num_blocks, self.kv_heads, _, self.head_dim = k.shape
         self.code = _CODES[k.dtype]
         self._index = k.get_device()                        # -1 on the host
-        self._pointers = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
         # made here, not in a call: a call may be the first of a graph's capture, whose memory goes with the graph
         self._status = status_word(k.device).data_ptr() if self._index >= 0 else 0
 
@@ -70,6 +69,9 @@ class KV8Cache:
         shape = (num_blocks, kv_heads, _BLOCK, head_dim)
         mk = lambda: torch.zeros(shape, dtype=torch.uint8, device=device).view(_PRECISIONS[precision])
         return cls(mk(), mk(), torch.zeros(shape[:2], device=device), torch.zeros(shape[:2], device=device))
+
+    def _pointers(self) -> Tuple[int, int, int, int]:
+        return self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
 
     @property
     def device(self) -> torch.device:
@@ -183,7 +185,7 @@ def kv8_append(qkv: torch.Tensor, k_off: int, v_off: int, slots: torch.Tensor, c
     with _On(index):
         if _checks.enabled():
             _run_check(_checks.kv8_append, qkv, slots, cache.k, positions)
-        rc = _native.cuda().ronn_kv8_append(_APPEND_CALL.pack(qkv.data_ptr(), rot, slot_ptr, pos, turns, *cache._pointers, cache._status, ld,
+        rc = _native.cuda().ronn_kv8_append(_APPEND_CALL.pack(qkv.data_ptr(), rot, slot_ptr, pos, turns, *cache._pointers(), cache._status, ld,
                                                               ld_rot, cache.num_blocks, tokens, k_off, v_off, heads, kvh, d,
                                                               _DTYPES[qkv.dtype], cache.code, 0), _raw_stream(index))
     _check(rc, "kv8_append")
@@ -200,7 +202,7 @@ def kv8_read(cache: KV8Cache, blocks: torch.Tensor, dtype: torch.dtype = torch.b
             _run_check(_checks._in_range, "blocks", blocks, 0, cache.num_blocks, "cache blocks")
         shape = (n, cache.kv_heads, _BLOCK, cache.head_dim)
         k, v = blocks.new_empty(shape, dtype=dtype), blocks.new_empty(shape, dtype=dtype)
-        rc = _native.cuda().ronn_kv8_read(_READ_CALL.pack(*cache._pointers, ptr, k.data_ptr(), v.data_ptr(), cache._status, n, cache.num_blocks,
+        rc = _native.cuda().ronn_kv8_read(_READ_CALL.pack(*cache._pointers(), ptr, k.data_ptr(), v.data_ptr(), cache._status, n, cache.num_blocks,
                                                           cache.kv_heads, cache.head_dim, _DTYPES[dtype], cache.code), _raw_stream(index))
     _check(rc, "kv8_read")
     return k, v
@@ -242,7 +244,7 @@ def _attention(what, cache, q, q_off, ld, tables, table, bt_row, seq_start, q_le
         scratch = q.new_empty((need,), dtype=torch.uint8) if need else None
         call = lib.ronn_kv8_chunk_attention if chunked else lib.ronn_kv8_attention
         rc = call(_ATTENTION_CALL.pack(
-            q.data_ptr() + 2 * q_off, *cache._pointers, tables.data_ptr(), bt_row, seq_start, q_len, kv_len, out.data_ptr(), slots, positions,
+            q.data_ptr() + 2 * q_off, *cache._pointers(), tables.data_ptr(), bt_row, seq_start, q_len, kv_len, out.data_ptr(), slots, positions,
             turns, scratch.data_ptr() if need else 0, cache._status, ld, q.shape[0], cache.num_blocks, table_ld, ld_o or heads * d, need,
             table_rows, width, n_seq, max_q, longest, heads, kvh, d, causal, _DTYPES[q.dtype], cache.code, k_off, v_off, scale), _raw_stream(index))
     _check(rc, what)
@@ -299,7 +301,8 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
     front of the first key gives zeros.  The new tokens' K and V are in the cache already.  Returns [tokens, heads * head_dim];
     rows that belong to no sequence are not written.  ``max_q_len`` bounds the queries of a sequence, ``max_kv_len`` its keys.
     Few queries read the codes as they are ("direct"); for many the contexts are expanded to 16-bit values first and the
-    tensor-core attention runs over those ("expanded", for a positive scale).  ``form`` names one, for measurements."""
+    tensor-core attention runs over those ("expanded", for a positive scale; fp16 keeps values within its range, and probabilities
+    in the activations' type).  ``form`` names one, for measurements."""
     d, index = cache.head_dim, cache._index
     _heads(heads, cache)
     _offset("q_off", q_off)
@@ -314,7 +317,7 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
         raise OperandError(f"max_q_len is {max_q_len}, max_kv_len {max_kv_len}")
 
     def check():
-        _run_check(_checks.sequences, tokens, seq_start, q_len, kv_len, False, block_tables.shape[1] * _BLOCK)
+        _run_check(_checks.sequences, tokens, seq_start, q_len, kv_len, False, block_tables.shape[1] * _BLOCK, True)
         rows_of = bt_row if bt_row is not None else torch.arange(n_seq, device=q.device, dtype=torch.int32)
         _run_check(_checks.paged_attention, kv_len[:n_seq, None], cache.k, block_tables, kv_len, 0, 0, block_tables.shape[1] * _BLOCK, rows_of)
     return _attention("kv8_prefill_attention", cache, q, q_off, ld, block_tables, table, at, start, count, keys, out,

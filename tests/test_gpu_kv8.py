@@ -130,7 +130,8 @@ def test_append_extremes(dtype, code):
     assert not math.isnan(float(cache.k_scale[3, 0]))
 
 
-def test_slots_outside_the_cache_are_skipped_and_reported():
+def test_slots_outside_the_cache_are_skipped_and_reported(monkeypatch):
+    monkeypatch.delenv("RONN_KERNEL_CHECKS", raising=False)          # the host's checks would refuse it first
     ops, d = _ops(), 64
     cache = _filled(2, 1, d, "int8", 1)
     kept = [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
@@ -297,7 +298,8 @@ def test_a_poisoned_block_is_seen_by_those_who_see_it(code, tensor, n, form):
         assert bool(nan[j, 2:].all()) == sees[j] and bool(nan[j, 2:].any()) == sees[j] and not nan[j, :2].any()
 
 
-def test_pages_outside_the_cache_are_left_out_and_reported():
+def test_pages_outside_the_cache_are_left_out_and_reported(monkeypatch):
+    monkeypatch.delenv("RONN_KERNEL_CHECKS", raising=False)          # the host's checks would refuse it first
     ops, d = _ops(), 64
     cache = _filled(4, 2, d, "int8", 61)
     table = torch.tensor([[0, 9, 1], [2, 3, -1]], dtype=torch.int32)
@@ -308,8 +310,9 @@ def test_pages_outside_the_cache_are_left_out_and_reported():
         ops.check_status()
 
 
-def test_expanded_chunks_in_groups_and_bounds_that_do_not_hold():
+def test_expanded_chunks_in_groups_and_bounds_that_do_not_hold(monkeypatch):
     """More contexts than are expanded at a time; sequences that pass the bounds or the buffer are left out and reported."""
+    monkeypatch.delenv("RONN_KERNEL_CHECKS", raising=False)          # the host's checks would refuse it first
     ops, heads, kvh, d = _ops(), 8, 8, 128
     keys, n_seq = 16000, 5                                            # 65 MiB of values a sequence: 3 at a time
     blocks = keys // 16
@@ -500,3 +503,23 @@ def test_rows_of_extreme_queries():
     out = ops.kv8_attention(q, cache, table.cuda(), _i32(lens), heads, 40)
     assert torch.isnan(out[0, :d]).all() and torch.isnan(out[1, :d]).all() and not torch.isnan(out[:2, d:]).any() and not torch.isnan(out[2:]).any()
     _compare(out[2:], cache, q[2:].where(q[2:].abs() > 1e-38, torch.zeros_like(q[2:])), table[2:], lens[2:], heads)
+
+
+def test_a_chunk_with_fewer_keys_than_queries_passes_the_index_checks(monkeypatch):
+    """Queries in front of the first key give zeros, with the host's index checks on as without them."""
+    monkeypatch.setenv("RONN_KERNEL_CHECKS", "1")
+    ops, d = _ops(), 64
+    cache = _filled(2, 1, d, "int8", 91)
+    out = ops.kv8_prefill_attention(_activations(5, d, "fp16", 92), 0, cache, _i32([[0, 1]]), _i32([0]), _i32([5]), _i32([3]), 5, 3, 1)
+    assert (out[:2] == 0).all() and (out[2:] != 0).any(1).all()
+
+
+def test_a_cache_whose_storage_moved():
+    """A cache's calls take its tensors where they are at the call: one set to another storage is read there."""
+    ops, d = _ops(), 64
+    cache, other = _filled(3, 1, d, "int8", 93), _filled(3, 1, d, "int8", 94)
+    want = ops.kv8_read(other, _i32([2, 0]))
+    for name in ("k", "v", "k_scale", "v_scale"):
+        getattr(cache, name).set_(getattr(other, name))
+    got = ops.kv8_read(cache, _i32([2, 0]))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -115,3 +115,12 @@ def test_reference_rounds_older_codes_again_when_a_larger_token_joins():
     assert c.scale[0, 0] == 1 and c.codes[0, 0, 0].tolist() == [1, 127]
     c.append(torch.tensor([[[254.0, 3.0]]]), [1])
     assert c.scale[0, 0] == 2 and c.codes[0, 0, :2].tolist() == [[0, 64], [127, 2]]      # 1/2 and 3/2 round to even
+
+
+def test_chunk_checks_allow_fewer_keys_than_queries():
+    start, count, keys = _i32([0, 4]), _i32([4, 3]), _i32([2, 32])
+    C.sequences(7, start, count, keys, False, 32, True)
+    with pytest.raises(C.IndexCheckError, match="4 queries but only 2 keys"):
+        C.sequences(7, start, count, keys, False, 32)
+    with pytest.raises(C.IndexCheckError, match="kv_len"):
+        C.sequences(7, start, count, _i32([2, 33]), False, 32, True)
