@@ -3,7 +3,8 @@
 //   ronn_kv8_attention : query rows grouped by sequence.  Sequence s has q_len[s] queries from row seq_start[s] on (without
 //                        these two: row s, one query) and attends to the kv_len[s] keys its block-table row lists; with
 //                        `causal` its queries are the last positions of that context.  Queries without keys give zeros.
-//                        With append slots (one query per sequence) the row's new K and V join the cache first.
+//                        With append slots (one query per sequence, up to 16 heads to a KV head) the row's new K and V join
+//                        the cache first.
 //
 // Bound by memory: every code is read once for all the queries that share it.  A warp takes cache blocks of 16 tokens one
 // after the other, by asynchronous 16-byte copies into a ring of its own in shared memory and from there into the fragments
@@ -673,6 +674,7 @@ extern "C" int ronn_kv8_attention(const Kv8AttnCall* call, cudaStream_t stream) 
   if ((seq_start == nullptr) != (q_len == nullptr)) return -2;
   if ((slots || positions) && seq_start) return -2;
   if (positions && (!turns || !slots)) return -2;
+  if (slots && heads / kv_heads > 16) return -2;               // several tiles would append the same token
   if (head_dim != 64 && head_dim != 128) return -1;
   const long group_rows = long(max_q_len) * (heads / kv_heads), mtiles = (group_rows + 15) / 16, xs = long(n_seq) * kv_heads;
   if (xs > 2147483647L || mtiles > 65535 || xs * mtiles * 16 > 2147483647L) return -2;

@@ -25,6 +25,7 @@ from .kernels import OperandError, _check, _run_check, status_word
 _CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _PRECISIONS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 _BLOCK = 16
+_TILE = 16                                   # query rows of an attention tile
 
 
 # the launchers' call records (kv8_attention.cu, kv8_cache.cu), packed: a decode step is made of calls of a few microseconds, and
@@ -255,11 +256,12 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, 
                   bt_row: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                   append=None, rope=None) -> torch.Tensor:
     """Attention of single rows: row r of q ([rows, ld], head h at column h * head_dim) attends to the first ``ctx_len[r]`` keys
-    that row ``bt_row[r]`` (default r) of the block tables lists.  Returns [rows, heads * head_dim]; a row with no keys gives
-    zeros.  ``max_ctx``, the longest context, sizes the launch.
+    that row ``bt_row[r]`` (default r) of the block tables lists.  Returns [rows, heads * head_dim], in ``out`` if given
+    (which must not overlap q); a row with no keys gives zeros.  ``max_ctx``, the longest context, sizes the launch.
     ``append=(k_off, v_off, slots)`` (decode, one row per sequence): q is the fused QKV activation, and each row's new K and V
     first join the cache at the row's slot, which is that of key ``ctx_len[r] - 1``.  ``rope=(positions, base)`` with
-    ``append``: q and the new k are rotated (q in memory stays as it is)."""
+    ``append``: q and the new k are rotated (q in memory stays as it is).  Where more than 16 heads share a cached head, the
+    append is a launch of its own."""
     d, index = cache.head_dim, cache._index
     _heads(heads, cache)
     more = {}
@@ -283,6 +285,12 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, 
             more.update(positions=_ints("positions", rope[0], rows, index), turns=angles[1])
     if max_ctx < 0:
         raise OperandError(f"max_ctx is {max_ctx}")
+    if append is not None and heads // cache.kv_heads > _TILE:           # several tiles of a head's rows: one append before them
+        factor = _scale(scale, d)
+        _out(out, q, rows, heads * d, index)
+        turned = None if rope is None else q.new_empty((rows, k_off + cache.kv_heads * d))
+        kv8_append(q, k_off, v_off, slots, cache, heads, *((rope[0], float(rope[1]), turned) if rope is not None else ()))
+        return kv8_attention(q if rope is None else turned, cache, block_tables, ctx_len, heads, max_ctx, bt_row, out, factor)
 
     def check():
         _run_check(_checks.paged_attention, q, cache.k, block_tables, ctx_len, heads, d, int(max_ctx), bt_row,

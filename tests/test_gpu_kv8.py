@@ -523,3 +523,32 @@ def test_a_cache_whose_storage_moved():
         getattr(cache, name).set_(getattr(other, name))
     got = ops.kv8_read(cache, _i32([2, 0]))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+@pytest.mark.parametrize("heads,kvh,d", [(17, 1, 64), (48, 2, 128), (40, 1, 64)])
+@pytest.mark.parametrize("rope", [0.0, 10000.0])
+@pytest.mark.parametrize("given", [False, True])
+def test_decode_step_appends_once_for_heads_of_several_tiles(code, heads, kvh, d, rope, given):
+    """More query heads to a cached head than a tile holds: the new token joins its block once, whose scale it makes grow."""
+    ops = _ops()
+    lens = [2, 16, 18, 333, 0, 700]
+    blocks = sum(-(-n // 16) for n in lens) + 1
+    cache, table = _filled(blocks, kvh, d, code, 95), _pages(lens, blocks, 96)
+    slots = [int(table[i, (n - 1) // 16]) * 16 + (n - 1) % 16 if n else -1 for i, n in enumerate(lens)]
+    positions = [max(n - 1, 0) for n in lens]
+    k_off, v_off = heads * d, (heads + kvh) * d
+    qkv = _activations(len(lens), (heads + 2 * kvh) * d, "bf16", 97)
+    qkv[:, k_off:] *= 16                                              # larger than what most blocks hold
+    kept = qkv.clone()
+    twin = ops.KV8Cache(*[t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)])
+    before = cache.k_scale.clone()
+    out = torch.empty(len(lens), heads * d, dtype=torch.bfloat16, device="cuda") if given else None
+    got = ops.kv8_attention(qkv, cache, table.cuda(), _i32(lens), heads, 700, append=(k_off, v_off, _i32(slots)), out=out,
+                            rope=(_i32(positions), rope) if rope else None)
+    assert torch.equal(qkv, kept) and (out is None or got is out) and (cache.k_scale > before).any()
+    ops.kv8_append(qkv, k_off, v_off, _i32(slots), twin, heads, _i32(positions) if rope else None, rope)
+    for mine, theirs in ((cache.k, twin.k), (cache.v, twin.v), (cache.k_scale, twin.k_scale), (cache.v_scale, twin.v_scale)):
+        assert torch.equal(mine.view(torch.uint8), theirs.view(torch.uint8))
+    _compare(got, cache, qkv[:, :heads * d], table, lens, heads)
+    ops.check_status()
