@@ -177,6 +177,8 @@ def kv8_append(qkv: torch.Tensor, k_off: int, v_off: int, slots: torch.Tensor, c
         if k_off < heads * d:
             raise OperandError(f"k_off {k_off} lies inside the {heads} heads of q")
         to = qkv if rotated is None else rotated
+        if to.data_ptr() == qkv.data_ptr() and (v_off < heads * d or abs(v_off - k_off) < kvh * d):
+            raise OperandError(f"v_off {v_off} lies inside the columns that are rotated in place")
         ld_rot = _rows16("rotated", to, k_off + kvh * d, index, qkv.dtype)
         if to.shape[0] < tokens:
             raise OperandError(f"rotated has {to.shape[0]} rows for {tokens} tokens")

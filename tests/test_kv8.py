@@ -124,3 +124,14 @@ def test_chunk_checks_allow_fewer_keys_than_queries():
         C.sequences(7, start, count, keys, False, 32)
     with pytest.raises(C.IndexCheckError, match="kv_len"):
         C.sequences(7, start, count, _i32([2, 33]), False, 32, True)
+
+
+def test_columns_that_are_both_rotated_in_place_and_stored_are_refused():
+    c, qkv, slots = _cache(), _q(), _i32([0, 1, 2])
+    for v_off in (0, 3 * 64, 4 * 64, 5 * 64):
+        with pytest.raises(ops.OperandError, match="rotated in place"):
+            ops.kv8_append(qkv, 4 * 64, v_off, slots, c, 4, slots, 1e4)
+        with pytest.raises(ops.OperandError, match="CUDA device"):
+            ops.kv8_append(qkv, 4 * 64, v_off, slots, c, 4, slots, 1e4, _q())
+        with pytest.raises(ops.OperandError, match="CUDA device"):
+            ops.kv8_append(qkv, 4 * 64, v_off, slots, c, 4)
