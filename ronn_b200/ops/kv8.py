@@ -131,8 +131,8 @@ def _table(t: torch.Tensor, rows: int, index: int) -> Tuple[int, int, int]:
     (n, width), (ld, unit) = t.shape, t.stride()
     if n <= 1:
         ld = max(ld, width)
-    if width < 1 or (unit != 1 and width > 1) or ld < width:
-        raise OperandError(f"block_tables must have columns, in unit stride, and rows that do not overlap, got {tuple(t.shape)}, strides {t.stride()}")
+    if not 1 <= width <= 1 << 26 or (unit != 1 and width > 1) or ld < width:
+        raise OperandError(f"block_tables must have columns (up to 2^26), in unit stride, and rows that do not overlap, got {tuple(t.shape)}, strides {t.stride()}")
     if n < rows:
         raise OperandError(f"block_tables has {n} rows for {rows}")
     return ld, n, width
@@ -331,5 +331,5 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
         rows_of = bt_row if bt_row is not None else torch.arange(n_seq, device=q.device, dtype=torch.int32)
         _run_check(_checks.paged_attention, kv_len[:n_seq, None], cache.k, block_tables, kv_len, 0, 0, block_tables.shape[1] * _BLOCK, rows_of)
     return _attention("kv8_prefill_attention", cache, q, q_off, ld, block_tables, table, at, start, count, keys, out,
-                      _out(out, q, tokens, heads * d, index), n_seq, int(max_q_len), int(max_kv_len), heads, 1 if causal else 0,
+                      _out(out, q, tokens, heads * d, index), n_seq, min(int(max_q_len), tokens), int(max_kv_len), heads, 1 if causal else 0,
                       _scale(scale, d), check, form=form)

@@ -552,3 +552,11 @@ def test_decode_step_appends_once_for_heads_of_several_tiles(code, heads, kvh, d
         assert torch.equal(mine.view(torch.uint8), theirs.view(torch.uint8))
     _compare(got, cache, qkv[:, :heads * d], table, lens, heads)
     ops.check_status()
+
+
+def test_a_loose_bound_of_queries_changes_nothing():
+    ops, heads, d = _ops(), 4, 64
+    cache = _filled(4, 2, d, "int8", 98)
+    args = (_activations(7, heads * d, "bf16", 99), 0, cache, _i32([[0, 1], [2, 3]]), _i32([0, 3]), _i32([3, 4]), _i32([20, 32]))
+    for form in ("direct", "expanded"):
+        assert torch.equal(ops.kv8_prefill_attention(*args, 4, 32, heads, form=form), ops.kv8_prefill_attention(*args, 2 ** 40, 32, heads, form=form))

@@ -135,3 +135,9 @@ def test_columns_that_are_both_rotated_in_place_and_stored_are_refused():
             ops.kv8_append(qkv, 4 * 64, v_off, slots, c, 4, slots, 1e4, _q())
         with pytest.raises(ops.OperandError, match="CUDA device"):
             ops.kv8_append(qkv, 4 * 64, v_off, slots, c, 4)
+
+
+def test_tables_whose_keys_pass_32_bits_are_refused():
+    wide = torch.empty(1, 2 ** 26 + 1, dtype=torch.int32)
+    with pytest.raises(ops.OperandError, match="2\\^26"):
+        ops.kv8_attention(_q(1), _cache(), wide, _i32([1]), 4, 16)
