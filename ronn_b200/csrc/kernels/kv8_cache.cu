@@ -3,15 +3,12 @@
 //   ronn_kv8_append : the K and V columns of a fused QKV activation into their cache slots, optionally after rotary
 //                     embedding of Q and K.
 //   ronn_kv8_read   : whole cache blocks as 16-bit values.
-//   ronn_kv8_chunk_attention : attention of long query chunks: the contexts' pages as 16-bit values in scratch, then the
-//                     tensor-core attention over them.
 //
 // Both are bound by memory: append reads 2 bytes and writes 1 for every value (with rotary embedding it also reads and
 // writes Q and writes K), read reads 1 and writes 2.  4384 tokens of 16 heads of 64 go in at 6.8 us, 3.9 TB/s; with rotary
 // embedding 2000 tokens of 32 / 8 heads of 128 take 22 us: the pairs of floats of a rotated value, 17 operations, fill 68 % of
 // the issue slots.
 #include "kv8.cuh"
-#include <type_traits>
 
 namespace ronn {
 
@@ -161,98 +158,9 @@ kv8_read_kernel(const uint8_t* __restrict__ kcodes, const uint8_t* __restrict__ 
   }
 }
 
-// The pages of n_seq contexts as values in order, for the tensor-core attention: [seq][nb][kv_heads][16][D] of K and of V and the
-// table that says so.  One warp for each (block, head, K or V).  A value is exact in bf16; in fp16 it is kept within the type's
-// range.  Slots behind the context are zeros.  A poisoned block has NaN keys and zero values, so that only those who see it
-// read NaN.  Sequences without keys get their zeros here.
-// The lengths it goes by were checked by the kernel before it: the attention that follows reads them before it waits for this
-// kernel, which therefore lets it start only once they are in memory.
-struct Kv8ExpandArgs {
-  const uint8_t *kcodes, *vcodes;
-  const float *kscale, *vscale;
-  const int *tables, *bt_row, *seq_start, *q_len, *kv_len;
-  void *k, *v, *out;
-  int *table, *start_out, *q_out, *kv_out;
-  uint32_t* status;
-  long table_ld, num_blocks, rows, ld_o;
-  int n_seq, table_rows, max_blocks, nb, kv_heads, heads, max_q;
-};
-
-// The sequences' places and lengths, checked: one that passes a bound has no queries and no keys, and is reported.
-__global__ void __launch_bounds__(256) kv8_lengths_kernel(Kv8ExpandArgs a) {
-  pdl_wait();
-  for (int seq = blockIdx.x * 256 + threadIdx.x; seq < a.n_seq; seq += gridDim.x * 256) {
-    const int n = a.q_len[seq], len = a.kv_len[seq], table = a.bt_row ? a.bt_row[seq] : seq;
-    const long row0 = a.seq_start[seq];
-    const bool ok = row0 >= 0 && n >= 0 && n <= a.max_q && row0 + n <= a.rows && len <= a.nb * KV8_BLOCK && len <= a.max_blocks * KV8_BLOCK &&
-                    table >= 0 && table < a.table_rows;
-    if (!ok) kv8_report(a.status);
-    a.start_out[seq] = ok ? int(row0) : 0, a.q_out[seq] = ok ? n : 0, a.kv_out[seq] = ok && len > 0 ? len : 0;
-  }
-}
-
-template <class T, int D, int CODE>
-__global__ void __launch_bounds__(256) kv8_expand_kernel(Kv8ExpandArgs a) {
-  pdl_wait();
-  pdl_trigger();
-  const int seq = blockIdx.y, lane = threadIdx.x & 31, unit = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int n = a.q_out[seq], len = a.kv_out[seq];
-  const long row0 = a.start_out[seq];
-  if (len == 0) {
-    const int width = a.heads * (D / 8);
-    for (long i = long(blockIdx.x) * 256 + threadIdx.x; i < long(n) * width; i += long(gridDim.x) * 256)
-      *reinterpret_cast<Vec8*>(static_cast<T*>(a.out) + (row0 + i / width) * a.ld_o + (i % width) * 8) = Vec8{{0u, 0u, 0u, 0u}};
-    return;
-  }
-  const int per = 2 * a.kv_heads, b = unit / per, rest = unit - b * per;
-  if (b * KV8_BLOCK >= len) return;
-  const bool is_v = rest >= a.kv_heads;
-  const int h = is_v ? rest - a.kv_heads : rest;
-  const int to = seq * a.nb + b;
-  if (rest == 0 && lane == 0) a.table[to] = to;
-  const int page = a.tables[long(a.bt_row ? a.bt_row[seq] : seq) * a.table_ld + b];
-  const bool there = page >= 0 && page < a.num_blocks;
-  if (!there && lane == 0) kv8_report(a.status);
-  const long src = long(there ? page : 0) * a.kv_heads + h;
-  const float ks = there ? a.kscale[src] : 0.f, vs = there ? a.vscale[src] : 0.f;
-  const bool poisoned = ks != ks || vs != vs;
-  const float s = is_v ? (poisoned ? 0.f : vs) : (poisoned ? __uint_as_float(0x7fc00000u) : ks);
-  const uint4* codes = reinterpret_cast<const uint4*>((is_v ? a.vcodes : a.kcodes) + src * (KV8_BLOCK * D));
-  T* out = static_cast<T*>(is_v ? a.v : a.k) + (long(to) * a.kv_heads + h) * (KV8_BLOCK * D);
-  constexpr int PASSES = KV8_BLOCK * D / 512;
-  constexpr float MOST = std::is_same<T, __half>::value ? 65504.f : 3.3e38f;
-#pragma unroll
-  for (int p = 0; p < PASSES; ++p) {
-    const int at = (p * 32 + lane) * 16;                    // 16 channels of one token
-    const bool live = there && b * KV8_BLOCK + at / D < len;
-    uint4 c = codes[p * 32 + lane];
-    if (!live) c = make_uint4(0u, 0u, 0u, 0u);
-    const float sc = live ? s : 0.f;
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float f[8], g[4];
-      kv8_unpack4<CODE>(w[2 * k], g);
-      f[0] = g[0] * sc, f[1] = g[1] * sc, f[2] = g[2] * sc, f[3] = g[3] * sc;
-      kv8_unpack4<CODE>(w[2 * k + 1], g);
-      f[4] = g[0] * sc, f[5] = g[1] * sc, f[6] = g[2] * sc, f[7] = g[3] * sc;
-      if (!poisoned) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = fminf(fmaxf(f[j], -MOST), MOST);
-      }
-      *reinterpret_cast<Vec8*>(out + at + k * 8) = pack8<T>(f);
-    }
-  }
-}
-
 }  // namespace ronn
 
 using namespace ronn;
-
-extern "C" int ronn_fmha_paged(const void* q, long ld_q, long total_rows, int q_off, const void* kcache, const void* vcache,
-                               long n_blocks, const int* block_tables, int max_blocks, const int* bt_row, const int* seq_start,
-                               const int* q_len, const int* kv_len, void* out, long ld_o, int n_seq, int max_q_len, int heads,
-                               int kv_heads, int head_dim, int causal, float scale, int dtype, uint32_t* status, cudaStream_t stream);
 
 static int launch_status() { return cudaGetLastError() == cudaSuccess ? 0 : -100; }
 
@@ -346,78 +254,4 @@ extern "C" int ronn_kv8_read(const Kv8ReadCall* call, cudaStream_t stream) {
 #undef RONN_KV8R
 #undef RONN_KV8R_
   return launch_status();
-}
-
-// Sequences that ronn_kv8_chunk_attention expands at a time: what fits 256 MiB, one at least.
-static int kv8_chunk_group(int n_seq, int max_kv, int kv_heads, int head_dim) {
-  const long per = 2L * ((max_kv + KV8_BLOCK - 1) / KV8_BLOCK) * kv_heads * KV8_BLOCK * head_dim * 2;
-  const long g = per > 0 ? (256L << 20) / per : n_seq;
-  return int(g < 1 ? 1 : g > n_seq ? n_seq : g > 32768 ? 32768 : g);
-}
-extern "C" long ronn_kv8_chunk_scratch(int n_seq, int max_kv, int kv_heads, int head_dim) {
-  if (n_seq <= 0 || max_kv <= 0) return 0;
-  const long g = kv8_chunk_group(n_seq, max_kv, kv_heads, head_dim), nb = (max_kv + KV8_BLOCK - 1) / KV8_BLOCK;
-  const long ints = (g * (nb + 3) * 4 + 255) / 256 * 256;
-  return ints + 2 * g * nb * kv_heads * KV8_BLOCK * head_dim * 2;
-}
-
-// Whether chunks of these sizes are faster that way (1) or straight from the codes (0), by what both cost in microseconds.
-// Expanded: a chain of 128-key tiles for each 128 queries and head, 2.4 us a tile (2.2 for heads of 128) while the SMs have
-// one such CTA each, and the values.  Direct: 0.4 ns (0.55) for each 16 query rows and 16 keys.  Over 252 sizes (1 to 16
-// sequences, contexts of 300 to 4000, 16 to 256 queries, four head layouts) the rule costs 0.3 % (1.0 %) against the faster
-// form of each on average and 12 % (27 %) at worst; 16 x 128 queries over 4000 keys, 32 / 8 heads of 128: 404 us against 670
-// direct; 4 x 32 queries over 4000 keys, 16 heads of 64: 86 against 37.
-extern "C" int ronn_kv8_chunk_form(int n_seq, int max_q, int max_ctx, int heads, int kv_heads, int head_dim) {
-  if (n_seq <= 0 || max_q <= 0 || max_ctx <= 0 || kv_heads <= 0) return 0;
-  const bool wide = head_dim > 64;
-  const double ctas = double(n_seq) * heads * ((max_q + 127) / 128) / device_sm_count() * (wide ? 0.9 : 0.7);
-  const double expanded = 11 + (max_ctx + 127) / 128 * (wide ? 2.2 : 2.4) * (ctas > 1 ? ctas : 1) +
-                          double(n_seq) * max_ctx * kv_heads * head_dim * 2 / 6.5e6;
-  const double tiles = double(n_seq) * kv_heads * ((long(max_q) * (heads / kv_heads) + 15) / 16);
-  return expanded < 15 + tiles * ((max_ctx + 15) / 16) * (wide ? 0.55e-3 : 0.4e-3);
-}
-
-// The same call as ronn_kv8_attention with queries grouped by sequence, no append, and scale > 0.
-extern "C" int ronn_kv8_chunk_attention(const Kv8AttnCall* c, cudaStream_t stream) {
-  if (c->n_seq <= 0 || c->max_q_len <= 0) return 0;
-  if (c->heads <= 0 || c->kv_heads <= 0 || c->heads % c->kv_heads || (c->ld_q & 7) || (c->ld_o & 7) || !c->seq_start || !c->q_len || c->slots ||
-      c->positions || !(c->scale > 0.f))
-    return -2;
-  const int nb = (c->max_ctx + KV8_BLOCK - 1) / KV8_BLOCK, group = kv8_chunk_group(c->n_seq, c->max_ctx, c->kv_heads, c->head_dim);
-  if (nb > 0 && (!c->scratch || c->scratch_bytes < ronn_kv8_chunk_scratch(c->n_seq, c->max_ctx, c->kv_heads, c->head_dim))) return -4;
-  if (nb == 0) return -5;
-  int* ints = static_cast<int*>(c->scratch);
-  const long int_bytes = (long(group) * (nb + 3) * 4 + 255) / 256 * 256, elems = long(group) * nb * c->kv_heads * KV8_BLOCK * c->head_dim;
-  uint16_t* k = reinterpret_cast<uint16_t*>(static_cast<char*>(c->scratch) + int_bytes);
-  for (int s0 = 0; s0 < c->n_seq; s0 += group) {
-    const int n = c->n_seq - s0 < group ? c->n_seq - s0 : group;
-    int *table = ints, *start = ints + long(group) * nb, *ql = start + group, *kl = ql + group;
-    // without bt_row the sequence is its own table row
-    Kv8ExpandArgs a{static_cast<const uint8_t*>(c->kcodes), static_cast<const uint8_t*>(c->vcodes), c->kscale, c->vscale,
-                    c->bt_row ? c->tables : c->tables + s0 * c->table_ld, c->bt_row ? c->bt_row + s0 : nullptr, c->seq_start + s0, c->q_len + s0,
-                    c->kv_len + s0, k, k + elems, c->out, table, start, ql, kl, c->status, c->table_ld, c->num_blocks, c->rows, c->ld_o,
-                    n, c->bt_row ? c->table_rows : c->table_rows - s0, c->max_blocks, nb, c->kv_heads, c->heads, c->max_q_len};
-    launch(kv8_lengths_kernel, dim3(unsigned(n < 4096 ? (n + 255) / 256 : 16)), dim3(256), 0, stream, a);
-    const long units = 2L * nb * c->kv_heads;
-    const dim3 grid{unsigned((units + 7) / 8), unsigned(n), 1u};
-#define RONN_KV8X(T, D, C) launch(kv8_expand_kernel<T, D, C>, grid, dim3(256), 0, stream, a)
-#define RONN_KV8X_(T) \
-  do { \
-    if (c->head_dim == 64 && c->code == 0) RONN_KV8X(T, 64, 0); \
-    else if (c->head_dim == 64 && c->code == 1) RONN_KV8X(T, 64, 1); \
-    else if (c->head_dim == 128 && c->code == 0) RONN_KV8X(T, 128, 0); \
-    else if (c->head_dim == 128 && c->code == 1) RONN_KV8X(T, 128, 1); \
-    else return -1; \
-  } while (0)
-    if (c->dtype == 0) RONN_KV8X_(__nv_bfloat16);
-    else if (c->dtype == 1) RONN_KV8X_(__half);
-    else return -1;
-#undef RONN_KV8X
-#undef RONN_KV8X_
-    if (cudaGetLastError() != cudaSuccess) return -100;
-    const int rc = ronn_fmha_paged(c->q, c->ld_q, c->rows, 0, k, k + elems, long(group) * nb, table, nb, nullptr, start, ql, kl, c->out, c->ld_o,
-                                   n, c->max_q_len, c->heads, c->kv_heads, c->head_dim, c->causal, c->scale, c->dtype, c->status, stream);
-    if (rc) return rc;
-  }
-  return 0;
 }
