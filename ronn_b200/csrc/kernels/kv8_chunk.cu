@@ -28,7 +28,7 @@ struct Kv8ChunkArgs {
   void *k, *v, *out;
   uint32_t* status;
   long table_ld, num_blocks, rows, ld_o;
-  int table_rows, max_blocks, nb, padded, kv_heads, heads, max_q, causal, pair_heads;      // padded: blocks of a (sequence, head) in scratch
+  int table_rows, max_blocks, nb, padded, kv_heads, heads, max_q, causal, pair_heads, sorted;      // padded: blocks of a (sequence, head) in scratch
   float scale_log2;
 };
 struct Kv8Chunk {
@@ -39,6 +39,45 @@ __device__ __forceinline__ bool kv8_chunk_of(const Kv8ChunkArgs& a, int seq, Kv8
   s.row0 = a.seq_start[seq], s.n = a.q_len[seq], s.len = max(a.kv_len[seq], 0), s.table = a.bt_row ? a.bt_row[seq] : seq;
   return s.row0 >= 0 && s.n >= 0 && s.n <= a.max_q && long(s.row0) + s.n <= a.rows && s.len <= a.nb * KV8_BLOCK &&
          s.len <= a.max_blocks * KV8_BLOCK && s.table >= 0 && s.table < a.table_rows;
+}
+
+// Place `at` in the order of all sequences' items (128 or 256 queries, `unit`), those that see the most keys first: item i of a
+// sequence stands at i + (keys in front of its first query) / unit.  For up to 64 sequences, two a lane; by a whole warp.  False
+// behind the last.
+constexpr int KC_SORTED = 64;
+__device__ __forceinline__ bool kv8_chunk_item(const Kv8ChunkArgs& a, int n_seq, int unit, int at, int& seq, int& item) {
+  const int lane = threadIdx.x & 31;
+  int lo[2], end[2];                                        // [lo, end): the places that a sequence's items have
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    Kv8Chunk s;
+    lo[k] = end[k] = 0;
+    if (lane + 32 * k < n_seq && kv8_chunk_of(a, lane + 32 * k, s)) {
+      const int shift = s.len - s.n;
+      lo[k] = shift >= 0 ? shift / unit : -((unit - 1 - shift) / unit);
+      end[k] = lo[k] + (s.n + unit - 1) / unit;
+    }
+  }
+  auto from = [&](int v) {                                  // items at place v or above
+    return __reduce_add_sync(0xffffffffu, max(0, end[0] - max(lo[0], v)) + max(0, end[1] - max(lo[1], v)));
+  };
+  int low = __reduce_min_sync(0xffffffffu, min(lo[0], lo[1])), high = __reduce_max_sync(0xffffffffu, max(end[0], end[1]));
+  if (at >= from(low)) return false;
+  while (high - low > 1) {                                  // the highest place that leaves `at` among its items
+    const int mid = low + (high - low) / 2;
+    if (from(mid) > at) low = mid;
+    else high = mid;
+  }
+  int rank = at - from(low + 1);
+  const uint32_t here0 = __ballot_sync(0xffffffffu, lo[0] <= low && low < end[0]), here1 = __ballot_sync(0xffffffffu, lo[1] <= low && low < end[1]);
+  const bool second = rank >= __popc(here0);
+  if (second) rank -= __popc(here0);
+  uint32_t left = second ? here1 : here0;
+  for (; rank > 0; --rank) left &= left - 1;
+  const int owner = __ffs(left) - 1;
+  seq = owner + (second ? 32 : 0);
+  item = low - __shfl_sync(0xffffffffu, second ? lo[1] : lo[0], owner);
+  return true;
 }
 
 // The pages of the sequences' contexts as values in order: [sequence][kv_head][padded * 16][D] of K and of V, one warp for each
@@ -185,8 +224,10 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
-  // the last tiles first: with a causal mask they have the most keys
-  const int seq = blockIdx.y, z = int(gridDim.z) - 1 - int(blockIdx.z);
+  // With a causal mask the items differ in their keys: the longest first.  Three sequences of 763 to 1024 queries over 1793 to
+  // 5024 keys, 336 CTAs of 9 to 40 steps, take 176 us, and 187 in the order of the grid.
+  int seq = blockIdx.y, z = int(gridDim.z) - 1 - int(blockIdx.z);
+  if (a.sorted && !kv8_chunk_item(a, a.sorted, a.pair_heads ? KC_TILE : 2 * KC_TILE, blockIdx.y, seq, z)) return;
   Kv8Chunk s;
   if (!kv8_chunk_of(a, seq, s)) return;
   const int head0 = a.pair_heads ? 2 * int(blockIdx.x) : int(blockIdx.x), tile0 = a.pair_heads ? z : 2 * z;
@@ -409,7 +450,8 @@ static int kv8_chunk_tiles(const CUtensorMap& mq, const CUtensorMap& mk, const C
   static bool seen[MAX_DEVICES] = {false};
   if (first_use_on_device(seen) && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::DYN) != cudaSuccess) return -3;
   const int tiles = (a.max_q + KC_TILE - 1) / KC_TILE;
-  const dim3 grid{unsigned(a.pair_heads ? a.heads / 2 : a.heads), unsigned(n_seq), unsigned(a.pair_heads ? tiles : (tiles + 1) / 2)};
+  const int items = a.pair_heads ? tiles : (tiles + 1) / 2;
+  const dim3 grid{unsigned(a.pair_heads ? a.heads / 2 : a.heads), unsigned(a.sorted ? n_seq * items : n_seq), unsigned(a.sorted ? 1 : items)};
   const uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
   const uint32_t idesc_pv = umma_idesc(KC_TILE, D, fmt, 1u) | (1u << 16);          // V's channels are contiguous, its keys are not
   launch(kern, grid, dim3(KC_THREADS), size_t(L::DYN), stream, mq, mk, mv, a, umma_idesc(KC_TILE, KC_TILE, fmt, 1u), idesc_pv);
@@ -478,7 +520,8 @@ extern "C" int ronn_kv8_chunk_attention(const Kv8AttnCall* c, cudaStream_t strea
                    c->bt_row ? c->tables : c->tables + s0 * c->table_ld, c->bt_row ? c->bt_row + s0 : nullptr, c->seq_start + s0, c->q_len + s0,
                    c->kv_len + s0, k, v, c->out, c->status, c->table_ld, c->num_blocks, c->rows, c->ld_o,
                    c->bt_row ? c->table_rows : c->table_rows - s0, c->max_blocks, nb, padded, c->kv_heads, c->heads, c->max_q_len, c->causal,
-                   c->heads / c->kv_heads % 2 == 0, c->scale * 1.4426950408889634f};
+                   c->heads / c->kv_heads % 2 == 0, c->causal && n <= KC_SORTED && long(n) * ((c->max_q_len + KC_TILE - 1) / KC_TILE) <= 65535 ? n : 0,
+                   c->scale * 1.4426950408889634f};
     const dim3 grid{unsigned((units + 7) / 8), unsigned(n), 1u};
 #define RONN_KV8X(T, D, C) \
   do { \
