@@ -476,19 +476,19 @@ extern "C" long ronn_kv8_chunk_scratch(int n_seq, int max_kv, int kv_heads, int 
 }
 
 // Whether chunks of these sizes are faster that way (1) or straight from the codes (0), by what both cost in microseconds.
-// Expanded: a chain of 128-key tiles for each 128 queries and head, 2.4 us a tile (2.2 for heads of 128) while the SMs have
-// one such CTA each, and the values.  Direct: 0.4 ns (0.55) for each 16 query rows and 16 keys.  Over 252 sizes (1 to 16
-// sequences, contexts of 300 to 4000, 16 to 256 queries, four head layouts) the rule costs 0.3 % (1.0 %) against the faster
-// form of each on average and 12 % (27 %) at worst; 16 x 128 queries over 4000 keys, 32 / 8 heads of 128: 404 us against 670
-// direct; 4 x 32 queries over 4000 keys, 16 heads of 64: 86 against 37.
+// Expanded: 128 keys after the other for each pair of tiles, 1.5 us a step (1.8 for heads of 128) while the SMs have no more than
+// two thirds of a CTA each, and the values, 2 (1.6) TB/s.  Direct: 0.5 ns (0.9) for each 16 query rows and 16 keys.  Over 240
+// sizes (1 to 16 sequences, contexts of 300 to 4000, 16 to 512 queries, four head layouts) the rule costs 0.5 % (1.0 %) against
+// the faster form of each on average and 13 % (25 %, 4 us) at worst; 16 x 128 queries over 4000 keys, 32 / 8 heads of 128: 225 us
+// against 711 direct; 4 x 32 queries over 4000 keys, 16 heads of 64: 78 against 37.
 extern "C" int ronn_kv8_chunk_form(int n_seq, int max_q, int max_ctx, int heads, int kv_heads, int head_dim) {
   if (n_seq <= 0 || max_q <= 0 || max_ctx <= 0 || kv_heads <= 0) return 0;
-  const bool wide = head_dim > 64;
-  const double ctas = double(n_seq) * heads * ((max_q + 127) / 128) / device_sm_count() * (wide ? 0.9 : 0.7);
-  const double expanded = 11 + (max_ctx + 127) / 128 * (wide ? 2.2 : 2.4) * (ctas > 1 ? ctas : 1) +
-                          double(n_seq) * max_ctx * kv_heads * head_dim * 2 / 6.5e6;
+  const bool wide = head_dim > 64, pairs = heads / kv_heads % 2 == 0;
+  const double ctas = double(n_seq) * (pairs ? heads / 2 * ((max_q + 127L) / 128) : heads * ((max_q + 255L) / 256)) / device_sm_count() * 1.5;
+  const double expanded = (wide ? 15 : 13) + (max_ctx + 127L) / 128 * (wide ? 1.8 : 1.53) * (ctas > 1 ? ctas : 1) +
+                          double(n_seq) * max_ctx * kv_heads * head_dim * 2 * (wide ? 6.1e-7 : 5.1e-7);
   const double tiles = double(n_seq) * kv_heads * ((long(max_q) * (heads / kv_heads) + 15) / 16);
-  return expanded < 15 + tiles * ((max_ctx + 15) / 16) * (wide ? 0.55e-3 : 0.4e-3);
+  return expanded < (wide ? 19.5 : 15) + tiles * ((max_ctx + 15L) / 16) * (wide ? 0.9e-3 : 0.49e-3);
 }
 
 // The same call as ronn_kv8_attention with queries grouped by sequence, no append, and scale > 0.
