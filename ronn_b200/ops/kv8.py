@@ -28,7 +28,7 @@ _BLOCK = 16
 _TILE = 16                                   # query rows of an attention tile
 
 
-# the launchers' call records (kv8_attention.cu, kv8_cache.cu), packed: a decode step is made of calls of a few microseconds, and
+# the launchers' call records (kv8_attention.cu, kv8_cache.cu, kv8_chunk.cu), packed: a decode step is made of calls of a few microseconds, and
 # three dozen arguments one by one cost as much as the kernel
 _APPEND_CALL = struct.Struct("=10Q4q8i")
 _READ_CALL = struct.Struct("=8Q2q4i")

@@ -560,3 +560,33 @@ def test_a_loose_bound_of_queries_changes_nothing():
     args = (_activations(7, heads * d, "bf16", 99), 0, cache, _i32([[0, 1], [2, 3]]), _i32([0, 3]), _i32([3, 4]), _i32([20, 32]))
     for form in ("direct", "expanded"):
         assert torch.equal(ops.kv8_prefill_attention(*args, 4, 32, heads, form=form), ops.kv8_prefill_attention(*args, 2 ** 40, 32, heads, form=form))
+
+
+@pytest.mark.parametrize("n_seq", [3, 33, 64, 65])
+@pytest.mark.parametrize("heads,kvh", [(2, 1), (3, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_expanded_chunks_of_many_sequences(monkeypatch, n_seq, heads, kvh, causal):
+    """Each tile of each sequence is worked on once, in whatever order: sequences without queries or keys, of several tiles, with
+    fewer keys than queries, and one that passes the bounds and is left out and reported."""
+    monkeypatch.delenv("RONN_KERNEL_CHECKS", raising=False)          # the host's checks would refuse the last first
+    ops, d = _ops(), 64
+    g = torch.Generator().manual_seed(n_seq)
+    counts = [(0, 1, 127, 128, 129, 300)[int(torch.randint(6, (1,), generator=g))] for _ in range(n_seq)]
+    lens = [int(torch.randint(0, 500, (1,), generator=g)) for _ in range(n_seq)]
+    counts[:2], lens[:2], bad = [300, 257], [480, 130], n_seq - 1
+    lens[bad] = 600                                                   # behind max_kv_len
+    starts = [sum(counts[:i]) for i in range(n_seq)]
+    blocks = sum(-(-n // 16) for n in lens) + 1
+    cache, table = _filled(blocks, kvh, d, "fp8", 101), _pages(lens, blocks, 102)
+    q = _activations(sum(counts), heads * d, "bf16", 103)
+    out = torch.full_like(q, 9.0)
+    call = lambda form, out: ops.kv8_prefill_attention(q, 0, cache, table.cuda(), _i32(starts), _i32(counts), _i32(lens), 300, 500, heads, causal,
+                                                       out=out, form=form)
+    call("expanded", out)
+    with pytest.raises(Exception, match="8-bit KV cache"):
+        ops.check_status()
+    rows = [(i, starts[i] + j, max(0, lens[i] - (counts[i] - 1 - j)) if causal else lens[i]) for i in range(n_seq) if i != bad for j in range(counts[i])]
+    assert bool((out[starts[bad]:] == 9).all()) and not bool((out[:starts[bad]] == 9).all(1).any())
+    some = rows[::max(1, len(rows) // 600)]
+    _compare(out[[r for _, r, _ in some]], cache, q[[r for _, r, _ in some]], [table[i] for i, _, _ in some], [n for _, _, n in some], heads,
+             p_round=2.0 ** -8)
