@@ -223,7 +223,6 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   volatile uint32_t* abort = tmem_slot + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  pdl_trigger();
   // With a causal mask the items differ in their keys: the longest first.  Three sequences of 763 to 1024 queries over 1793 to
   // 5024 keys, 336 CTAs of 9 to 40 steps, take 176 us, and 187 in the order of the grid.
   int seq = blockIdx.y, z = int(gridDim.z) - 1 - int(blockIdx.z);
@@ -261,6 +260,9 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;                         // S of tile u at 128 u, O at 256 + 128 u
+  // Only now may the next kernel start: one that takes tensor memory and then waits for this grid would keep a CTA that has
+  // none yet waiting for good.
+  pdl_trigger();
 
   if (warp == 0) {
     if (lane == 0 && all > 0) {

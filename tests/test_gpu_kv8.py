@@ -590,3 +590,38 @@ def test_expanded_chunks_of_many_sequences(monkeypatch, n_seq, heads, kvh, causa
     some = rows[::max(1, len(rows) // 600)]
     _compare(out[[r for _, r, _ in some]], cache, q[[r for _, r, _ in some]], [table[i] for i, _, _ in some], [n for _, _, n in some], heads,
              p_round=2.0 ** -8)
+
+
+def test_expanded_chunks_between_products_that_take_tensor_memory():
+    """Chunk attention takes all of an SM's tensor memory; products before and behind it in the stream start early and take some."""
+    ops, heads, kvh, d, n = _ops(), 16, 16, 64, 700
+    lens = [900, 700, 1300]
+    cache, table = _filled(sum(-(-k // 16) for k in lens) + 1, kvh, d, "int8", 121), _pages(lens, sum(-(-k // 16) for k in lens) + 1, 122)
+    x, w = _activations(3 * n, heads * d, "bf16", 123), _activations(heads * d, heads * d, "bf16", 124) / 32
+    tab, start, count, keys = table.cuda(), _i32([0, n, 2 * n]), _i32([n] * 3), _i32(lens)
+
+    def chain():
+        y = x
+        for _ in range(4):
+            q = ops.gemm(y, w)
+            y = ops.gemm(ops.kv8_prefill_attention(q, 0, cache, tab, start, count, keys, n, 1300, heads, form="expanded"), w)
+        return y
+    want = chain()
+    torch.cuda.synchronize()
+    apart = x
+    for _ in range(4):
+        q = ops.gemm(apart, w)
+        torch.cuda.synchronize()
+        o = ops.kv8_prefill_attention(q, 0, cache, tab, start, count, keys, n, 1300, heads, form="expanded")
+        torch.cuda.synchronize()
+        apart = ops.gemm(o, w)
+        torch.cuda.synchronize()
+    assert torch.equal(want, apart) and bool(torch.isfinite(want).all())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        again = chain()
+    for _ in range(5):
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, want)
+    ops.check_status()
