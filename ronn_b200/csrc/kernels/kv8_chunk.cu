@@ -9,6 +9,11 @@
 //   warps 2-9   four a tile, one query row a thread: the row of S in registers, maximum, exponentials, sum, P back.  O stays in
 //               tensor memory and is rescaled only when a row's maximum has grown by more than 2^8.
 // Statistics and O are in 32 bits; P is rounded to the activations' type, by half a step.
+// A step of 128 keys is a chain of softmax (1800 cycles, 1024 of them a warp's exponentials), P V and the next Q K^T (750 each);
+// two tiles overlap theirs, so that neither the tensor pipe (46 % of a causal chunk) nor the exponentials are full.  2 x 4096
+// queries over 4096 keys, 32 / 8 heads of 128, without a mask: 510 us, 1078 TFLOP/s.  674 us with instructions issued from a lane
+// of its own; an issuer that looked for whichever tile could go on was slower still (3 chunks of 763 to 1024 queries: 230 us
+// against 191 for taking the tiles in turn).
 #include "kv8.cuh"
 #include "ptx_sm100.cuh"
 #include "tma_desc.cuh"
