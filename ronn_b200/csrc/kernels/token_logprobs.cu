@@ -29,6 +29,10 @@ constexpr int TL_SLACK = 8;            // threads beyond `top` that may offer ca
 constexpr int TL_CAND = 1024;
 constexpr float TL_LOG2E = 1.4426950408889634f;
 constexpr int TL_BATCH = 4;            // vectors a lane has on their way
+// A term's exponent is x log2 e - m log2 e in one operation, and what rounding m log2 e leaves over (m_lo) is made good once a
+// row.  That is half a unit at most up to this magnitude; further out it would pass the range of an exponent.  A warp whose
+// maximum lies there (nothing but masks of -1e9 so far, a token forced by 1e10) takes x - m first, element by element.
+constexpr float TL_FAR = 8388608.f;
 
 struct TlArgs {
   const void* logits;
@@ -107,6 +111,7 @@ template <class T> struct TlVec {
   }
   // With a maximum above LOW, -inf and the type's lowest value weigh the same: nothing.
   static constexpr float LOW = std::is_same<T, __half>::value ? -6e4f : -1e30f;
+  static constexpr float FROM = std::is_same<T, __half>::value ? -6e4f : -TL_FAR;        // maxima from here to TL_FAR: the fast way
   static __device__ __forceinline__ uint4 finite(uint4 v) {
     const uint32_t low = std::is_same<T, __half>::value ? 0xfbfffbffu : 0xfe96fe96u;        // bf16: -1e38, whose product with log2 e is finite
     return make_uint4(tl_max2<T>(v.x, low), tl_max2<T>(v.y, low), tl_max2<T>(v.z, low), tl_max2<T>(v.w, low));
@@ -134,6 +139,7 @@ template <class T> struct TlVec {
       return int(lo + hi);
     }
   };
+  static __device__ __forceinline__ uint32_t word(float x) { return Pair16<T>::pack(x, x); }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
     Pair16<T>::unpack(v.x, f[0], f[1]);
     Pair16<T>::unpack(v.y, f[2], f[3]);
@@ -146,7 +152,7 @@ template <> struct TlVec<float> {
   static __device__ __forceinline__ float largest(const uint4& v) {
     return tl_max_nan(tl_max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), tl_max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
-  static constexpr float LOW = -1e30f;
+  static constexpr float LOW = -1e30f, FROM = -TL_FAR;
   static __device__ __forceinline__ uint4 finite(uint4 v) {
     return make_uint4(__float_as_uint(fmaxf(__uint_as_float(v.x), -1e32f)), __float_as_uint(fmaxf(__uint_as_float(v.y), -1e32f)),
                       __float_as_uint(fmaxf(__uint_as_float(v.z), -1e32f)), __float_as_uint(fmaxf(__uint_as_float(v.w), -1e32f)));
@@ -163,6 +169,7 @@ template <> struct TlVec<float> {
     }
     __device__ __forceinline__ int sum() const { return n; }
   };
+  static __device__ __forceinline__ uint32_t word(float x) { return __float_as_uint(x); }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
   }
@@ -300,10 +307,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
         equal = 0;
       }
       m_hi = up * TL_LOG2E;                                              // m log2 e in two parts
-      m_lo = fabsf(up) < 1e30f ? fmaf(up, TL_LOG2E, -m_hi) : 0.f;
+      m_lo = fabsf(up) < TL_FAR ? fmaf(up, TL_LOG2E, -m_hi) : 0.f;
       m = up, mk = bk;
     }
-    if (m > V::LOW && m < 1e30f) {
+    if (m > V::FROM && m < TL_FAR) {
       const unsigned long long minus = tl_two(-m_hi, -m_hi), log2e = tl_two(TL_LOG2E, TL_LOG2E);
       unsigned long long r2 = 0, e2 = 0;
       if (top > above) {                                                 // logits before the token's
@@ -335,11 +342,20 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
       }
       const float2 rs = tl_split(r2), es = tl_split(e2);
       r += rs.x + rs.y, e += es.x + es.y;
-    } else {                                                             // nothing seen yet, or logits at the end of their range
+    } else {                                                             // nothing seen yet, or a maximum far out: differences first
+      const uint32_t word = V::word(m);                                  // a mask's vectors, all maximum, are counted whole
+      uint32_t mixed = 0;
+#pragma unroll
+      for (int k = 0; k < TL_BATCH; ++k)
+        if (raw[k].x != word || raw[k].y != word || raw[k].z != word || raw[k].w != word) mixed |= 1u << k;
       for (int k = 0; k < TL_BATCH && k0 + k < left; ++k) {
+        const float th = v_lo + tid + (k0 + k) * TL_THREADS < vt ? above : xt;
+        if (!(mixed >> k & 1)) {
+          if (m != none) equal += E, ahead += m > th ? E : 0;
+          continue;
+        }
         float f[E];
         V::unpack(tl_load(base, v_lo + tid + (k0 + k) * TL_THREADS, skip, end), f);
-        const float th = v_lo + tid + (k0 + k) * TL_THREADS < vt ? above : xt;
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           ahead += f[j] > th ? 1 : 0;
