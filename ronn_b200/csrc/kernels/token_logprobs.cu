@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1024 / TL_THREADS) token_logprobs_
         equal = 0;
       }
       m_hi = up * TL_LOG2E;                                              // m log2 e in two parts
-      m_lo = fabsf(up) < TL_FAR ? fmaf(up, TL_LOG2E, -m_hi) : 0.f;
+      m_lo = up > V::FROM && up < TL_FAR ? fmaf(up, TL_LOG2E, -m_hi) : 0.f;        // only terms of the branch below lack 2^-m_lo
       m = up, mk = bk;
     }
     if (m > V::FROM && m < TL_FAR) {

@@ -71,3 +71,16 @@ def test_magnitudes_over_the_whole_range(dtype, rows, vocab):
     x = (size * (1 + step)).to(DT[dtype])
     x[::3, 5] = 1.0                                                   # an ordinary token beside them
     _check(x, torch.randint(0, vocab, (rows,), generator=g), 3)
+
+
+def test_fp16_rows_at_the_end_of_the_range():
+    """Logits between the type's lowest and -60000, 32 and more apart: a nearly certain token's log probability is the sum of
+    the others, whose digits it keeps."""
+    vocab = 20011
+    x = torch.full((5, vocab), -65504.0)
+    for r, m in enumerate((-60000, -60032, -60672, -64000, -65472)):
+        x[r, 100 * r + 7] = m
+        x[r, 5000:9000] = m - 32
+    x = x.half()
+    assert x.max(1).values.tolist() == [-60000, -60032, -60672, -64000, -65472]
+    _check(x, torch.tensor([7, 107, 207, 307, 407]), 3)
