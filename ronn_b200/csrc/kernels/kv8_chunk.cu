@@ -87,7 +87,8 @@ __device__ __forceinline__ bool kv8_chunk_item(const Kv8ChunkArgs& a, int n_seq,
 
 // The pages of the sequences' contexts as values in order: [sequence][kv_head][padded * 16][D] of K and of V, one warp for each
 // (block, head, K or V).  A value is exact in bf16; in fp16 it is kept within the type's range.  Slots behind the context, to the
-// end of the last 128 keys, are zeros.  A poisoned block has NaN keys and zero values, so that only those who see it read NaN.
+// end of the last 128 keys, and blocks whose page lies outside the cache are zeros, which the attention leaves out.  A poisoned block
+// has NaN keys and zero values, so that only those who see it read NaN.
 template <class T, int D, int CODE>
 __global__ void __launch_bounds__(256) kv8_expand_kernel(Kv8ChunkArgs a) {
   pdl_wait();
@@ -226,6 +227,8 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   uint64_t *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 13;                                             // one a tile
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
   volatile uint32_t* abort = tmem_slot + 1;
+  const int* volatile* s_pages = reinterpret_cast<const int* volatile*>(bars + 16);                   // the context's pages, and its last block
+  volatile int* s_last = reinterpret_cast<volatile int*>(bars + 17);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   // With a causal mask the items differ in their keys: the longest first.  Three sequences of 763 to 1024 queries over 1793 to
@@ -253,6 +256,7 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&o_full[i], 1);
     }
     *abort = 0;
+    *s_pages = a.tables + long(s.table) * a.table_ld, *s_last = (s.len - 1) / KV8_BLOCK;
     mbar_fence_init();
     fence_proxy_async_smem();
   }
@@ -345,12 +349,24 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int mine = u == 0 ? steps[0] : steps[1];
     const int head = a.pair_heads ? head0 + u : head0, tile = a.pair_heads ? tile0 : tile0 + u;
     const int qi = tile * KC_TILE + quarter * 32 + lane;                 // this thread's query
-    const int limit = a.causal ? min(s.len, qi + shift + 1) : s.len;     // the keys it sees
+    int limit = a.causal ? max(min(s.len, qi + shift + 1), 0) : s.len;   // the keys it sees
     const uint32_t at = tmem + (uint32_t(quarter * 32) << 16), s_at = at + u * 128, o_at = at + 256 + u * 128;
     const unsigned long long scale2 = kc_two(a.scale_log2, a.scale_log2);
     float m = -1e30f;
     unsigned long long l2[2] = {0ull, 0ull};
     bool ok = true;
+    // Pages outside the cache: looked for while the first scores are on their way, and again in each step only where there are some:
+    // `limit` is then its complement, below 0 in every lane, and all steps count as edges.  Anything more that lives through the
+    // loop is spilled and took 1.4 % of a chunk, as did looking at one page after the other.
+    auto absent = [&](int page) { return uint32_t(page) >= uint32_t(a.num_blocks); };
+    bool lacks = false;
+    {
+      const int* const pages = *s_pages;
+      const int last = *s_last;
+#pragma unroll 8
+      for (int b = lane; b < mine * KC_PAGES; b += 32) lacks |= absent(pages[min(b, last)]);
+    }
+    if (__any_sync(0xffffffffu, lacks)) limit = ~limit;
     for (int j = 0; j < mine; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[u], j & 1, abort, a.status, STATUS_WAIT_ACCUM)) && ok;
       tc_fence_after_sync();
@@ -360,11 +376,20 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tmem_ld_wait();
       const int key0 = j * KC_TILE;
       if (!__all_sync(0xffffffffu, key0 + KC_TILE <= limit)) {
+        const int seen = (limit < 0 ? ~limit : limit) - key0;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (key0 + c * 32 + i >= limit) x[c][i] = 0xff800000u;       // -inf
+            if (c * 32 + i >= seen) x[c][i] = 0xff800000u;               // -inf
+        if (limit < 0) {                                    // keys that are not there are left out
+          const uint32_t gone = __ballot_sync(0xffffffffu, lane < KC_PAGES && absent((*s_pages)[min(j * KC_PAGES + lane, *s_last)]));
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (gone >> (2 * c + i / KV8_BLOCK) & 1) x[c][i] = 0xff800000u;
+        }
       }
       float top[4];
 #pragma unroll
