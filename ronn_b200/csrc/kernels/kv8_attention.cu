@@ -51,9 +51,25 @@ struct Kv8AttnArgs {
   float* part;                // splits > 1: [item][split][rows][D + 2] partial results
   uint32_t* status;
   long ld_q, ld_o, num_blocks, rows, table_ld;
-  int group, items_x, table_rows, max_blocks, heads, kv_heads, causal, splits, share, part_rows, max_q, k_off, v_off;
+  int group, items_x, table_rows, max_blocks, heads, kv_heads, causal, splits, share, part_rows, max_q, max_keys, k_off, v_off;
   float scale_log2;
 };
+
+// A sequence's table row, the keys that it lists, and whether it has fewer than the sequence has keys: the others are left out.
+struct Kv8Keys {
+  int table, len;
+  bool cut;
+};
+__device__ __forceinline__ Kv8Keys kv8_keys(const Kv8AttnArgs& a, int seq) {
+  const int table = a.bt_row ? a.bt_row[seq] : seq, keys = a.kv_len[seq];
+  const bool listed = table >= 0 && table < a.table_rows;
+  const int len = listed ? min(keys, a.max_blocks * KV8_BLOCK) : 0;
+  return {listed ? table : 0, len, !listed || len < keys};
+}
+// False for a sequence of a chunk whose rows or lengths pass the call's bounds: it is left out, and its rows stay as they are.
+__device__ __forceinline__ bool kv8_takes_part(const Kv8AttnArgs& a, long row0, int n, int len) {
+  return row0 >= 0 && n >= 0 && row0 + n <= a.rows && (!a.q_len || (n <= a.max_q && len <= a.max_keys));
+}
 
 __device__ __forceinline__ void kv8_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -200,21 +216,14 @@ __global__ void __launch_bounds__(KV8_NW * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT
   const int n = a.q_len ? a.q_len[seq] : 1;
   const int r0 = blockIdx.y * 16;
   const int live = min(min(16, a.part_rows), n * group - r0);   // rows of this tile
-  if (n > a.max_q && it == 0) kv8_report(a.status);             // more queries than the launch was sized for: left out
-  if (live <= 0) return;
   const long row0 = a.seq_start ? long(a.seq_start[seq]) : seq;
-  const int table = a.bt_row ? a.bt_row[seq] : seq;
+  const Kv8Keys keys = kv8_keys(a, seq);
+  const int len = keys.len, table = keys.table;
+  const bool takes_part = kv8_takes_part(a, row0, n, len);
+  if ((!takes_part || keys.cut) && it == 0) kv8_report(a.status);
+  if (!takes_part || live <= 0) return;
   const int slot = a.slots ? a.slots[seq] : -1;
   const int pos = a.positions ? a.positions[seq] : 0;
-  int len = min(a.kv_len[seq], a.max_blocks * KV8_BLOCK);
-  if (row0 < 0 || row0 + n > a.rows) {
-    if (it == 0) kv8_report(a.status);
-    return;
-  }
-  if (table < 0 || table >= a.table_rows) {
-    if (it == 0) kv8_report(a.status);
-    len = 0;
-  }
   // keys that the tile's last query sees, this share's blocks, this warp's
   auto query_of = [&](int r) { return n == 1 ? 0 : r / group; };          // of row r: a decode step has one
   const int seen = a.causal ? len - (n - 1 - query_of(r0 + live - 1)) : len;
@@ -586,7 +595,7 @@ __global__ void __launch_bounds__(KV8_CW * 32) kv8_combine_kernel(Kv8AttnArgs a)
   const int n = a.q_len ? a.q_len[seq] : 1;
   if (r0 + r >= n * group || r >= 16) return;
   const long row0 = a.seq_start ? long(a.seq_start[seq]) : seq;
-  if (row0 < 0 || row0 + n > a.rows) return;
+  if (!kv8_takes_part(a, row0, n, a.q_len ? kv8_keys(a, seq).len : 0)) return;
   const float* src = a.part + (long(tile) * a.splits * a.part_rows + r) * (D + 2);
   const long step = long(a.part_rows) * (D + 2);
   auto share = [&](int z) { return z < a.splits ? *reinterpret_cast<const float2*>(src + z * step + D) : make_float2(-INFINITY, 0.f); };
@@ -688,7 +697,7 @@ extern "C" int ronn_kv8_attention(const Kv8AttnCall* call, cudaStream_t stream) 
     for (int j = 0; j < head_dim / 2; ++j) tn.t[j] = turns[j];
   Kv8AttnArgs a{q, out, (uint8_t*)kcodes, (uint8_t*)vcodes, kscale, vscale, tables, kv_len, bt_row, seq_start, q_len, slots, positions,
                 (float*)scratch, status, ld_q, ld_o, num_blocks, rows, table_ld, heads / kv_heads, int(xs), table_rows, max_blocks, heads, kv_heads, causal,
-                plan.splits, plan.share, part_rows, max_q_len, k_off, v_off, scale * 1.4426950408889634f};
+                plan.splits, plan.share, part_rows, max_q_len, int((long(max_ctx) + KV8_BLOCK - 1) / KV8_BLOCK * KV8_BLOCK), k_off, v_off, scale * 1.4426950408889634f};
   const long per_cta = KV8_NW / wpi;
   const dim3 grid{unsigned((xs + per_cta - 1) / per_cta), unsigned(mtiles), unsigned(splits)};
   const bool small = group_rows <= 8;

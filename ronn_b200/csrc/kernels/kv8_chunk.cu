@@ -38,12 +38,17 @@ struct Kv8ChunkArgs {
 };
 struct Kv8Chunk {
   int row0, n, len, table;
+  bool cut;                                                 // keys that no table row lists are left out
 };
-// A sequence's place and lengths; false where they pass a bound: it has no queries then.
+// A sequence's place and lengths; false where they pass a bound: it is left out, and its rows stay as they are.
 __device__ __forceinline__ bool kv8_chunk_of(const Kv8ChunkArgs& a, int seq, Kv8Chunk& s) {
-  s.row0 = a.seq_start[seq], s.n = a.q_len[seq], s.len = max(a.kv_len[seq], 0), s.table = a.bt_row ? a.bt_row[seq] : seq;
-  return s.row0 >= 0 && s.n >= 0 && s.n <= a.max_q && long(s.row0) + s.n <= a.rows && s.len <= a.nb * KV8_BLOCK &&
-         s.len <= a.max_blocks * KV8_BLOCK && s.table >= 0 && s.table < a.table_rows;
+  s.row0 = a.seq_start[seq], s.n = a.q_len[seq], s.table = a.bt_row ? a.bt_row[seq] : seq;
+  const int keys = max(a.kv_len[seq], 0);
+  const bool listed = s.table >= 0 && s.table < a.table_rows;
+  s.len = listed ? min(keys, a.max_blocks * KV8_BLOCK) : 0;
+  s.cut = !listed || s.len < keys;
+  if (!listed) s.table = 0;
+  return s.row0 >= 0 && s.n >= 0 && s.n <= a.max_q && long(s.row0) + s.n <= a.rows && s.len <= a.nb * KV8_BLOCK;
 }
 
 // Place `at` in the order of all sequences' items (128 or 256 queries, `unit`), those that see the most keys first: item i of a
@@ -95,10 +100,9 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(Kv8ChunkArgs a) {
   pdl_trigger();
   const int seq = blockIdx.y, lane = threadIdx.x & 31, unit = blockIdx.x * 8 + (threadIdx.x >> 5);
   Kv8Chunk s;
-  if (!kv8_chunk_of(a, seq, s)) {
-    if (unit == 0 && lane == 0) kv8_report(a.status);
-    return;
-  }
+  const bool takes_part = kv8_chunk_of(a, seq, s);
+  if ((!takes_part || s.cut) && unit == 0 && lane == 0) kv8_report(a.status);
+  if (!takes_part) return;
   const int len = s.len, per = 2 * a.kv_heads, b = unit / per, rest = unit - b * per;
   if (b >= (len + KC_TILE - 1) / KC_TILE * KC_PAGES) return;
   const bool is_v = rest >= a.kv_heads;

@@ -5,8 +5,9 @@ fp32 scale for each (block, head), a power of two; keys and values have scales o
 0 is written; tokens that join it later can raise its scale, and then the codes below them are rounded once more.  A token
 with a value that is not finite makes its block and head read as NaN until the block begins again.
 
-Page numbers, slots and table rows come from device memory.  One that lies outside the cache is not accessed: the key it
-stands for is left out, the kernel sets the device's status word, and ``check_status`` raises.
+Page numbers, slots, table rows and lengths come from device memory.  What lies outside the cache or its tables is not accessed:
+the keys that a page, a table row, or columns behind the table's last stand for are left out, the kernel sets the device's status
+word, and ``check_status`` raises.
 """
 from __future__ import annotations
 
@@ -309,7 +310,8 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
     on ([tokens, ld], head h at column q_off + h * head_dim) and attends to the ``kv_len[s]`` keys that row ``bt_row[s]``
     (default s) of the block tables lists; with ``causal`` its queries are the last positions of that context, and a query in
     front of the first key gives zeros.  The new tokens' K and V are in the cache already.  Returns [tokens, heads * head_dim];
-    rows that belong to no sequence are not written.  ``max_q_len`` bounds the queries of a sequence, ``max_kv_len`` its keys.
+    rows that belong to no sequence are not written.  ``max_q_len`` bounds the queries of a sequence, ``max_kv_len`` (in
+    whole cache blocks) its keys; a sequence that passes them or the rows of q is left out and reported, its rows are not written.
     Few queries read the codes as they are ("direct"); for many the contexts are expanded to 16-bit values first and the
     tensor-core attention runs over those ("expanded", for a positive scale; fp16 keeps values within its range, and probabilities
     in the activations' type).  ``form`` names one, for measurements."""

@@ -53,3 +53,67 @@ def test_keys_of_pages_outside_the_cache_are_left_out(dtype, code, heads, kvh, d
     whole = ops.kv8_prefill_attention(q[208:], 0, cache, table[3:].cuda(), _i32([0]), _i32([40]), _i32([40]), 40, 40, heads, causal, form=form)
     assert torch.equal(whole, out[208:])
     ops.check_status()
+
+
+@pytest.mark.parametrize("form", ["direct", "expanded"])
+@pytest.mark.parametrize("rows", [True, False])
+def test_a_table_row_outside_the_table_lists_no_keys(form, rows):
+    """Rows of such a sequence are zeros; one without table rows of its own (fewer rows than sequences) is refused."""
+    ops, heads, d = _ops(), 4, 64
+    cache, table = _filled(9, 2, d, "int8", 211), _pages([60, 50], 9, 212)
+    q = _activations(90, heads * d, "bf16", 213)
+    if not rows:
+        with pytest.raises(ops.OperandError, match="2 rows for 3"):
+            ops.kv8_prefill_attention(q, 0, cache, table.cuda(), _i32([0, 30, 60]), _i32([30] * 3), _i32([60, 50, 40]), 30, 60, heads, form=form)
+        return
+    for bad in (-1, 2, 2 ** 31 - 1, -2 ** 31):
+        out = torch.full_like(q, 9.0)
+        ops.kv8_prefill_attention(q, 0, cache, table.cuda(), _i32([0, 30, 60]), _i32([30] * 3), _i32([60, 50, 40]), 30, 60, heads, True,
+                                  _i32([0, bad, 1]), out=out, form=form)
+        assert bool((out[30:60] == 0).all())
+        _reported(ops)
+        limits = [60 - 29 + j for j in range(30)] + [40 - 29 + j for j in range(30)]
+        _compare(torch.cat([out[:30], out[60:]]), cache, torch.cat([q[:30], q[60:]]), [table[0]] * 30 + [table[1]] * 30, limits, heads,
+                 **_round("bf16", form))
+
+
+@pytest.mark.parametrize("form", ["direct", "expanded"])
+@pytest.mark.parametrize("max_kv", [96, 1000])
+def test_keys_beyond_the_table_are_cut_off(form, max_kv):
+    """A context longer than its table's columns list ends with them, for its queries' places too."""
+    ops, heads, d = _ops(), 4, 64
+    cache = _filled(9, 2, d, "fp8", 221)
+    table = torch.tensor([[0, 1, 2, 3, 4, 5], [8, 7, 6, 5, 4, 3]], dtype=torch.int32)
+    q = _activations(80, heads * d, "bf16", 223)
+    for long in (97, 2 ** 31 - 1):
+        out = ops.kv8_prefill_attention(q, 0, cache, table.cuda(), _i32([0, 40]), _i32([40, 40]), _i32([long, 77]), 40, max_kv, heads, form=form)
+        _compare(out, cache, q, [table[0]] * 40 + [table[1]] * 40, [96 - 39 + j for j in range(40)] + [77 - 39 + j for j in range(40)], heads,
+                 **_round("bf16", form))
+        _reported(ops)
+
+
+def test_single_rows_beyond_the_table_are_cut_off_and_reported():
+    ops, heads, d = _ops(), 4, 64
+    cache, table = _filled(9, 2, d, "fp8", 225), torch.tensor([[0, 1], [5, 4], [7, 8]], dtype=torch.int32)
+    q = _activations(3, heads * d, "bf16", 226)
+    for long in (33, 2 ** 31 - 1):
+        _compare(ops.kv8_attention(q, cache, table.cuda(), _i32([32, long, 5]), heads, 1000), cache, q, table, [32, 32, 5], heads)
+        _reported(ops)
+
+
+@pytest.mark.parametrize("form", ["direct", "expanded"])
+@pytest.mark.parametrize("heads,kvh,d,keys", [(4, 2, 64, 64), (8, 1, 128, 2000)])
+@pytest.mark.parametrize("what", ["more queries than max_q_len", "fewer than none", "more keys than max_kv_len", "rows behind the last", "rows in front"])
+def test_sequences_that_pass_their_bounds_are_left_out(form, heads, kvh, d, keys, what):
+    """Not a row of theirs is written; with few and with many keys (shares of a context that are joined)."""
+    ops = _ops()
+    blocks = 2 * (-(-keys // 16)) + 10
+    cache, table = _filled(blocks, kvh, d, "int8", 231), _pages([keys, keys + 100], blocks, 232)
+    q = _activations(30, heads * d, "bf16", 233) * 0.5
+    start, count, kv = {"more queries than max_q_len": (5, 8, keys), "fewer than none": (5, -3, keys), "more keys than max_kv_len": (5, 7, keys + 40),
+                        "rows behind the last": (24, 7, keys), "rows in front": (-1, 7, keys)}[what]
+    out = torch.full_like(q, 9.0)
+    ops.kv8_prefill_attention(q, 0, cache, table.cuda(), _i32([0, start]), _i32([5, count]), _i32([keys, kv]), 7, keys, heads, out=out, form=form)
+    _reported(ops)
+    assert bool((out[5:] == 9).all())
+    _compare(out[:5], cache, q[:5], [table[0]] * 5, [keys - 4 + j for j in range(5)], heads, **_round("bf16", form))
