@@ -34,7 +34,7 @@ struct Kv8ChunkArgs {
   uint32_t* status;
   long table_ld, num_blocks, rows, ld_o;
   int table_rows, max_blocks, nb, padded, kv_heads, heads, max_q, causal, pair_heads, sorted;      // padded: blocks of a (sequence, head) in scratch
-  float scale_log2;
+  float scale_log2, slack;      // slack: a growth of the maximum by 2^8, in scores before their scale
 };
 struct Kv8Chunk {
   int row0, n, len, table;
@@ -166,14 +166,14 @@ __device__ __forceinline__ float2 kc_split(unsigned long long v) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
-__device__ __forceinline__ unsigned long long kc_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 __device__ __forceinline__ unsigned long long kc_add2(unsigned long long a, unsigned long long b) {
   unsigned long long r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long kc_mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ float kc_max3(float a, float b, float c) {
@@ -356,7 +356,7 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     int limit = a.causal ? max(min(s.len, qi + shift + 1), 0) : s.len;   // the keys it sees
     const uint32_t at = tmem + (uint32_t(quarter * 32) << 16), s_at = at + u * 128, o_at = at + 256 + u * 128;
     const unsigned long long scale2 = kc_two(a.scale_log2, a.scale_log2);
-    float m = -1e30f;
+    float m = -INFINITY;                                    // of the scores before their scale, which is positive
     unsigned long long l2[2] = {0ull, 0ull};
     bool ok = true;
     // Pages outside the cache: looked for while the first scores are on their way, and again in each step only where there are some:
@@ -402,10 +402,11 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
         for (int i = 2; i < 32; i += 2) top[c] = kc_max3(top[c], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
       }
-      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;          // the scale is positive
-      const float m_new = mx > m + 8.f ? mx : m;
+      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      const float m_new = mx > m + a.slack ? mx : m;
+      const float back = m_new == -INFINITY ? 0.f : -m_new;              // without a key all exponents are -inf, from 0 too
       if (__any_sync(0xffffffffu, m_new != m)) {
-        const float alpha = kc_exp2(m - m_new);
+        const float alpha = kc_exp2((m + back) * a.scale_log2);
         if (j > 0) {                                        // the products so far are complete: S of this step came after them
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
@@ -421,13 +422,15 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         l2[0] = kc_two(e.x * alpha, e.y * alpha), l2[1] = kc_two(f.x * alpha, f.y * alpha);
         m = m_new;
       }
-      const unsigned long long minus = kc_two(-m, -m);
+      // The difference first, then the scale: x scale - m scale in one operation leaves over what rounding m scale lost, which passes
+      // an exponent's range where scores are far out (from 2^31 on; fp16 queries and keys can reach 2^35).  2 % of a chunk.
+      const unsigned long long minus = kc_two(back, back);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float2 d = kc_split(kc_fma2(kc_two(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), scale2, minus));
+          const float2 d = kc_split(kc_mul2(kc_add2(kc_two(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), minus), scale2));
           const float p0 = kc_exp2(d.x), p1 = kc_exp2(d.y);
           l2[i & 1] = kc_add2(l2[i & 1], kc_two(p0, p1));
           p[i] = Pair16<T>::pack(p0, p1);
@@ -542,6 +545,7 @@ extern "C" int ronn_kv8_chunk_attention(const Kv8AttnCall* c, cudaStream_t strea
   const long rows = elems / c->head_dim;
   if (rows > 2147483647L || (units + 7) / 8 > 2147483647L) return -2;
   uint16_t *k = static_cast<uint16_t*>(c->scratch), *v = k + elems;
+  const float scale_log2 = c->scale * 1.4426950408889634f;
   CUtensorMap mq, mk, mv;
   int rc = make_tmap_2d(&mq, c->q, uint64_t(c->rows), uint64_t(c->heads) * c->head_dim, uint64_t(c->ld_q), KC_TILE, 64, 2);
   if (rc) return rc - 20;
@@ -557,7 +561,7 @@ extern "C" int ronn_kv8_chunk_attention(const Kv8AttnCall* c, cudaStream_t strea
                    c->kv_len + s0, k, v, c->out, c->status, c->table_ld, c->num_blocks, c->rows, c->ld_o,
                    c->bt_row ? c->table_rows : c->table_rows - s0, c->max_blocks, nb, padded, c->kv_heads, c->heads, c->max_q_len, c->causal,
                    c->heads / c->kv_heads % 2 == 0, c->causal && n <= KC_SORTED && long(n) * ((c->max_q_len + KC_TILE - 1) / KC_TILE) <= 65535 ? n : 0,
-                   c->scale * 1.4426950408889634f};
+                   scale_log2, fminf(8.f / scale_log2, 1e30f)};
     const dim3 grid{unsigned((units + 7) / 8), unsigned(n), 1u};
 #define RONN_KV8X(T, D, C) \
   do { \

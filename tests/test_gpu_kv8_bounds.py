@@ -117,3 +117,39 @@ def test_sequences_that_pass_their_bounds_are_left_out(form, heads, kvh, d, keys
     _reported(ops)
     assert bool((out[5:] == 9).all())
     _compare(out[:5], cache, q[:5], [table[0]] * 5, [keys - 4 + j for j in range(5)], heads, **_round("bf16", form))
+
+
+@pytest.mark.parametrize("form", ["direct", "expanded"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,query,code,scale", [("bf16", -1e16, 100, 2.0 ** 50), ("bf16", 1e16, 100, 2.0 ** 50), ("bf16", -1e13, 77, 2.0 ** 20),
+                                                    ("bf16", 3e4, 77, 2.0 ** 9), ("fp16", 60000, 63, 2.0 ** 10), ("fp16", -60000, 63, 2.0 ** 10)])
+def test_scores_of_any_magnitude_count(dtype, query, code, scale, form, causal):
+    """All of a row's scores alike, from 1e9 to 1e35 away from 0 on either side: the mean of the values it sees, as for scores
+    of 0, to the bit.  Equal keys give equal sums in any order, so that only differences of 0 are left."""
+    ops, d, n = _ops(), 64, 150
+    cache, table = _filled(20, 1, d, "int8", 241), _pages([300], 20, 242)
+    cache.k.fill_(code)
+    cache.k_scale.fill_(scale)
+    q = torch.full((n, d), query, dtype=DT[dtype], device="cuda")
+    out = ops.kv8_prefill_attention(q, 0, cache, table.cuda(), _i32([0]), _i32([n]), _i32([300]), n, 300, 1, causal, form=form)
+    zero = ops.kv8_prefill_attention(torch.zeros_like(q), 0, cache, table.cuda(), _i32([0]), _i32([n]), _i32([300]), n, 300, 1, causal, form=form)
+    assert torch.equal(out, zero) and bool((out != 0).any(1).all())
+    _compare(zero, cache, torch.zeros_like(q), [table[0]] * n, [300 - (n - 1 - j) if causal else 300 for j in range(n)], 1, **_round(dtype, form))
+    ops.check_status()
+
+
+@pytest.mark.parametrize("form", ["direct", "expanded"])
+def test_one_key_far_above_the_others(form):
+    """Scores some 1e11 apart: the value of the key that lies ahead, whether it comes first, last or in between."""
+    ops, d, n = _ops(), 64, 130
+    cache, table = _filled(40, 1, d, "int8", 251), _pages([600], 40, 252)
+    cache.k.fill_(-100)
+    cache.k_scale.fill_(2.0 ** 20)
+    q = torch.full((n, d), 1e3, dtype=torch.bfloat16, device="cuda")
+    for key in (0, 130, 299, 300, 599):
+        cache.k[int(table[0, key // 16]), 0, key % 16] = 100
+        out = ops.kv8_prefill_attention(q, 0, cache, table.cuda(), _i32([0]), _i32([n]), _i32([600]), n, 600, 1, False, form=form)
+        value = cache.v[int(table[0, key // 16]), 0, key % 16].float() * cache.v_scale[int(table[0, key // 16]), 0]
+        assert torch.equal(out.float(), value.expand(n, d))              # codes and scales are exact in bf16
+        cache.k[int(table[0, key // 16]), 0, key % 16] = -100
+    ops.check_status()
