@@ -74,11 +74,11 @@ __device__ __forceinline__ void kv8_unpack4(uint32_t w, float (&f)[4]) {
   f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
 }
 
-// Rotary embedding: the angle of pair j at position p is p * base^(-2j/d).  `turns[j]` is base^(-2j/d) / (2 pi) as a
-// 64-bit binary fraction, so p * turns[j] modulo 2^64 is the angle's fraction of a turn, exact to 2^-44 at p = 2^20 (a
-// 32-bit angle is off by 0.004 rad at p = 65536).  Sine and cosine are taken in 64 bits and the rotated value is formed to 44,
-// then rounded to 32 bits and to the activations' type, as a 64-bit tensor is converted: a value next to a rounding border
-// falls on the same side wherever it is computed.
+// Rotary embedding: the angle of pair j at position p is p * base^(-2j/d).  `turns[j]` is base^(-2j/d) / (2 pi) as the nearest
+// 64-bit binary fraction, so p * turns[j] modulo 2^64 is the angle's fraction of a turn, right to 2^-45 at p = 2^20 (a 32-bit
+// angle is off by 0.004 rad at p = 65536).  Sine and cosine are taken in 64 bits and the rotated value is formed to 44, then
+// rounded to 32 bits and to the activations' type, as a 64-bit tensor is converted: but for values within some 2^-40 of a
+// rounding border the result is the one that 64-bit arithmetic gives.
 constexpr int KV8_MAX_HALF = 64;
 struct Kv8Turns {
   unsigned long long t[KV8_MAX_HALF];

@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+from decimal import Decimal, localcontext
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -35,6 +36,7 @@ _APPEND_CALL = struct.Struct("=10Q4q8i")
 _READ_CALL = struct.Struct("=8Q2q4i")
 _ATTENTION_CALL = struct.Struct("=16Q6q13if")
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899862803482534211706798")
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
@@ -151,10 +153,13 @@ def _offset(what: str, off: int) -> None:
 
 @lru_cache(maxsize=64)
 def _turns(head_dim: int, base: float):
-    """base^(-2j/d) / (2 pi) for each channel pair, as 64-bit fractions of a turn: the array, which must live, and its address."""
+    """base^(-2j/d) / (2 pi) for each channel pair, as the nearest 64-bit fractions of a turn: the array, which must live, and its address."""
     if not (base > 0.0 and math.isfinite(base)):
         raise OperandError(f"rotary base must be a positive number, got {base}")
-    f = [int(base ** (-2.0 * j / head_dim) / (2.0 * math.pi) * 2.0 ** 64) & (2 ** 64 - 1) for j in range(head_dim // 2)]
+    with localcontext() as ctx:                              # 64 bits behind the point, and what stands in front of it where base < 1
+        ctx.prec = 40 + max(0, -math.floor(math.log10(base)))
+        log, unit = Decimal(base).ln(), 2 ** 64 / (2 * _PI)
+        f = [int(((log * (-2 * j) / head_dim).exp() * unit).to_integral_value()) & (2 ** 64 - 1) for j in range(head_dim // 2)]
     arr = (ctypes.c_ulonglong * len(f))(*f)
     return arr, ctypes.addressof(arr)
 

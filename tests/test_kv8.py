@@ -141,3 +141,32 @@ def test_tables_whose_keys_pass_32_bits_are_refused():
     wide = torch.empty(1, 2 ** 26 + 1, dtype=torch.int32)
     with pytest.raises(ops.OperandError, match="2\\^26"):
         ops.kv8_attention(_q(1), _cache(), wide, _i32([1]), 4, 16)
+
+
+@pytest.mark.parametrize("base", [10000.0, 500000.0, 1e6, 3.7, 1.0, 1e-30])
+@pytest.mark.parametrize("d", [64, 128])
+def test_rotary_turns_are_right_to_their_last_bit(base, d):
+    """base^(-2j/d) / (2 pi) as 64-bit fractions, against integers: d / 2 is a power of two, so the root is one of square roots,
+    and pi is Machin's sum."""
+    from fractions import Fraction
+    from ronn_b200.ops.kv8 import _turns
+    bits = 2000                                                      # base^-64 has fewer zeros behind the point
+
+    def inverse_tangent(x):
+        total = term = (1 << bits) // x
+        n = 1
+        while term:
+            term //= -x * x
+            n += 2
+            total += term // n
+            term = 0 if abs(term) <= 1 else term
+        return total
+    pi = 4 * (4 * inverse_tangent(5) - inverse_tangent(239))
+    for j, got in enumerate(_turns(d, base)[0]):
+        v = Fraction(base) ** -j
+        v = (v.numerator << bits) // v.denominator
+        for _ in range((d // 2).bit_length() - 1):
+            v = math.isqrt(v << bits)
+        want = (v << (bits + 64)) // (2 * pi)                        # in units of 2^-64, with `bits` behind the point
+        off = ((got << bits) - want) % (1 << (bits + 64))
+        assert min(off, (1 << (bits + 64)) - off) <= (1 << bits) * 51 // 100, (j, base)
