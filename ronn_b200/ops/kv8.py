@@ -120,6 +120,15 @@ def _rows16(what: str, t: torch.Tensor, cols: int, index: int, dtype: Optional[t
     return ld
 
 
+def _apart(at: int, ld: int, cols: int, at2: int, ld2: int, cols2: int, rows: int) -> bool:
+    """Whether two matrices of 16-bit values (address, row stride, columns) have no element in common.  Of two row strides, only
+    matrices that lie one behind the other count as apart."""
+    gap = (at2 - at) // 2
+    if gap >= (rows - 1) * ld + cols or -gap >= (rows - 1) * ld2 + cols2:
+        return True
+    return ld == ld2 and gap % ld >= cols and gap % ld + cols2 <= ld
+
+
 def _ints(what: str, t: torch.Tensor, n: int, index: int) -> int:
     """Address of n int32 values."""
     if t.dtype is not torch.int32 or t.get_device() != index or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
@@ -168,7 +177,8 @@ def kv8_append(qkv: torch.Tensor, k_off: int, v_off: int, slots: torch.Tensor, c
                positions: Optional[torch.Tensor] = None, rope_base: float = 0.0, rotated: Optional[torch.Tensor] = None) -> None:
     """Put the K and V columns of a fused QKV activation [tokens, ld] into their cache slots (int32 [tokens], -1: not cached).
     The tokens of one block stand in consecutive rows with rising slots, as a scheduler lists them.  With ``positions`` and
-    ``rope_base`` > 0, q and k are rotated first; the rotated columns go to ``rotated`` (laid out as qkv; default: qkv itself)."""
+    ``rope_base`` > 0, q and k are rotated first; the rotated columns go to ``rotated`` (laid out as qkv; default: qkv
+    itself, with which another buffer shares no element)."""
     d, kvh, index = cache.head_dim, cache.kv_heads, cache._index
     _heads(heads, cache)
     rope = positions is not None and rope_base > 0
@@ -183,11 +193,14 @@ def kv8_append(qkv: torch.Tensor, k_off: int, v_off: int, slots: torch.Tensor, c
         if k_off < heads * d:
             raise OperandError(f"k_off {k_off} lies inside the {heads} heads of q")
         to = qkv if rotated is None else rotated
-        if to.data_ptr() == qkv.data_ptr() and (v_off < heads * d or abs(v_off - k_off) < kvh * d):
-            raise OperandError(f"v_off {v_off} lies inside the columns that are rotated in place")
         ld_rot = _rows16("rotated", to, k_off + kvh * d, index, qkv.dtype)
         if to.shape[0] < tokens:
             raise OperandError(f"rotated has {to.shape[0]} rows for {tokens} tokens")
+        if to.data_ptr() == qkv.data_ptr() and (ld_rot == ld or tokens <= 1):
+            if v_off < heads * d or abs(v_off - k_off) < kvh * d:
+                raise OperandError(f"v_off {v_off} lies inside the columns that are rotated in place")
+        elif tokens and not _apart(qkv.data_ptr(), ld, max(k_off, v_off) + kvh * d, to.data_ptr(), ld_rot, k_off + kvh * d, tokens):
+            raise OperandError("rotated overlaps qkv; it is qkv itself, or apart from it")
         angles = _turns(d, float(rope_base))                 # kept while the launcher copies it
         rot, pos, turns = to.data_ptr(), _ints("positions", positions, tokens, index), angles[1]
 

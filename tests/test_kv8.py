@@ -170,3 +170,26 @@ def test_rotary_turns_are_right_to_their_last_bit(base, d):
         want = (v << (bits + 64)) // (2 * pi)                        # in units of 2^-64, with `bits` behind the point
         off = ((got << bits) - want) % (1 << (bits + 64))
         assert min(off, (1 << (bits + 64)) - off) <= (1 << bits) * 51 // 100, (j, base)
+
+
+def test_rotated_columns_that_overlap_the_activation_elsewhere_are_refused():
+    """In place, or apart: a shifted, a differently strided or a partly shared buffer would be read and written at once."""
+    c, slots = _cache(), _i32([0, 1, 2])
+    buf = torch.zeros(8, 24 * 64, dtype=torch.bfloat16)
+    qkv = buf[2:5, 8 * 64:16 * 64]
+    flat = buf.view(-1)
+    call = lambda rotated, qkv=qkv, n=3: ops.kv8_append(qkv, 4 * 64, 6 * 64, slots[:n], c, 4, slots[:n], 1e4, rotated)
+    at = (2 * 24 + 8) * 64                                           # where qkv starts
+    for rotated in (buf[1:4, 8 * 64:16 * 64], buf[3:6, 8 * 64:16 * 64], buf[2:5, 9 * 64:17 * 64], buf[2:5, 7 * 64:15 * 64], buf[2:5, 3 * 64:9 * 64 + 8],
+                    flat[at:at + 3 * 512].view(3, 512), flat[at - 512:at + 3 * 512 - 512].view(3, 512)):
+        with pytest.raises(ops.OperandError, match="overlap"):
+            call(rotated)
+    apart = (qkv, buf[2:5, :8 * 64], buf[2:5, 16 * 64:], buf[2:5, :6 * 64], buf[5:], _q(),
+             buf[2:5, 1 * 64:7 * 64], buf[3:6, 1 * 64:8 * 64])
+    for rotated in apart:
+        with pytest.raises(ops.OperandError, match="CUDA device"):  # right but for where it is
+            call(rotated)
+    with pytest.raises(ops.OperandError, match="CUDA device"):       # one row in place, whatever its stride
+        call(flat[at:at + 512].view(1, 512), qkv[:1], 1)
+    with pytest.raises(ops.OperandError, match="overlap"):
+        call(flat[at + 8:at + 520].view(1, 512), qkv[:1], 1)
