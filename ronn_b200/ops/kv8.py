@@ -230,13 +230,15 @@ def kv8_read(cache: KV8Cache, blocks: torch.Tensor, dtype: torch.dtype = torch.b
     return k, v
 
 
-def _out(out: Optional[torch.Tensor], q: torch.Tensor, rows: int, cols: int, index: int) -> int:
-    """Row stride of the result, 0 where it is still to be made."""
+def _out(out: Optional[torch.Tensor], q: torch.Tensor, q_off: int, ld_q: int, read: int, rows: int, cols: int, index: int) -> int:
+    """Row stride of the result, 0 where it is still to be made.  ``read``: columns of q from q_off on that the call reads."""
     if out is None:
         return 0
     ld = _rows16("out", out, cols, index, q.dtype)
     if out.shape[0] < rows:
         raise OperandError(f"out has {out.shape[0]} rows for {rows} of q")
+    if rows and not _apart(q.data_ptr() + 2 * q_off, ld_q, read, out.data_ptr(), ld, cols, rows):
+        raise OperandError("out overlaps the columns of q that are read")
     return ld
 
 
@@ -308,7 +310,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, 
         raise OperandError(f"max_ctx is {max_ctx}")
     if append is not None and heads // cache.kv_heads > _TILE:           # several tiles of a head's rows: one append before them
         factor = _scale(scale, d)
-        _out(out, q, rows, heads * d, index)
+        _out(out, q, 0, ld, cols, rows, heads * d, index)
         turned = None if rope is None else q.new_empty((rows, k_off + cache.kv_heads * d))
         kv8_append(q, k_off, v_off, slots, cache, heads, *((rope[0], float(rope[1]), turned) if rope is not None else ()))
         return kv8_attention(q if rope is None else turned, cache, block_tables, ctx_len, heads, max_ctx, bt_row, out, factor)
@@ -316,7 +318,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_tables: torch.Tensor, 
     def check():
         _run_check(_checks.paged_attention, q, cache.k, block_tables, ctx_len, heads, d, int(max_ctx), bt_row,
                    append[2] if append else None, rope[0] if rope else None)
-    return _attention("kv8_attention", cache, q, 0, ld, block_tables, table, at, 0, 0, ctx, out, _out(out, q, rows, heads * d, index), rows,
+    return _attention("kv8_attention", cache, q, 0, ld, block_tables, table, at, 0, 0, ctx, out, _out(out, q, 0, ld, cols, rows, heads * d, index), rows,
                       1, int(max_ctx), heads, 0, _scale(scale, d), check, **more)
 
 
@@ -327,8 +329,8 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
     """Attention of query chunks (chunked prompts, prefix hits): sequence s has ``q_len[s]`` queries from row ``seq_start[s]`` of q
     on ([tokens, ld], head h at column q_off + h * head_dim) and attends to the ``kv_len[s]`` keys that row ``bt_row[s]``
     (default s) of the block tables lists; with ``causal`` its queries are the last positions of that context, and a query in
-    front of the first key gives zeros.  The new tokens' K and V are in the cache already.  Returns [tokens, heads * head_dim];
-    rows that belong to no sequence are not written.  ``max_q_len`` bounds the queries of a sequence, ``max_kv_len`` (in
+    front of the first key gives zeros.  The new tokens' K and V are in the cache already.  Returns [tokens, heads * head_dim], in
+    ``out`` if given (which must not overlap these columns of q); rows that belong to no sequence are not written.  ``max_q_len`` bounds the queries of a sequence, ``max_kv_len`` (in
     whole cache blocks) its keys; a sequence that passes them or the rows of q is left out and reported, its rows are not written.
     Few queries read the codes as they are ("direct"); for many the contexts are expanded to 16-bit values first and the
     tensor-core attention runs over those ("expanded", for a positive scale; fp16 keeps values within its range, and probabilities
@@ -351,5 +353,5 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
         rows_of = bt_row if bt_row is not None else torch.arange(n_seq, device=q.device, dtype=torch.int32)
         _run_check(_checks.paged_attention, kv_len[:n_seq, None], cache.k, block_tables, kv_len, 0, 0, block_tables.shape[1] * _BLOCK, rows_of)
     return _attention("kv8_prefill_attention", cache, q, q_off, ld, block_tables, table, at, start, count, keys, out,
-                      _out(out, q, tokens, heads * d, index), n_seq, min(int(max_q_len), tokens), int(max_kv_len), heads, 1 if causal else 0,
+                      _out(out, q, q_off, ld, heads * d, tokens, heads * d, index), n_seq, min(int(max_q_len), tokens), int(max_kv_len), heads, 1 if causal else 0,
                       _scale(scale, d), check, form=form)

@@ -193,3 +193,22 @@ def test_rotated_columns_that_overlap_the_activation_elsewhere_are_refused():
         call(flat[at:at + 512].view(1, 512), qkv[:1], 1)
     with pytest.raises(ops.OperandError, match="overlap"):
         call(flat[at + 8:at + 520].view(1, 512), qkv[:1], 1)
+
+
+def test_results_that_overlap_the_queries_are_refused():
+    """Query heads are read by other CTAs than the one that writes a result over them."""
+    c, tab, three = _cache(), _i32([[0, 1, -1]] * 3), _i32([17, 3, 0])
+    buf = torch.zeros(8, 12 * 64, dtype=torch.bfloat16)
+    q = buf[2:5, :8 * 64]
+    row = lambda out, **kw: ops.kv8_attention(q, c, tab, three, 4, 32, out=out, **kw)
+    chunk = lambda out: ops.kv8_prefill_attention(q, 64, c, tab[:1], _i32([0]), _i32([3]), _i32([20]), 3, 20, 4, out=out)
+    append = dict(append=(4 * 64, 6 * 64, three))
+    for call, bad, good in ((row, (q, buf[1:4, 64:], buf[2:5, 3 * 64:]), (buf[2:5, 4 * 64:], buf[5:], buf[2:5, 8 * 64:])),
+                            (lambda out: row(out, **append), (q, buf[2:5, 4 * 64:]), (buf[2:5, 8 * 64:], buf[5:])),
+                            (chunk, (q, buf[2:5, 4 * 64:]), (buf[2:5, 5 * 64:], buf[2:5, 8 * 64:], buf[5:]))):
+        for out in bad:
+            with pytest.raises(ops.OperandError, match="overlap"):
+                call(out)
+        for out in good:
+            with pytest.raises(ops.OperandError, match="CUDA device"):
+                call(out)
