@@ -173,8 +173,7 @@ __device__ __forceinline__ void kv8_append_one(const Kv8AttnArgs& a, long row, i
 // Barrier of the warps that share an item.
 template <int WPI>
 __device__ __forceinline__ void kv8_item_sync(int item) {
-  if constexpr (WPI == 1) __syncwarp();
-  else if constexpr (WPI == KV8_NW) __syncthreads();
+  if constexpr (WPI == KV8_NW) __syncthreads();
   else asm volatile("bar.sync %0, %1;" ::"r"(item + 1), "n"(WPI * 32) : "memory");
 }
 
@@ -703,8 +702,7 @@ extern "C" int ronn_kv8_attention(const Kv8AttnCall* call, cudaStream_t stream) 
   const bool small = group_rows <= 8;
 #define RONN_KV8T(T, D, C, NT) \
   do { \
-    if (wpi == 1) RONN_KV8W(T, D, C, NT, 1); \
-    else if (wpi == 2) RONN_KV8W(T, D, C, NT, 2); \
+    if (wpi == 2) RONN_KV8W(T, D, C, NT, 2); \
     else RONN_KV8W(T, D, C, NT, 4); \
   } while (0)
 #define RONN_KV8W(T, D, C, NT, W) \

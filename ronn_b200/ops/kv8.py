@@ -330,8 +330,9 @@ def kv8_prefill_attention(q: torch.Tensor, q_off: int, cache: KV8Cache, block_ta
     on ([tokens, ld], head h at column q_off + h * head_dim) and attends to the ``kv_len[s]`` keys that row ``bt_row[s]``
     (default s) of the block tables lists; with ``causal`` its queries are the last positions of that context, and a query in
     front of the first key gives zeros.  The new tokens' K and V are in the cache already.  Returns [tokens, heads * head_dim], in
-    ``out`` if given (which must not overlap these columns of q); rows that belong to no sequence are not written.  ``max_q_len`` bounds the queries of a sequence, ``max_kv_len`` (in
-    whole cache blocks) its keys; a sequence that passes them or the rows of q is left out and reported, its rows are not written.
+    ``out`` if given (which must not overlap these columns of q); rows that belong to no sequence are not written.  ``max_q_len``
+    bounds the queries of a sequence, ``max_kv_len`` (in whole cache blocks) its keys; a sequence that passes them or the rows of q
+    is left out and reported, its rows are not written.
     Few queries read the codes as they are ("direct"); for many the contexts are expanded to 16-bit values first and the
     tensor-core attention runs over those ("expanded", for a positive scale; fp16 keeps values within its range, and probabilities
     in the activations' type).  ``form`` names one, for measurements."""
