@@ -291,8 +291,12 @@ def create_app(engine: LLMEngine, tokenizer=None, admission=None):
                         sent.extend(new)
                         full = tokenizer.decode(sent)            # decode the whole prefix: a character may span tokens
                         delta, text = full[len(text):], full
+                        r = loop.result(rid)
+                        more = {}
+                        if r is not None and r.output_logprobs is not None:
+                            more["logprobs"] = {"content": [_logprob(p) for p in r.output_logprobs[len(sent) - len(new):len(sent)]]}
                         chunk = {"id": rid, "object": "chat.completion.chunk",
-                                 "choices": [{"index": 0, "delta": {"content": delta}, "token_ids": new}]}
+                                 "choices": [{"index": 0, "delta": {"content": delta}, "token_ids": new, **more}]}
                         yield f"data: {json.dumps(chunk)}\n\n"
                     if done or adm.expired(ticket):
                         r = loop.result(rid)

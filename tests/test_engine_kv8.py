@@ -130,3 +130,26 @@ def test_completions_carry_log_probabilities(model):
                                                     "top_logprobs": 1}).json()["choices"][0]
         assert [p["token_id"] for p in chat["logprobs"]["content"]] == chat["token_ids"]
     app.state.loop.stop()
+
+
+def test_streamed_chat_carries_log_probabilities(model):
+    """Every chunk has those of its own tokens; a request that asks for none gets none."""
+    from ronn_b200.serving.tokenizer import load_tokenizer
+    eng = engine(model)
+    app = create_app(eng, load_tokenizer("bytes", eng.arch.vocab))
+    ask = {"messages": [{"role": "user", "content": "hi"}], "max_tokens": 9}
+    with TestClient(app) as c:
+        whole = c.post("/v1/chat/completions", json={**ask, "logprobs": True, "top_logprobs": 2}).json()["choices"][0]
+
+        def stream(**more):
+            with c.stream("POST", "/v1/chat/completions", json={**ask, **more, "stream": True}) as s:
+                return [json.loads(l[6:])["choices"][0] for l in s.iter_lines() if l.startswith("data: {")]
+        chunks = [x for x in stream(logprobs=True, top_logprobs=2) if "token_ids" in x]
+        assert [t for x in chunks for t in x["token_ids"]] == whole["token_ids"]
+        assert all([p["token_id"] for p in x["logprobs"]["content"]] == x["token_ids"] for x in chunks)
+        got = [p for x in chunks for p in x["logprobs"]["content"]]
+        assert [(p["rank"], [t["token_id"] for t in p["top_logprobs"]]) for p in got] == \
+            [(p["rank"], [t["token_id"] for t in p["top_logprobs"]]) for p in whole["logprobs"]["content"]]
+        assert all(abs(p["logprob"] - w["logprob"]) < 1e-4 for p, w in zip(got, whole["logprobs"]["content"]))
+        assert all("logprobs" not in x for x in stream())
+    app.state.loop.stop()
