@@ -141,14 +141,25 @@ class TorchOps:
 
     def token_logprobs(self, logits, tokens, top):
         from ..ops import TokenLogprobs
-        lp = torch.log_softmax(logits.float(), -1)
-        t = tokens.long()[:, None]
-        own = logits.gather(1, t)
-        ahead = (logits > own) | ((logits == own) & (torch.arange(logits.shape[1], device=logits.device)[None, :] < t))
+        x = logits.float()
+        rows, vocab = x.shape
+        m = x.amax(-1, keepdim=True)
+        empty = m == -math.inf                                            # no token has a probability
+        lp = torch.where(empty, m, torch.log_softmax(x, -1) + (m - m))    # NaN and +inf spoil the whole row
         p = lp.exp()
-        ids = torch.sort(logits, dim=1, descending=True, stable=True).indices[:, :top]
-        return TokenLogprobs(lp.gather(1, t)[:, 0], ahead.sum(1).to(torch.int32) + 1, -torch.where(p > 0, p * lp, torch.zeros_like(p)).sum(1),
-                             ids.to(torch.int32), lp.gather(1, ids))
+        entropy = -torch.where(p == 0, torch.zeros_like(p), p * lp).sum(1)
+        # NaN above all, in 64 bits, which have room above +inf of 32
+        order = torch.nan_to_num(x.double(), nan=1e301, posinf=1e300, neginf=-1e300)
+        ids = torch.sort(order, dim=1, descending=True, stable=True).indices[:, :top]
+        logprob, rank = torch.zeros_like(entropy), torch.zeros(rows, dtype=torch.int32, device=x.device)
+        if tokens is not None:
+            t = tokens.long()[:, None]
+            given, t = ((t >= 0) & (t < vocab))[:, 0], t.clamp(0, vocab - 1)
+            own = order.gather(1, t)
+            ahead = (order > own) | ((order == own) & (torch.arange(vocab, device=x.device)[None, :] < t))
+            logprob = torch.where(given, lp.gather(1, t)[:, 0], logprob)
+            rank = torch.where(given, ahead.sum(1).to(torch.int32) + 1, rank)
+        return TokenLogprobs(logprob, rank, entropy, ids.to(torch.int32), lp.gather(1, ids))
 
     def argmax(self, logits, col_offset=0, return_max=False):
         m, i = logits.float().max(dim=-1)

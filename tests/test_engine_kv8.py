@@ -153,3 +153,30 @@ def test_streamed_chat_carries_log_probabilities(model):
         assert all(abs(p["logprob"] - w["logprob"]) < 1e-4 for p, w in zip(got, whole["logprobs"]["content"]))
         assert all("logprobs" not in x for x in stream())
     app.state.loop.stop()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_library_backend_gives_log_probabilities_as_they_are_defined(dtype):
+    """Rows masked altogether, tokens that are none, NaN and +inf, equal logits: as the operator documents them."""
+    inf, nan = float("inf"), float("nan")
+    x = torch.zeros(9, 12)
+    x[0] = -inf
+    x[1, 3:] = -inf
+    x[2, 5] = nan
+    x[3, 7] = inf
+    x[4, [2, 9]] = 4.0
+    x[5, 2], x[5, 3] = nan, inf
+    x[6, 1], x[6, 2] = -0.0, 0.0
+    x[8] = torch.arange(12.0)
+    tokens = torch.tensor([4, 2, 5, 1, 9, 3, 2, 12, -1])
+    r = TorchOps().token_logprobs(x.to(dtype), tokens, 4)
+    assert r.logprob.dtype == r.entropy.dtype == r.top_logprobs.dtype == torch.float32 and r.rank.dtype == r.top_ids.dtype == torch.int32
+    assert r.rank.tolist() == [5, 3, 1, 3, 2, 2, 3, 0, 0]
+    assert r.top_ids.tolist() == [[0, 1, 2, 3], [0, 1, 2, 3], [5, 0, 1, 2], [7, 0, 1, 2], [2, 9, 0, 1], [2, 3, 0, 1], [0, 1, 2, 3], [0, 1, 2, 3], [11, 10, 9, 8]]
+    assert r.logprob[0] == -inf and r.entropy[0] == 0 and bool((r.top_logprobs[0] == -inf).all())
+    assert abs(float(r.logprob[1]) + 1.0986123) < 1e-6 and r.top_logprobs[1, 3] == -inf and abs(float(r.entropy[1]) - 1.0986123) < 1e-6
+    for row in (2, 3, 5):
+        assert torch.isnan(r.logprob[row]) and torch.isnan(r.entropy[row]) and bool(torch.isnan(r.top_logprobs[row]).all())
+    assert r.logprob[7] == 0 and r.logprob[8] == 0 and abs(float(r.entropy[7]) - 2.4849066) < 1e-6
+    none = TorchOps().token_logprobs(x.to(dtype), None, 4)
+    assert bool((none.logprob == 0).all() and (none.rank == 0).all()) and torch.equal(none.top_ids, r.top_ids)
