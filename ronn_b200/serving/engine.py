@@ -336,7 +336,7 @@ class LLMEngine:
                 self._status_host.copy_(status, non_blocking=True)
             if self.device.type == "cuda":
                 torch.cuda.current_stream().synchronize()
-            self.d2h_bytes_last = n_items * 4 + (16 if status is not None else 0)
+            self.d2h_bytes_last = n_items * 4 + (16 if status is not None else 0) + sum(t.nbytes for t in scores or ())
             if status is not None and int(self._status_host[0]) != 0:
                 self.runner.ops.check()                  # reads, clears and raises
         except Exception:

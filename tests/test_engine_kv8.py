@@ -180,3 +180,17 @@ def test_the_library_backend_gives_log_probabilities_as_they_are_defined(dtype):
     assert r.logprob[7] == 0 and r.logprob[8] == 0 and abs(float(r.entropy[7]) - 2.4849066) < 1e-6
     none = TorchOps().token_logprobs(x.to(dtype), None, 4)
     assert bool((none.logprob == 0).all() and (none.rank == 0).all()) and torch.equal(none.top_ids, r.top_ids)
+
+
+def test_bytes_to_the_host_count_the_log_probabilities(model):
+    """Token, log probability, rank and entropy of each request, and the alternatives that the step computed (2 asked for: 5)."""
+    eng = engine(model)
+    for n in (None, 2, 0):
+        eng.add_request([1, 2, 3], SamplingParams(max_new_tokens=4, logprobs=n))
+    for _ in range(2):                                               # the prompts, then a decode step
+        eng.step()
+        assert eng.d2h_bytes_last == 3 * (4 + 12 + 5 * 8)
+    plain = engine(model)
+    plain.add_request([1, 2, 3], SamplingParams(max_new_tokens=4))
+    plain.step()
+    assert plain.d2h_bytes_last == 4
