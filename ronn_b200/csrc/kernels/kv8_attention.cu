@@ -17,11 +17,12 @@
 //                 interleaves the bytes of two.
 // Queries as B waste nothing on a decode step's missing rows: 8 products a block of 64 channels, not 12.
 // The 16-byte pieces of a row stand in the ring in an order that depends on the row (Kv8Ring), so that neither read meets a
-// bank twice.  256 rows of 64 to 768 keys, 16 heads of 64 in int8, took 76 us with the blocks in registers (48 of them, and not
-// enough left), 76 with the ring and 80 registers a thread, 61 with the ring and 128: 16 warps an SM without spills beat 24
-// with.  54 us of the 61 are this kernel: it issues in 59 % of its cycles, about 180 instructions a block (a third of them turn
-// int8 into f16; e4m3 takes one for two codes) and 1100 a warp around them, and the longest rows are alone at the end.  Long
-// contexts of e4m3 go by at 5 TB/s.
+// bank twice.  With the blocks in registers (48 of them, and not enough left) or the ring and 80 registers a thread, 256 rows of 64
+// to 768 keys, 16 heads of 64 in int8, took a quarter longer than with the ring and 128: 16 warps an SM without spills beat 24
+// with.  They take 53 us, 4.2 TB/s of codes, and nothing is full: issue slots 58 %, ALU 50 %, DRAM 53 %, with 3.6 warps a scheduler
+// to hide what each waits for.  An SM is idle for 12 % of the time on average, as the longest rows are alone at the end.  A block
+// takes about 180 instructions (a third of them turn int8 into f16; e4m3 takes one for two codes), and a warp 1100 around its
+// blocks.  Long contexts of e4m3 go by at 5 TB/s.
 // Codes become f16 exactly.  Q in bf16 is scaled by a power of two for each row, so that it fits f16 (its 8 significant bits
 // do; what is 2^-34 of the row's largest is lost).  Softmax statistics, sums and O are in 32 bits; P is rounded to f16 as
 // 2^15 p, by at most 2^-11 of it or 2^-40.  The scale of a K block multiplies its scores, that of a V block its P,

@@ -8,10 +8,12 @@
 //               each tile, whose first 64 become P (16-bit pairs), and O has D.  S of the next keys waits for that product.
 //   warps 2-9   four a tile, one query row a thread: the row of S in registers, maximum, exponentials, sum, P back.  O stays in
 //               tensor memory and is rescaled only when a row's maximum has grown by more than 2^8.
-// Statistics and O are in 32 bits; P is rounded to the activations' type, by half a step.
+// Statistics and O are in 32 bits.  P is rounded to the activations' type, by half a step: both operands of a product have one type,
+// and bf16 holds any value of the cache where fp16 would not.  That adds a quarter to the error of bf16 results (0.0021 of the
+// result's norm against 0.0017 with P in 32 bits, three chunks of 763 to 1024 queries over 1793 to 5024 keys).
 // A step of 128 keys is a chain of softmax (1800 cycles, 1024 of them a warp's exponentials), P V and the next Q K^T (750 each);
 // two tiles overlap theirs, so that neither the tensor pipe (46 % of a causal chunk) nor the exponentials are full.  2 x 4096
-// queries over 4096 keys, 32 / 8 heads of 128, without a mask: 510 us, 1078 TFLOP/s.  674 us with instructions issued from a lane
+// queries over 4096 keys, 32 / 8 heads of 128, without a mask: 514 us, 1069 TFLOP/s.  674 us with instructions issued from a lane
 // of its own; an issuer that looked for whichever tile could go on was slower still (3 chunks of 763 to 1024 queries: 230 us
 // against 191 for taking the tiles in turn).
 #include "kv8.cuh"
@@ -236,7 +238,7 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   // With a causal mask the items differ in their keys: the longest first.  Three sequences of 763 to 1024 queries over 1793 to
-  // 5024 keys, 336 CTAs of 9 to 40 steps, take 176 us, and 187 in the order of the grid.
+  // 5024 keys, 336 CTAs of 9 to 40 steps, take 174 us, and 185 in the order of the grid.
   int seq = blockIdx.y, z = int(gridDim.z) - 1 - int(blockIdx.z);
   if (a.sorted && !kv8_chunk_item(a, a.sorted, a.pair_heads ? KC_TILE : 2 * KC_TILE, blockIdx.y, seq, z)) return;
   Kv8Chunk s;
@@ -423,7 +425,8 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         m = m_new;
       }
       // The difference first, then the scale: x scale - m scale in one operation leaves over what rounding m scale lost, which passes
-      // an exponent's range where scores are far out (from 2^31 on; fp16 queries and keys can reach 2^35).  2 % of a chunk.
+      // an exponent's range where scores are far out (from 2^31 on; fp16 queries and keys can reach 2^35).  One operation more for two
+      // scores: 514 us against 510 at 2 x 4096 queries with heads of 128, 260 against 252 with 16 heads of 64.
       const unsigned long long minus = kc_two(back, back);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {

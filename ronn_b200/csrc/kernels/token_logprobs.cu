@@ -15,7 +15,7 @@
 // The best tokens of a share: the top-th best of its threads' maxima bounds them from below, so no more threads than that
 // (and a few) hold any; those threads' vectors are read again, from the L2 cache, and a candidate's rank is the number of
 // its betters.  Where that leaves more candidates than there is room for, the best are taken one by one.
-// 4662 x 50257 bf16 take 117 us, 4.0 TB/s, at 13 instructions a logit: issue slots bound it, three quarters of them taken.  Two
+// 4662 x 50257 bf16 take 116 us, 4.0 TB/s, at 13 instructions a logit: issue slots bound it, three quarters of them taken.  Two
 // floats an instruction, counting in pairs of 16 bits and vectors without edges brought it there from 362 us with a row's
 // logits held in registers and every pass over them.
 #include "common.cuh"
